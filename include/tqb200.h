@@ -384,6 +384,87 @@ int tq_prefill_sdpa(const void* q, const void* k, const void* v, void* out, int 
                     int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
                     int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
                     float attn_scale, int causal, int* status, void* stream);
+/* The same with a sliding window and sink tokens (causal only; window 0: none): query row i sees keys
+ * j <= i + (seq_k - seq_q) with j > i + (seq_k - seq_q) - window or j < sinks.  Key tiles that no row of a query tile
+ * sees are neither read nor computed, so the time follows the window, not the sequence.  No reference counterpart
+ * (its mask helpers build such masks as arrays, cache.py:311-334). */
+int tq_prefill_sdpa_window(const void* q, const void* k, const void* v, void* out, int dtype, int batch,
+                           int n_q_heads, int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim,
+                           int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
+                           int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
+                           int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
+                           int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
+                           float attn_scale, int causal, int64_t window, int64_t sinks, int* status, void* stream);
+
+/* ---- paged caches ------------------------------------------------------------
+ * No reference counterpart (its caches are one array per layer).  A pool keeps the
+ * K / V rows of many sequences in pages of `page_size` positions (a power of two, 32
+ * at least) for every kv head, all heads of a page side by side; page_table[b][i] is
+ * the pool page of positions [i * page_size, (i + 1) * page_size) of sequence b.  Rows
+ * have the layout of the contiguous caches.  Pages may be shared between sequences;
+ * entries behind a sequence, or wholly outside its window, are never read.  Lengths
+ * and tables live on the device and are read when a kernel runs, so a captured step can
+ * be replayed while they advance.  A page id outside the pool (or a position behind the
+ * table) is never followed: an insert skips the row, a decode output row or a row read
+ * back becomes NaN, and tq_paged_status reports it. */
+typedef struct tq_paged_half {   /* the keys or the values of a pool */
+  int32_t format;                /* TQ_KV_POLAR or TQ_KV_DENSE */
+  int32_t bits, dtype;           /* code width (polar); element type (dense) */
+  int32_t rows_dtype;
+  void* data;                    /* polar: uint32 words, dense: elements, rows of one (page, head) contiguous */
+  float* norms;                  /* polar only */
+  int64_t page_stride, head_stride;                 /* in units of data's element type */
+  int64_t norm_page_stride, norm_head_stride;
+  const float* centroids_host;   /* reading */
+  const float* boundaries_host;  /* inserting */
+  const float* signs_host;
+  const void* rows;              /* tq_paged_append: new rows (batch, heads, tokens, dim) */
+  int64_t rows_batch_stride, rows_head_stride, rows_token_stride;
+} tq_paged_half;
+
+typedef struct tq_paged_params {
+  int32_t struct_bytes;          /* sizeof(tq_paged_params) */
+  int32_t batch, n_q_heads, n_kv_heads, dim, page_size;
+  int64_t n_pages;               /* pages of the pool */
+  const int32_t* page_table;     /* (batch, table_width) */
+  int64_t table_stride;
+  const int32_t* seq_lens;       /* (batch): decode / dequantize: positions; append: position of the first new token */
+  const int32_t* counts;         /* append, optional (batch): new tokens per sequence, at most `tokens` */
+  int64_t tokens;                /* append: tokens of `rows`; dequantize: positions of the output */
+  int32_t table_width;
+  int32_t q_dtype, out_dtype;
+  float attn_scale;
+  int32_t window, sinks;         /* decode: the newest token sees positions >= len - window and < sinks; window 0: all */
+  const void* q;                 /* (batch, n_q_heads, dim) */
+  int64_t q_batch_stride, q_head_stride;
+  void* out;
+  int64_t out_batch_stride, out_head_stride;
+  void* workspace;               /* decode: tq_paged_decode_workspace_bytes(dim), 16-byte aligned, contents irrelevant */
+  int64_t workspace_bytes;
+  void* stream;
+  tq_paged_half k, v;            /* dequantize reads `v` */
+} tq_paged_params;
+
+/* Stores token t < counts[b] of sequence b at position seq_lens[b] + t: packed halves are
+ * quantized with tq_quantize's arithmetic (the same words), dense halves copied. */
+int tq_paged_append(const tq_paged_params* p);
+/* One query token per sequence (the last of seq_lens[b] positions) over the pages; a
+ * sequence of length 0 gives zeros.  The workspace holds nothing between calls; calls
+ * that may overlap need one each. */
+int64_t tq_paged_decode_workspace_bytes(int dim);
+int tq_paged_decode(const tq_paged_params* p);
+/* Positions [0, tokens) of every sequence as dense rows (batch, heads, tokens, dim), contiguous;
+ * rows at and behind seq_lens[b] are zero.  tq_dequantize's arithmetic (the same bits). */
+int tq_paged_dequantize(const tq_paged_params* p);
+/* Copies page src[i] to page dst[i] in each of n_pools arrays of n_pages pages (page_bytes[j]
+ * bytes per page, multiples of 16, 16-byte aligned).  src / dst are device arrays; no page may be
+ * written twice, or read and written, by one call. */
+int tq_copy_pages(void* const* pools, const int64_t* page_bytes, int n_pools, int64_t n_pages, const int32_t* src,
+                  const int32_t* dst, int64_t n_pairs, void* stream);
+/* What the paged kernels of the current device found wrong since the last call (synchronises the
+ * stream; resets the word): 0 nothing, 1 a page id outside the pool, 2 a position behind the
+ * page table, 3 a bounded wait that gave up. */
+int tq_paged_status(int* status, void* stream);
 
 /* Peer-to-peer exchange of a block between the GPUs of one node (sequence-sharded
  * decode: the per-rank (m, l, acc) partial states that tq_merge_partials combines).

@@ -24,6 +24,7 @@ from .kernels import (
     MergePlan,
     prefill_attention,
 )
+from .paged import paged_append, paged_decode, paged_dequantize, copy_pages, paged_status
 from .fused_attention import turboquant_attention
 from .packing import pack_indices, unpack_indices, packed_dim
 from .rotation import (

@@ -71,6 +71,37 @@ class FlashParams(ctypes.Structure):
     ]
 
 
+class PagedHalf(ctypes.Structure):
+    """Mirror of `tq_paged_half` (include/tqb200.h)."""
+
+    _fields_ = [
+        ("format", c_int32), ("bits", c_int32), ("dtype", c_int32), ("rows_dtype", c_int32),
+        ("data", c_void_p), ("norms", c_void_p),
+        ("page_stride", c_int64), ("head_stride", c_int64),
+        ("norm_page_stride", c_int64), ("norm_head_stride", c_int64),
+        ("centroids_host", POINTER(c_float)), ("boundaries_host", POINTER(c_float)), ("signs_host", POINTER(c_float)),
+        ("rows", c_void_p),
+        ("rows_batch_stride", c_int64), ("rows_head_stride", c_int64), ("rows_token_stride", c_int64),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    """Mirror of `tq_paged_params` (include/tqb200.h)."""
+
+    _fields_ = [
+        ("struct_bytes", c_int32),
+        ("batch", c_int32), ("n_q_heads", c_int32), ("n_kv_heads", c_int32), ("dim", c_int32), ("page_size", c_int32),
+        ("n_pages", c_int64), ("page_table", c_void_p), ("table_stride", c_int64),
+        ("seq_lens", c_void_p), ("counts", c_void_p), ("tokens", c_int64),
+        ("table_width", c_int32), ("q_dtype", c_int32), ("out_dtype", c_int32), ("attn_scale", c_float),
+        ("window", c_int32), ("sinks", c_int32),
+        ("q", c_void_p), ("q_batch_stride", c_int64), ("q_head_stride", c_int64),
+        ("out", c_void_p), ("out_batch_stride", c_int64), ("out_head_stride", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64), ("stream", c_void_p),
+        ("k", PagedHalf), ("v", PagedHalf),
+    ]
+
+
 _lib = None
 
 _FP = POINTER(c_float)
@@ -119,6 +150,15 @@ _SIGNATURES = {
     "tq_set_peer_wait_limit_ms": (c_int, [c_int]),
     "tq_peer_push": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p), c_int, c_uint32, c_void_p]),
     "tq_peer_wait": (c_int, [c_void_p, c_int, c_uint32, c_void_p, c_void_p]),
+    "tq_paged_append": (c_int, [POINTER(PagedParams)]),
+    "tq_paged_decode_workspace_bytes": (c_int64, [c_int]),
+    "tq_paged_decode": (c_int, [POINTER(PagedParams)]),
+    "tq_paged_dequantize": (c_int, [POINTER(PagedParams)]),
+    "tq_copy_pages": (c_int, [POINTER(c_void_p), POINTER(c_int64), c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "tq_paged_status": (c_int, [POINTER(c_int), c_void_p]),
+    "tq_prefill_sdpa_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                       c_int64, c_int64, c_int] + [c_int64] * 12
+                               + [c_float, c_int, c_int64, c_int64, c_void_p, c_void_p]),
     "tq_prefill_sdpa": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                 c_int64, c_int64, c_int] + [c_int64] * 12 + [c_float, c_int, c_void_p, c_void_p]),
 }

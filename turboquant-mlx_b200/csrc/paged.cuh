@@ -1,0 +1,220 @@
+// Paged caches: argument blocks, and how the decode kernels share out their work.
+//
+// A pool holds pages of `page` positions for every kv head; page_table[b][i] names the pool page of
+// positions [i * page, (i + 1) * page) of sequence b.  Pages may be anywhere in the pool and may be shared
+// between sequences (forks), so nothing here assumes an order.
+//
+// The unit of decode work is a tile: 32 consecutive positions of one (sequence, kv head, group of up to 8
+// query heads), which never straddles a page (page sizes are powers of two, 32 at least).  A sequence has
+// only the tiles that its newest token sees: all of them, or with a sliding window the tiles of the first
+// `sinks` positions and those from position len - window on.  The tiles of a launch, numbered sequence by
+// sequence, group by group, are cut into equal runs, one per CTA, whatever the lengths of the sequences:
+// a ragged batch loads every SM alike, and a single long sequence is split as finely as it needs.  A CTA
+// that holds all tiles of a group writes its output; otherwise it leaves a partial state (m, l, acc) in
+// one of its two slots of the workspace, which the merge kernel joins.
+#pragma once
+
+#include "common.cuh"
+
+namespace tq {
+
+constexpr int kPagedTile = 32;       // positions per tile
+constexpr int kPagedRows = 8;        // query heads per group
+constexpr int kPlanEntries = 1024;   // prefix entries of a CTA's plan (each covers ceil(batch / 1024) sequences)
+constexpr float kPagedLog2e = 1.4426950408889634f;
+
+struct PagedHalf {                   // the K or the V half of a pool
+  int format, bits, dtype;           // tq_kv_format; code width; element type of dense rows
+  void* data;                        // packed words or dense rows, rows of one (page, head) contiguous
+  float* norms;                      // packed rows only
+  int64_t page_stride, head_stride;              // in 32-bit words (packed) or elements (dense)
+  int64_t norm_page_stride, norm_head_stride;
+  Table16 cent;
+  SignMask signs;
+};
+
+struct PageView {
+  const int* table;
+  int64_t table_stride;
+  int table_width, page_shift;
+  int64_t n_pages;
+  int* status;                       // set when a page id lies outside the pool
+
+  __device__ __forceinline__ int capacity() const {
+    const int64_t c = (int64_t)table_width << page_shift;
+    return c > 0x7fffffe0 ? 0x7fffffe0 : (int)c;
+  }
+  // Pool page of position `pos` of sequence b, -1 when the table names none in the pool.
+  __device__ __forceinline__ int page_of(int b, int pos) const {
+    const int id = __ldg(table + b * table_stride + (pos >> page_shift));
+    return id >= 0 && id < n_pages ? id : -1;
+  }
+};
+
+struct PagedDecodeArgs {
+  PagedHalf k, v;
+  PageView view;
+  int batch, n_q_heads, n_kv_heads, n_rep, groups;     // groups = n_kv_heads * ceil(n_rep / 8)
+  const int* lens;
+  int window, sinks;                 // window 0: every position is visible
+  const void* q;
+  int q_dtype, out_dtype;
+  int64_t q_batch_stride, q_head_stride;
+  void* out;
+  int64_t out_batch_stride, out_head_stride;
+  float scale_log2;                  // attn_scale * log2(e)
+  float* part;                       // [2 * ctas][8][dim + 2]: acc (rotated domain), m (log2 domain), l
+  int ctas, min_tiles;               // grid of the main kernel; fewest tiles worth a CTA
+};
+
+#ifdef __CUDACC__
+// What the newest token of a sequence sees.
+struct SeqSpan {
+  int n;        // positions
+  int lo;       // positions below lo are visible only as sinks
+  int st, wt;   // tiles of the sinks; first tile behind them
+  int tiles;
+  __device__ __forceinline__ int tile_at(int j) const { return j < st ? j : j - st + wt; }
+  __device__ __forceinline__ bool sees(int pos, int sinks) const { return pos < n && (pos >= lo || pos < sinks); }
+};
+
+__device__ __forceinline__ SeqSpan span_of(const PagedDecodeArgs& a, int b) {
+  SeqSpan s;
+  s.n = min(max(__ldg(a.lens + b), 0), a.view.capacity());
+  s.lo = a.window > 0 ? max(0, s.n - a.window) : 0;
+  const int full = (s.n + kPagedTile - 1) / kPagedTile;
+  s.st = s.lo > 0 ? (int)min(((int64_t)a.sinks + kPagedTile - 1) / kPagedTile, (int64_t)full) : 0;
+  s.wt = max(s.lo / kPagedTile, s.st);
+  s.tiles = s.st + full - s.wt;
+  return s;
+}
+
+// prefix[e] = tiles of one group in the sequences in front of entry e, prefix[n] = of all sequences.
+// Called by every thread of the block; `prefix` holds kPlanEntries + 1 ints.
+__device__ __forceinline__ void plan_tiles(const PagedDecodeArgs& a, int* prefix) {
+  const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
+  const int n = (a.batch + per - 1) / per;
+  for (int e = threadIdx.x; e < n; e += blockDim.x) {
+    int t = 0;
+    for (int b = e * per; b < min(a.batch, (e + 1) * per); ++b) t += span_of(a, b).tiles;
+    prefix[e + 1] = t;
+  }
+  if (threadIdx.x == 0) prefix[0] = 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int carry = 0;
+    for (int e0 = 1; e0 <= n; e0 += 32) {
+      const int e = e0 + threadIdx.x;
+      int t = e <= n ? prefix[e] : 0;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, t, k);
+        if ((int)threadIdx.x >= k) t += o;
+      }
+      t += carry;
+      if (e <= n) prefix[e] = t;
+      carry = __shfl_sync(0xffffffffu, t, 31);
+    }
+  }
+  __syncthreads();
+}
+
+struct Plan {
+  int64_t total;       // tiles of the launch
+  int ctas;            // CTAs that get any
+  __device__ __forceinline__ int64_t begin(int cta) const { return total * cta / ctas; }
+  // the CTA whose run holds tile t
+  __device__ __forceinline__ int owner(int64_t t) const {
+    int c = (int)(t * ctas / total);
+    while (begin(c + 1) <= t) ++c;
+    while (begin(c) > t) --c;
+    return c;
+  }
+};
+__device__ __forceinline__ int plan_entries(const PagedDecodeArgs& a) {
+  const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
+  return (a.batch + per - 1) / per;
+}
+__device__ __forceinline__ Plan make_paged_plan(const PagedDecodeArgs& a, const int* prefix) {
+  Plan p;
+  p.total = (int64_t)prefix[plan_entries(a)] * a.groups;
+  const int64_t want = (p.total + a.min_tiles - 1) / a.min_tiles;
+  p.ctas = (int)max((int64_t)1, min((int64_t)a.ctas, want));
+  return p;
+}
+// Tiles of one group in the sequences in front of sequence b.
+__device__ __forceinline__ int tiles_before(const PagedDecodeArgs& a, const int* prefix, int b) {
+  const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
+  int t = prefix[b / per];
+  for (int i = b / per * per; i < b; ++i) t += span_of(a, i).tiles;
+  return t;
+}
+
+// Walks the tiles of a run in order.
+struct Cursor {
+  int b, group, j;     // sequence, (kv head, row group), tile inside the group
+  SeqSpan span;
+  __device__ __forceinline__ void seek(const PagedDecodeArgs& a, const int* prefix, int64_t t) {
+    const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
+    int lo = 0, hi = plan_entries(a) - 1;          // last entry whose first tile is not behind t
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if ((int64_t)prefix[mid] * a.groups <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    int64_t rest = t - (int64_t)prefix[lo] * a.groups;
+    b = lo * per;
+    span = span_of(a, b);
+    while (rest >= (int64_t)span.tiles * a.groups && b + 1 < a.batch) {
+      rest -= (int64_t)span.tiles * a.groups;
+      span = span_of(a, ++b);
+    }
+    group = span.tiles > 0 ? (int)(rest / span.tiles) : 0;
+    j = span.tiles > 0 ? (int)(rest % span.tiles) : 0;
+  }
+  // to the first tile of the next group that has any
+  __device__ __forceinline__ void next_group(const PagedDecodeArgs& a) {
+    j = 0;
+    if (++group < a.groups) return;
+    group = 0;
+    do {
+      if (++b >= a.batch) return;
+      span = span_of(a, b);
+    } while (span.tiles == 0);
+  }
+};
+
+__device__ __forceinline__ float paged_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float load_elem(const void* base, int dtype, int64_t i) {
+  return dtype == TQ_F32 ? reinterpret_cast<const float*>(base)[i]
+         : dtype == TQ_F16 ? __half2float(reinterpret_cast<const __half*>(base)[i])
+                           : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
+}
+__device__ __forceinline__ void store_elem(void* base, int dtype, int64_t i, float x) {
+  if (dtype == TQ_F32) reinterpret_cast<float*>(base)[i] = x;
+  else if (dtype == TQ_F16) reinterpret_cast<__half*>(base)[i] = __float2half_rn(x);
+  else reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
+}
+
+// Output row of one query head, held by one warp (lane = EPL consecutive elements of the rotated
+// accumulator): signs * butterfly(acc) / dim / l.  A row that saw nothing (l == 0) is zero.
+template <int EPL>
+__device__ __forceinline__ void finish_row(const PagedDecodeArgs& a, int b, int head, float (&v)[EPL], float l, int lane) {
+  warp_butterfly<EPL>(v, lane);
+  const float inv = l == 0.f ? 0.f : 1.0f / (l * (EPL * 32));
+  const int64_t off = b * a.out_batch_stride + head * a.out_head_stride + lane * EPL;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j)
+    store_elem(a.out, a.out_dtype, off + j, l == 0.f ? 0.f : v[j] * sign_at(a.v.signs, lane * EPL + j) * inv);
+}
+#endif  // __CUDACC__
+
+int launch_paged_merge(const PagedDecodeArgs& a, int dim, cudaStream_t st);
+bool paged_mma_supported(const PagedDecodeArgs& a, int dim);
+int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st);
+
+}  // namespace tq

@@ -22,6 +22,10 @@
 //     loads, masks and reduces its scores, and the tensor core works meanwhile
 //     on the products of the surrounding tiles.  O is rescaled lazily (only when
 //     a row maximum grows by more than 2^8) by the group that sees the growth.
+//   * A sliding window with sinks (tq_prefill_sdpa_window) is the same kernel over a shorter list of key tiles: those
+//     of the sinks, then those from the window of the tile's first row to its diagonal.  Tiles that the window's
+//     edge, the sinks' end or the diagonal crosses are masked per row; a row whose first tiles are masked whole keeps
+//     m = -inf and its P at zero until it sees a key.  The full form is compiled without any of it.
 //   * Every wait is bounded; a wait that gives up sets the status word, the CTA
 //     drains its copies, frees its tensor memory and returns.
 #include <cuda.h>
@@ -68,6 +72,7 @@ struct PrefillArgs {
   void* out;
   int64_t o_batch_stride, o_head_stride, o_row_stride;   // elements
   int seq_q, seq_k, n_rep, causal, bf16;
+  int window, sinks;             // windowed kernel: row i sees keys > i + off - window and keys < sinks
   float scale_log2;
   int* status;
 };
@@ -192,6 +197,7 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
 enum : int { B_Q = 0, B_K_FULL = 1, B_K_EMPTY = 4, B_V_FULL = 7, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 14,
              B_PV_DONE = 17 /* 2: by tile parity */, B_ALL_DONE = 19, B_MBOX = 20 /* 8: [row group][tile parity] */ };
 
+template <bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v, const PrefillArgs a) {
@@ -206,7 +212,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const int off = a.seq_k - a.seq_q;                           // key index of query row 0's diagonal
   // keys this tile can see: [0, k_end)
   const int k_end = a.causal ? min(a.seq_k, q0 + kBM + off) : a.seq_k;
-  const int n_tiles = (k_end + kBN - 1) / kBN;
+  // windowed: tiles of the sinks, then those from the window of the tile's first row on (tile 0 .. first - 1 hidden)
+  const int first = WINDOW ? (int)(max((int64_t)0, (int64_t)q0 + off - a.window + 1) / kBN) : 0;
+  const int sink_tiles = WINDOW ? min((min(a.sinks, a.seq_k) + kBN - 1) / kBN, first) : 0;
+  const int n_tiles = (k_end + kBN - 1) / kBN - first + sink_tiles;
+  auto key0 = [&](int j) { return (!WINDOW || j < sink_tiles ? j : j - sink_tiles + first) * kBN; };   // first key of the j-th tile
   auto bar = [&](int i) { return sbase + Smem::bars + 8u * i; };
   auto wait = [&](uint32_t b, uint32_t parity) { return mbar_wait(b, parity, a.status); };
 
@@ -253,8 +263,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         if (j >= kKStages && !wait(bar(B_K_EMPTY + s), ((j / kKStages) - 1) & 1)) return false;
         const uint32_t dst = sbase + Smem::k0 + s * kTileBytes;
         mbar_expect_tx(bar(B_K_FULL + s), kTileBytes);
-        tma_load_4d(dst, &map_k, 0, j * kBN, kv_head, batch, bar(B_K_FULL + s));
-        tma_load_4d(dst + kHalfBytes, &map_k, 64, j * kBN, kv_head, batch, bar(B_K_FULL + s));
+        tma_load_4d(dst, &map_k, 0, key0(j), kv_head, batch, bar(B_K_FULL + s));
+        tma_load_4d(dst + kHalfBytes, &map_k, 64, key0(j), kv_head, batch, bar(B_K_FULL + s));
         return true;
       };
       auto load_v = [&](int j) {
@@ -262,8 +272,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         if (j >= kVStages && !wait(bar(B_V_EMPTY + s), ((j / kVStages) - 1) & 1)) return false;
         const uint32_t dst = sbase + Smem::v0 + s * kTileBytes;
         mbar_expect_tx(bar(B_V_FULL + s), kTileBytes);
-        tma_load_4d(dst, &map_v, 0, j * kBN, kv_head, batch, bar(B_V_FULL + s));
-        tma_load_4d(dst + kHalfBytes, &map_v, 64, j * kBN, kv_head, batch, bar(B_V_FULL + s));
+        tma_load_4d(dst, &map_v, 0, key0(j), kv_head, batch, bar(B_V_FULL + s));
+        tma_load_4d(dst + kHalfBytes, &map_v, 64, key0(j), kv_head, batch, bar(B_V_FULL + s));
         return true;
       };
       // K runs ahead of V: the scores are computed up to three tiles ahead of the softmax
@@ -361,9 +371,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       tmem_ld32(src, v[0]);
       tmem_ld32(src + 32, v[1]);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      const bool need_mask = (j * kBN + kBN - 1 > (a.causal ? q0 + off : a.seq_k - 1)) || (j * kBN + kBN > a.seq_k);
+      const int k0 = key0(j);
+      const bool need_mask = (k0 + kBN - 1 > (a.causal ? q0 + off : a.seq_k - 1)) || (k0 + kBN > a.seq_k);
+      if (WINDOW && k0 <= q0 + off + kBM - 1 - a.window && k0 + kBN > a.sinks) {
+        // the window of the tile's last row starts inside or behind this key tile, and not all of it are sinks:
+        // columns in [slim, wlo) are hidden
+        const int slim = a.sinks - (k0 + h * 64), wlo = kmax - a.window + 1 - (k0 + h * 64);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i >= slim && c * 32 + i < wlo) v[c][i] = 0xff800000u;
+      }
       if (need_mask) {
-        const int klim = min(kmax, a.seq_k - 1) - (j * kBN + h * 64);     // columns <= klim are visible
+        const int klim = min(kmax, a.seq_k - 1) - (k0 + h * 64);     // columns <= klim are visible
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -562,14 +583,18 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 }  // namespace tq
 
-extern "C" int tq_prefill_sdpa(const void* q, const void* k, const void* v, void* out, int dtype, int batch,
-                               int n_q_heads, int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim,
-                               int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
-                               int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
-                               int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
-                               int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
-                               float attn_scale, int causal, int* status, void* stream) {
+extern "C" int tq_prefill_sdpa_window(const void* q, const void* k, const void* v, void* out, int dtype, int batch,
+                                      int n_q_heads, int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim,
+                                      int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
+                                      int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
+                                      int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
+                                      int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
+                                      float attn_scale, int causal, int64_t window, int64_t sinks, int* status,
+                                      void* stream) {
   using namespace tq;
+  TQ_REQUIRE(window >= 0 && sinks >= 0, TQ_ERR_BAD_ARG, "window and sinks must not be negative");
+  TQ_REQUIRE(window == 0 || causal, TQ_ERR_UNSUPPORTED, "a window needs causal attention");
+  TQ_REQUIRE(window > 0 || sinks == 0, TQ_ERR_BAD_ARG, "sinks need a window");
   TQ_REQUIRE(q && k && v && out && status, TQ_ERR_BAD_ARG, "tq_prefill_sdpa: NULL pointer");
   TQ_REQUIRE(dim == kD, TQ_ERR_BAD_DIM, "tq_prefill_sdpa supports head_dim 128, got %d", dim);
   TQ_REQUIRE(dtype == TQ_F16 || dtype == TQ_BF16, TQ_ERR_UNSUPPORTED, "tq_prefill_sdpa takes f16 or bf16 tensors");
@@ -605,13 +630,33 @@ extern "C" int tq_prefill_sdpa(const void* q, const void* k, const void* v, void
   a.bf16 = bf16;
   a.scale_log2 = attn_scale * kLog2e;
   a.status = status;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
-  });
-  if (attr_err != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "tq_prefill_sdpa: %s", cudaGetErrorString(attr_err));
+  // a window that reaches the first key from every row hides nothing: the full form
+  const bool windowed = window > 0 && window < seq_k;
+  a.window = windowed ? (int)window : 0;
+  a.sinks = windowed ? (int)(sinks < seq_k ? sinks : seq_k) : 0;
+  auto kernel = windowed ? prefill_kernel<true> : prefill_kernel<false>;
+  static bool ready[2][64] = {{false}};        // per device: the attribute belongs to the device's context
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && (dev < 0 || dev >= 64 || !ready[windowed][dev])) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    if (err == cudaSuccess && dev >= 0 && dev < 64) ready[windowed][dev] = true;
+  }
+  if (err != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "tq_prefill_sdpa: %s", cudaGetErrorString(err));
   const dim3 grid((unsigned)((seq_q + kBM - 1) / kBM), (unsigned)n_q_heads, (unsigned)batch);
-  prefill_kernel<<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(mq, mk, mv, a);
+  kernel<<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(mq, mk, mv, a);
   return check_launch("tq_prefill_sdpa");
+}
+
+extern "C" int tq_prefill_sdpa(const void* q, const void* k, const void* v, void* out, int dtype, int batch,
+                               int n_q_heads, int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim,
+                               int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
+                               int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
+                               int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
+                               int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
+                               float attn_scale, int causal, int* status, void* stream) {
+  return tq_prefill_sdpa_window(q, k, v, out, dtype, batch, n_q_heads, n_kv_heads, seq_q, seq_k, dim, q_batch_stride,
+                                q_head_stride, q_row_stride, k_batch_stride, k_head_stride, k_row_stride, v_batch_stride,
+                                v_head_stride, v_row_stride, o_batch_stride, o_head_stride, o_row_stride, attn_scale,
+                                causal, 0, 0, status, stream);
 }

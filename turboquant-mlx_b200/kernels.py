@@ -689,11 +689,16 @@ def prefill_supported(queries, keys, values, mask) -> bool:
 
 
 def prefill_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,
-                      causal: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+                      causal: bool = True, out: torch.Tensor | None = None, window: int = 0,
+                      sinks: int = 0) -> torch.Tensor:
     """softmax(scale * Q K^T [+ causal]) V for (B, n_q, L, 128) queries and
     (B, n_kv, S, 128) keys / values of one 16-bit dtype (GQA without replication).
     The call the reference leaves to its array library for every step that is not
-    a single-token decode (turboquant_mlx/patch.py:37)."""
+    a single-token decode (turboquant_mlx/patch.py:37).
+
+    window > 0 (causal only): the query at position i = row + S - L sees the keys in (i - window, i]
+    and the first `sinks` ones; key tiles that nothing sees are skipped.  As in any masked matrix
+    product, a hidden value row that is Inf or NaN still reaches rows that share a 128-key tile with it."""
     _lib.require_cuda(queries, keys, values)
     if queries.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("prefill_attention takes float16 or bfloat16 tensors")
@@ -715,7 +720,19 @@ def prefill_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.T
     q, k, v = usable(queries), usable(keys), usable(values)
     if out is None:
         out = torch.empty((B, n_q, L, D), dtype=q.dtype, device=q.device)
+    if window < 0 or sinks < 0 or (sinks and not window) or (window and not causal):
+        raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, sinks need a window, "
+                         "and a window needs causal attention")
     status = _lib.workspace(16, q.device, tag="prefill")
+    if window:
+        with torch.cuda.device(q.device):
+            _lib.check(_lib.lib().tq_prefill_sdpa_window(
+                _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
+                q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
+                v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1), out.stride(2),
+                float(scale), 1, min(int(window), 1 << 40), min(int(sinks), 1 << 40), _lib.ptr(status),
+                _lib.stream_ptr(q.device)))
+        return out
     _lib.check(_lib.lib().tq_prefill_sdpa(
         _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
         q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
