@@ -436,6 +436,7 @@ extern "C" int tq_paged_decode(const tq_paged_params* p) {
   a.part = (float*)p->workspace;
   a.ctas = num_sms();
   cudaStream_t st = (cudaStream_t)p->stream;
+  if (paged_mma_supported(a, p->dim)) return launch_paged_mma(a, st);
   a.min_tiles = kWarps;
   switch (p->dim) {
     case 32: return launch_general<1>(a, st);
