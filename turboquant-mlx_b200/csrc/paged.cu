@@ -29,6 +29,7 @@ int paged_status_ptr(int** out) {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kMaxCtas = 256;        // of a decode launch (one per SM)
 
 // ---- general decode -----------------------------------------------------------------------------------
 // out = sum_p softmax(scale * q . k_p) v_p in 32 bits on the CUDA cores, for every head dimension, code width
@@ -54,22 +55,21 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
     kc_s[threadIdx.x] = a.k.cent.v[threadIdx.x];
     vc_s[threadIdx.x] = a.v.cent.v[threadIdx.x];
   }
-  plan_tiles(a, prefix);
+  plan_costs(a, prefix);
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
-  int64_t t = plan.begin(cta);
-  const int64_t t_end = plan.begin(cta + 1);
-  Cursor cur;
-  cur.seek(a, prefix, t);
+  Cursor cur, end;
+  cur.seek(a, prefix, plan.begin(cta));
+  end.seek(a, prefix, plan.begin(cta + 1));
   const int kvpw = vals_per_word(a.k.bits), kpd = packed_words(DIM, a.k.bits);
   const int vvpw = vals_per_word(a.v.bits), vpd = packed_words(DIM, a.v.bits);
   const uint32_t kmask = (1u << a.k.bits) - 1u, vmask = (1u << a.v.bits) - 1u;
   const bool polar = a.k.format == TQ_KV_POLAR;
   const int rg_per_head = a.groups / a.n_kv_heads;
 
-  while (t < t_end) {
-    const int cnt = (int)min((int64_t)(cur.span.tiles - cur.j), t_end - t);
+  while (!cur.at(end)) {
+    const int cnt = cur.count_to(end);
     const int b = cur.b, kvh = cur.group / rg_per_head, r0 = (cur.group % rg_per_head) * kPagedRows;
     const int nr = min(kPagedRows, a.n_rep - r0), h0 = kvh * a.n_rep + r0;
     {   // query rows of the group: warp r prepares row r (rotated for packed keys), stored [element][row]
@@ -196,8 +196,8 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
       }
     }
     __syncthreads();
-    t += cnt;
-    if (cur.j + cnt == cur.span.tiles) cur.next_group(a);
+    if (cur.j + cnt < cur.span.tiles) break;
+    cur.next_group(a);
   }
 }
 
@@ -209,10 +209,12 @@ template <int EPL>
 __global__ void __launch_bounds__(kPagedRows * 32)
 paged_merge_kernel(const PagedDecodeArgs a) {
   constexpr int DIM = EPL * 32;
+  constexpr int kBatch = 8;          // partial states whose rows a lane has in flight
   __shared__ int prefix[kPlanEntries + 1];
+  __shared__ float w_s[kPagedRows][kMaxCtas];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = blockIdx.x, rg_per_head = a.groups / a.n_kv_heads;
-  plan_tiles(a, prefix);
+  plan_costs(a, prefix);
   const Plan plan = make_paged_plan(a, prefix);
   const int kvh = group / rg_per_head, r0 = (group % rg_per_head) * kPagedRows;
   if (warp >= min(kPagedRows, a.n_rep - r0)) return;
@@ -226,23 +228,45 @@ paged_merge_kernel(const PagedDecodeArgs a) {
       finish_row<EPL>(a, b, head, v, 0.f, lane);
       continue;
     }
-    const int64_t first = (int64_t)tiles_before(a, prefix, b) * a.groups + (int64_t)group * span.tiles;
+    const int64_t first = (int64_t)cost_before(a, prefix, b) * a.groups + (int64_t)group * cost_of(a, span) + a.group_cost;
     const int c0 = plan.owner(first), c1 = plan.owner(first + span.tiles - 1);
     if (c0 == c1) continue;
+    // the group's first CTA left its tail piece (slot 1), the others their head pieces (slot 0)
     auto slot = [&](int c) { return a.part + ((int64_t)(2 * c + (c == c0)) * kPagedRows + warp) * (DIM + 2); };
-    float mx = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(slot(c) + DIM));
+    const int n = c1 - c0 + 1;
+    float mx = -INFINITY, l = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float m = __ldcg(slot(c0 + i) + DIM);
+      w_s[warp][i] = m;
+      mx = fmaxf(mx, m);
+    }
     mx = warp_max(mx);
-    float l = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const float* p = slot(c);
-      const float m = __ldcg(p + DIM), li = __ldcg(p + DIM + 1);
-      const float f = m == -INFINITY ? (li == 0.f ? 0.f : 1.f) : paged_ex2(m - mx);
+    for (int i = lane; i < n; i += 32) {
+      const float m = w_s[warp][i], li = __ldcg(slot(c0 + i) + DIM + 1);
+      const float f = m == -INFINITY ? 1.f : paged_ex2(m - mx);      // m = -inf: l is 0, or NaN (a missing page)
+      w_s[warp][i] = f;
       l += li * f;
+    }
+    l = warp_sum(l);
+    __syncwarp();
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+      float x[kBatch][EPL];
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) v[j] += __ldcg(p + lane * EPL + j) * f;
+      for (int k = 0; k < kBatch; ++k) {
+        const float* p = slot(c0 + min(i0 + k, n - 1)) + lane * EPL;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float f = i0 + k < n ? w_s[warp][i0 + k] : 0.f;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (i0 + k < n) v[j] += x[k][j] * f;
+      }
     }
     finish_row<EPL>(a, b, head, v, l, lane);
+    __syncwarp();
   }
 }
 
@@ -434,10 +458,11 @@ extern "C" int tq_paged_decode(const tq_paged_params* p) {
   a.out_head_stride = p->out_head_stride;
   a.scale_log2 = p->attn_scale * kPagedLog2e;
   a.part = (float*)p->workspace;
-  a.ctas = num_sms();
+  a.ctas = num_sms() < kMaxCtas ? num_sms() : kMaxCtas;
   cudaStream_t st = (cudaStream_t)p->stream;
   if (paged_mma_supported(a, p->dim)) return launch_paged_mma(a, st);
   a.min_tiles = kWarps;
+  a.group_cost = 2;
   switch (p->dim) {
     case 32: return launch_general<1>(a, st);
     case 64: return launch_general<2>(a, st);

@@ -8,10 +8,12 @@
 // query heads), which never straddles a page (page sizes are powers of two, 32 at least).  A sequence has
 // only the tiles that its newest token sees: all of them, or with a sliding window the tiles of the first
 // `sinks` positions and those from position len - window on.  The tiles of a launch, numbered sequence by
-// sequence, group by group, are cut into equal runs, one per CTA, whatever the lengths of the sequences:
-// a ragged batch loads every SM alike, and a single long sequence is split as finely as it needs.  A CTA
-// that holds all tiles of a group writes its output; otherwise it leaves a partial state (m, l, acc) in
-// one of its two slots of the workspace, which the merge kernel joins.
+// sequence, group by group, are cut into runs of equal cost, one per CTA, whatever the lengths of the
+// sequences: a ragged batch loads every SM alike, and a single long sequence is split as finely as it needs.
+// Starting and finishing a group costs a CTA time too, so each group counts group_cost tiles more than it has
+// (a run that begins inside that lead begins at the group's first tile).  A CTA that holds all tiles of a
+// group writes its output; otherwise it leaves a partial state (m, l, acc) in one of its two slots of the
+// workspace, which the merge kernel joins.
 #pragma once
 
 #include "common.cuh"
@@ -20,7 +22,7 @@ namespace tq {
 
 constexpr int kPagedTile = 32;       // positions per tile
 constexpr int kPagedRows = 8;        // query heads per group
-constexpr int kPlanEntries = 1024;   // prefix entries of a CTA's plan (each covers ceil(batch / 1024) sequences)
+constexpr int kPlanEntries = 512;    // prefix entries of a CTA's plan (each covers ceil(batch / 512) sequences)
 constexpr float kPagedLog2e = 1.4426950408889634f;
 
 struct PagedHalf {                   // the K or the V half of a pool
@@ -63,8 +65,9 @@ struct PagedDecodeArgs {
   void* out;
   int64_t out_batch_stride, out_head_stride;
   float scale_log2;                  // attn_scale * log2(e)
+  uint32_t k_page_bytes, v_page_bytes, kn_page_bytes, vn_page_bytes;   // tensor-core kernel: page distances
   float* part;                       // [2 * ctas][8][dim + 2]: acc (rotated domain), m (log2 domain), l
-  int ctas, min_tiles;               // grid of the main kernel; fewest tiles worth a CTA
+  int ctas, min_tiles, group_cost;   // grid of the main kernel; fewest tiles worth a CTA; what a group costs besides, in tiles
 };
 
 #ifdef __CUDACC__
@@ -89,75 +92,89 @@ __device__ __forceinline__ SeqSpan span_of(const PagedDecodeArgs& a, int b) {
   return s;
 }
 
-// prefix[e] = tiles of one group in the sequences in front of entry e, prefix[n] = of all sequences.
+// What one group of a sequence costs in the plan.
+__device__ __forceinline__ int cost_of(const PagedDecodeArgs& a, const SeqSpan& s) { return s.tiles > 0 ? s.tiles + a.group_cost : 0; }
+
+__device__ __forceinline__ int plan_stride(const PagedDecodeArgs& a) { return (a.batch + kPlanEntries - 1) / kPlanEntries; }
+__device__ __forceinline__ int plan_entries(const PagedDecodeArgs& a) { const int per = plan_stride(a); return (a.batch + per - 1) / per; }
+
+// prefix[e] = cost of one group in the sequences in front of entry e, prefix[n] = of all sequences.
 // Called by every thread of the block; `prefix` holds kPlanEntries + 1 ints.
-__device__ __forceinline__ void plan_tiles(const PagedDecodeArgs& a, int* prefix) {
-  const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
-  const int n = (a.batch + per - 1) / per;
+__device__ __forceinline__ void plan_costs(const PagedDecodeArgs& a, int* prefix) {
+  const int per = plan_stride(a), n = plan_entries(a);
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
     int t = 0;
-    for (int b = e * per; b < min(a.batch, (e + 1) * per); ++b) t += span_of(a, b).tiles;
+    for (int b = e * per; b < min(a.batch, (e + 1) * per); ++b) t += cost_of(a, span_of(a, b));
     prefix[e + 1] = t;
   }
   if (threadIdx.x == 0) prefix[0] = 0;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    int carry = 0;
-    for (int e0 = 1; e0 <= n; e0 += 32) {
-      const int e = e0 + threadIdx.x;
-      int t = e <= n ? prefix[e] : 0;
+  if (n > 1) {
+    if (threadIdx.x < 32) {
+      int carry = 0;
+      for (int e0 = 1; e0 <= n; e0 += 32) {
+        const int e = e0 + threadIdx.x;
+        int t = e <= n ? prefix[e] : 0;
 #pragma unroll
-      for (int k = 1; k < 32; k <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, t, k);
-        if ((int)threadIdx.x >= k) t += o;
+        for (int k = 1; k < 32; k <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, t, k);
+          if ((int)threadIdx.x >= k) t += o;
+        }
+        t += carry;
+        if (e <= n) prefix[e] = t;
+        carry = __shfl_sync(0xffffffffu, t, 31);
       }
-      t += carry;
-      if (e <= n) prefix[e] = t;
-      carry = __shfl_sync(0xffffffffu, t, 31);
     }
+    __syncthreads();
   }
-  __syncthreads();
 }
 
 struct Plan {
-  int64_t total;       // tiles of the launch
-  int ctas;            // CTAs that get any
-  __device__ __forceinline__ int64_t begin(int cta) const { return total * cta / ctas; }
-  // the CTA whose run holds tile t
+  int64_t total, q;    // cost of the launch; cost of a run (the first `r` runs have one more)
+  int ctas, r;
+  __device__ __forceinline__ int64_t begin(int cta) const { return cta * q + min(cta, r); }
+  // the CTA whose run holds point t of the numbering
   __device__ __forceinline__ int owner(int64_t t) const {
-    int c = (int)(t * ctas / total);
-    while (begin(c + 1) <= t) ++c;
-    while (begin(c) > t) --c;
-    return c;
+    const int64_t head = r * (q + 1);
+    return t < head ? (int)(t / (q + 1)) : r + (int)((t - head) / q);
   }
 };
-__device__ __forceinline__ int plan_entries(const PagedDecodeArgs& a) {
-  const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
-  return (a.batch + per - 1) / per;
-}
 __device__ __forceinline__ Plan make_paged_plan(const PagedDecodeArgs& a, const int* prefix) {
   Plan p;
   p.total = (int64_t)prefix[plan_entries(a)] * a.groups;
-  const int64_t want = (p.total + a.min_tiles - 1) / a.min_tiles;
-  p.ctas = (int)max((int64_t)1, min((int64_t)a.ctas, want));
+  p.ctas = p.total >= (int64_t)a.ctas * a.min_tiles ? a.ctas : max(1, (int)(p.total + a.min_tiles - 1) / a.min_tiles);
+  if (p.total < (1ll << 31)) {           // 32-bit division is a tenth of the 64-bit one
+    p.q = (uint32_t)p.total / (uint32_t)p.ctas;
+    p.r = (int)((uint32_t)p.total - (uint32_t)p.q * (uint32_t)p.ctas);
+  } else {
+    p.q = p.total / p.ctas;
+    p.r = (int)(p.total - p.q * p.ctas);
+  }
   return p;
 }
-// Tiles of one group in the sequences in front of sequence b.
-__device__ __forceinline__ int tiles_before(const PagedDecodeArgs& a, const int* prefix, int b) {
-  const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
+// Cost of one group in the sequences in front of sequence b.
+__device__ __forceinline__ int cost_before(const PagedDecodeArgs& a, const int* prefix, int b) {
+  const int per = plan_stride(a);
   int t = prefix[b / per];
-  for (int i = b / per * per; i < b; ++i) t += span_of(a, i).tiles;
+  for (int i = b / per * per; i < b; ++i) t += cost_of(a, span_of(a, i));
   return t;
 }
 
-// Walks the tiles of a run in order.
+// A tile of the numbering: sequence, (kv head, row group), tile inside the group.
 struct Cursor {
-  int b, group, j;     // sequence, (kv head, row group), tile inside the group
-  SeqSpan span;
+  int b, group, j;
+  SeqSpan span;        // of sequence b
+  // the first tile at or behind point t; (batch, 0, 0) behind the last
   __device__ __forceinline__ void seek(const PagedDecodeArgs& a, const int* prefix, int64_t t) {
-    const int per = (a.batch + kPlanEntries - 1) / kPlanEntries;
-    int lo = 0, hi = plan_entries(a) - 1;          // last entry whose first tile is not behind t
-    while (lo < hi) {
+    const int per = plan_stride(a);
+    int lo = 0, hi = plan_entries(a) - 1;
+    if (t >= (int64_t)prefix[hi + 1] * a.groups) {
+      b = a.batch;
+      group = j = 0;
+      span.tiles = 0;
+      return;
+    }
+    while (lo < hi) {                            // last entry that does not begin behind t
       const int mid = (lo + hi + 1) / 2;
       if ((int64_t)prefix[mid] * a.groups <= t) lo = mid;
       else hi = mid - 1;
@@ -165,20 +182,36 @@ struct Cursor {
     int64_t rest = t - (int64_t)prefix[lo] * a.groups;
     b = lo * per;
     span = span_of(a, b);
-    while (rest >= (int64_t)span.tiles * a.groups && b + 1 < a.batch) {
-      rest -= (int64_t)span.tiles * a.groups;
+    int cost = cost_of(a, span);
+    while (rest >= (int64_t)cost * a.groups) {
+      rest -= (int64_t)cost * a.groups;
       span = span_of(a, ++b);
+      cost = cost_of(a, span);
     }
-    group = span.tiles > 0 ? (int)(rest / span.tiles) : 0;
-    j = span.tiles > 0 ? (int)(rest % span.tiles) : 0;
+    if (rest < (1ll << 31)) {
+      group = (int)((uint32_t)rest / (uint32_t)cost);
+      j = (int)((uint32_t)rest - (uint32_t)group * (uint32_t)cost);
+    } else {
+      group = (int)(rest / cost);
+      j = (int)(rest - (int64_t)group * cost);
+    }
+    j = max(0, j - a.group_cost);
   }
+  // tiles from here to the end of the group, at most to `end`
+  __device__ __forceinline__ int count_to(const Cursor& end) const {
+    return (b == end.b && group == end.group ? end.j : span.tiles) - j;
+  }
+  __device__ __forceinline__ bool at(const Cursor& end) const { return b == end.b && group == end.group && j == end.j; }
   // to the first tile of the next group that has any
   __device__ __forceinline__ void next_group(const PagedDecodeArgs& a) {
     j = 0;
     if (++group < a.groups) return;
     group = 0;
     do {
-      if (++b >= a.batch) return;
+      if (++b >= a.batch) {
+        span.tiles = 0;
+        return;
+      }
       span = span_of(a, b);
     } while (span.tiles == 0);
   }

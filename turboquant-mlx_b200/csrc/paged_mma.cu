@@ -42,45 +42,83 @@ struct MmaTables {
   float k_post, v_post;            // what scores and accumulators are multiplied with: ... / beta
 };
 
-// Shared memory of one CTA.
+// Shared memory of one CTA, by address in the shared window (kBase: where dynamic memory begins when a kernel has no
+// static arrays).  The pair tables lie at a multiple of their own size, so that a lookup's address is put together from
+// bits alone: one byte permute, or a shift and one logic operation, and no add.
+constexpr uint32_t kBase = 1024;
+constexpr uint32_t kEnd = 228 * 1024;
+constexpr uint32_t up16(uint32_t x) { return (x + 15) & ~15u; }
 template <int KF, int VB, int W, int S>
 struct Layout {
-  static constexpr int entry = dense(KF) ? 128 : 256;                  // bytes between table entries (K and V side by side)
-  static constexpr int v_entry = dense(KF) ? 0 : 128;
-  static constexpr int entries = (KF == KF_P4 || VB == 4) ? 256 : 64;
-  static constexpr int table = 0;
-  static constexpr int q = table + entries * entry;                    // query fragments [k-step][lane][4]
-  static constexpr int norms = q + 8 * 32 * 16;                        // per warp: key norms, log2 value norms, value norms of a tile
+  static constexpr uint32_t entry = dense(KF) ? 128 : 256;              // bytes between table entries (K and V side by side)
+  static constexpr uint32_t v_entry = dense(KF) ? 0 : 128;
+  static constexpr uint32_t entries = (KF == KF_P4 || VB == 4) ? 256 : 64;
+  static constexpr uint32_t table_bytes = entries * entry;
+  static constexpr uint32_t table = table_bytes > 16384 ? table_bytes : 16384, table_end = table + table_bytes;
+  static constexpr uint32_t k_off = 0;
+  static constexpr uint32_t kn_off = 32 * k_row_bytes(KF);
+  static constexpr uint32_t v_off = kn_off + (dense(KF) ? 0 : 128);
+  static constexpr uint32_t vn_off = v_off + 32 * v_row_bytes(VB);
+  static constexpr uint32_t stage = vn_off + 128;
+  // below the table: barriers, scalars, the plan; what does not fit goes behind the table, ring stages fill both sides
+  static constexpr uint32_t full = kBase, empty = full + W * S * 8;     // mbarriers of the ring stages
+  static constexpr uint32_t info = empty + W * S * 8;                   // per stage: first position of its tile | flags
+  static constexpr uint32_t q_post = up16(info + W * S * 4);            // 8 floats
+  static constexpr uint32_t ml = q_post + 32;                           // m, l of the warps that hand over rows: [2][W][8]
+  static constexpr uint32_t flag = ml + 2 * W * 32;
+  static constexpr uint32_t prefix = flag + 16;
+  static constexpr uint32_t norms = up16(prefix + (kPlanEntries + 1) * 4);   // per warp: key norms, log2 value norms, value norms
+  static constexpr uint32_t q = norms + W * 3 * 32 * 4;                 // query fragments [k-step][lane][4]
+  static constexpr uint32_t small_end = q + 8 * 32 * 16;
   static constexpr int xch_warps = (W + 1) / 2;
-  static constexpr int xch_row = kDim + 4;                             // padded: conflict-free stores
-  static constexpr int xch = norms + W * 3 * 32 * 4;                   // [xch_warps][8][xch_row] or [xch_warps][34][32]
-  static constexpr int xch_bytes = xch_warps * 34 * 32 * 4;
-  static constexpr int k_off = 0;
-  static constexpr int kn_off = 32 * k_row_bytes(KF);
-  static constexpr int v_off = kn_off + (dense(KF) ? 0 : 128);
-  static constexpr int vn_off = v_off + 32 * v_row_bytes(VB);
-  static constexpr int stage_bytes = vn_off + 128;
-  static constexpr int ring = xch + xch_bytes;
-  static constexpr int total = ring + W * S * stage_bytes;
+  static constexpr uint32_t xch_row = kDim + 4;                         // padded: conflict-free stores
+  static constexpr uint32_t xch_bytes = xch_warps * 34 * 32 * 4;        // [xch_warps][34][32] or [xch_warps][8][xch_row]
+  static constexpr bool xch_low = small_end + xch_bytes <= table;
+  static constexpr uint32_t xch = xch_low ? small_end : table_end;
+  static constexpr uint32_t low = xch_low ? xch + xch_bytes : small_end;       // ring stages 0 .. low_stages - 1
+  static constexpr uint32_t high = xch_low ? table_end : xch + xch_bytes;      // the others
+  static constexpr int low_fit = (int)((table - low) / stage);
+  static constexpr int low_stages = low_fit < W * S ? low_fit : W * S;
+  static constexpr uint32_t end = high + (W * S - low_stages) * stage;
+  static_assert(small_end <= table, "the small arrays fit below the table");
   static_assert(xch_warps * 8 * xch_row * 4 <= xch_bytes, "row exchange fits");
-  static_assert(ring % 16 == 0 && stage_bytes % 16 == 0 && q % 16 == 0 && norms % 16 == 0, "alignment");
-  static_assert(total + 6 * 1024 <= 227 * 1024, "shared memory of an SM");
+  static_assert(low % 16 == 0 && high % 16 == 0 && stage % 16 == 0 && q % 16 == 0 && norms % 16 == 0, "alignment");
+  static_assert(end <= kEnd, "shared memory of an SM");
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t it = 0; it < kSpin; ++it) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
+  for (uint32_t it = 0; it < kSpin; ++it)
+    if (mbar_try(bar, parity)) return true;
   return false;
+}
+template <int W>
+__device__ __forceinline__ void consumer_barrier() {
+  asm volatile("bar.sync 1, %0;" ::"n"(W * 32) : "memory");
+}
+// Two 32-bit floats at once.
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return r;
 }
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -160,145 +198,202 @@ __device__ __forceinline__ void value_slot(int e, int& g, int& s) {
   }
 }
 
-// What a warp fetches next: walks the warp's tiles of the CTA's run, one tile ahead of its page id.
-struct Feed {
-  Cursor c;
-  int64_t t, t_end;      // run position of the current piece's first tile; end of the run
-  int i, cnt, page;      // tile inside the piece (first: c.j); tiles of the piece; page of tile i, < 0: not in the pool
-};
+// Table entries never change once built, so the loads are not volatile; OFF: a constant part of the address.
+template <uint32_t OFF>
+__device__ __forceinline__ uint32_t lut(uint32_t addr) {
+  uint32_t v;
+  asm("ld.shared.u32 %0, [%1+%2];" : "=r"(v) : "r"(addr), "n"(OFF));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t addr) { return __uint_as_float(lds32(addr)); }
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void sts_f32(uint32_t addr, float v) { sts32(addr, __float_as_uint(v)); }
 
 template <int KF, int VB, int W, int S>
-__global__ void __launch_bounds__(W * 32, 1)
+__global__ void __launch_bounds__((W + 1) * 32, 1)
 paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constant__ MmaTables tb) {
   using L = Layout<KF, VB, W, S>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int prefix[kPlanEntries + 1];
-  __shared__ __align__(8) uint64_t bars[W * S];
-  __shared__ float q_post_s[kPagedRows];
-  __shared__ float m_s[W][kPagedRows], l_s[W][kPagedRows];
-  __shared__ int gave_up_s;
+  extern __shared__ __align__(1024) uint8_t smem[];       // shared address kBase
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  const uint32_t ring = smem_u32(smem) + L::ring + warp * S * L::stage_bytes;
-  const uint32_t bar0 = smem_u32(bars) + warp * S * 8;
-
-  if (threadIdx.x == 0) gave_up_s = 0;
-  if (lane == 0) {
-    for (int s = 0; s < S; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * s) : "memory");
+  const uint32_t lane4 = lane * 4;
+  int* prefix = reinterpret_cast<int*>(smem + L::prefix - kBase);
+  if (smem_u32(smem) != kBase) {         // the layout above would not hold
+    if (threadIdx.x == 0) atomicExch(a.view.status, 4);
+    return;
+  }
+  auto stage_addr = [&](int w, int s) {
+    const int k = w * S + s;
+    return k < L::low_stages ? L::low + k * L::stage : L::high + (k - L::low_stages) * L::stage;
+  };
+  if (threadIdx.x == 0) sts32(L::flag, 0);
+  if (threadIdx.x < W * S) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(L::full + 8 * threadIdx.x) : "memory");
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(L::empty + 8 * threadIdx.x) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // pair tables, one copy per lane: K entry = (code of the lower element | code of the upper << bits), V entry =
   // (code of the lower position | code of the upper << bits)
-  for (int i = threadIdx.x; i < L::entries * 32; i += W * 32) {
-    const int e = i >> 5;
-    uint32_t* at = reinterpret_cast<uint32_t*>(smem + L::table + e * L::entry) + (i & 31);
+  for (uint32_t i = threadIdx.x; i < L::entries * 32; i += (W + 1) * 32) {
+    const uint32_t e = i >> 5, at = L::table + e * L::entry + lane4;
     if (!dense(KF)) {
       constexpr int KB = KF == KF_P4 ? 4 : 3;
-      if (e < (1 << (2 * KB))) at[0] = (uint32_t)tb.k_c16[e & ((1 << KB) - 1)] | ((uint32_t)tb.k_c16[e >> KB] << 16);
+      if (e < (1u << (2 * KB))) sts32(at, (uint32_t)tb.k_c16[e & ((1 << KB) - 1)] | ((uint32_t)tb.k_c16[e >> KB] << 16));
     }
-    if (e < (1 << (2 * VB))) at[L::v_entry / 4] = (uint32_t)tb.v_c16[e & ((1 << VB) - 1)] | ((uint32_t)tb.v_c16[e >> VB] << 16);
+    if (e < (1u << (2 * VB))) sts32(at + L::v_entry, (uint32_t)tb.v_c16[e & ((1 << VB) - 1)] | ((uint32_t)tb.v_c16[e >> VB] << 16));
   }
-  plan_tiles(a, prefix);          // also the barrier behind the tables
+  plan_costs(a, prefix);          // also the barrier behind the tables
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
   const int rg_per_head = a.groups / a.n_kv_heads;
+  Cursor cur, end;
+  cur.seek(a, prefix, plan.begin(cta));
+  end.seek(a, prefix, plan.begin(cta + 1));
+  if (cur.at(end)) return;
 
-  // ---------------- the warp's copies ----------------
-  Feed f;
-  f.t = plan.begin(cta);
-  f.t_end = plan.begin(cta + 1);
-  f.c.seek(a, prefix, f.t);
-  f.cnt = (int)min((int64_t)(f.c.span.tiles - f.c.j), f.t_end - f.t);
-  f.i = warp;
-  Cursor cur = f.c;
-  int64_t run = f.t;
-  const int64_t run_end = f.t_end;
-  uint32_t bad = 0;               // bit s: the tile of stage s has no page in the pool
-  int issued = 0, used = 0;       // tiles fetched and consumed by this warp
-  auto settle = [&]() {           // to the next tile this warp owns; starts loading its page id
-    while (f.i >= f.cnt) {
-      f.t += f.cnt;
-      if (f.t >= f.t_end) {
-        f.cnt = 0;
-        return;
+  // ---------------- producer: lane w fetches for warp w ----------------
+  // Each lane walks its warp's tiles on its own; the warp executes that walk once for all of them.
+  if (warp == W) {
+    const bool polar = !dense(KF);
+    const int row_mask = (1 << a.view.page_shift) - 1;
+    Cursor fc = cur;                  // the piece the lane's next tile is in
+    int i = lane, cnt = lane < W ? cur.count_to(end) : 0, page = 0;       // cnt 0: the lane has no tile left
+    const uint8_t *kb = nullptr, *vb = nullptr, *kn = nullptr, *vn = nullptr;      // the group's head in page 0
+    auto bases = [&]() {
+      const int head = rg_per_head == 1 ? fc.group : fc.group / rg_per_head;
+      kb = reinterpret_cast<const uint8_t*>(a.k.data) + head * a.k.head_stride * (polar ? 4 : 2);
+      vb = reinterpret_cast<const uint8_t*>(a.v.data) + head * a.v.head_stride * 4;
+      kn = reinterpret_cast<const uint8_t*>(a.k.norms) + head * a.k.norm_head_stride * 4;
+      vn = reinterpret_cast<const uint8_t*>(a.v.norms) + head * a.v.norm_head_stride * 4;
+    };
+    auto settle = [&]() {             // to the lane's next tile; its page id is on its way when this returns
+      while (cnt != 0 && i >= cnt) {
+        if (fc.j + cnt < fc.span.tiles) {      // the run ends inside this group
+          cnt = 0;
+          break;
+        }
+        i -= cnt;
+        fc.next_group(a);
+        cnt = fc.at(end) ? 0 : fc.count_to(end);
+        if (cnt != 0) bases();
       }
-      f.c.next_group(a);
-      f.cnt = (int)min((int64_t)f.c.span.tiles, f.t_end - f.t);
-      f.i = warp;
-    }
-    const int pos = f.c.span.tile_at(f.c.j + f.i) * kPagedTile;
-    f.page = __ldg(a.view.table + f.c.b * a.view.table_stride + (pos >> a.view.page_shift));
-  };
-  auto fetch = [&]() {            // issues the copies of the current tile into the next stage
-    if (f.cnt == 0) return;
-    const int s = issued % S;
-    const int pos = f.c.span.tile_at(f.c.j + f.i) * kPagedTile;
-    const int row = pos & ((1 << a.view.page_shift) - 1);
-    const int head = f.c.group / rg_per_head;
-    const bool ok = f.page >= 0 && f.page < a.view.n_pages;
-    bad = (bad & ~(1u << s)) | (ok ? 0u : 1u << s);
-    if (lane == 0) {
-      const uint32_t bar = bar0 + 8 * s, st = ring + s * L::stage_bytes;
-      const uint32_t tx = ok ? L::stage_bytes : 0;
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(tx) : "memory");
-      if (ok) {
-        const int64_t page = f.page;
-        constexpr int kunit = dense(KF) ? 2 : 4;
-        bulk_g2s(st + L::k_off,
-                 reinterpret_cast<const uint8_t*>(a.k.data) + (page * a.k.page_stride + head * a.k.head_stride) * kunit +
-                     (int64_t)row * k_row_bytes(KF),
-                 32 * k_row_bytes(KF), bar);
-        if (!dense(KF))
-          bulk_g2s(st + L::kn_off, a.k.norms + page * a.k.norm_page_stride + head * a.k.norm_head_stride + row, 128, bar);
-        bulk_g2s(st + L::v_off,
-                 reinterpret_cast<const uint8_t*>(a.v.data) + (page * a.v.page_stride + head * a.v.head_stride) * 4 +
-                     (int64_t)row * v_row_bytes(VB),
-                 32 * v_row_bytes(VB), bar);
-        bulk_g2s(st + L::vn_off, a.v.norms + page * a.v.norm_page_stride + head * a.v.norm_head_stride + row, 128, bar);
-      } else {
-        atomicExch(a.view.status, 1);
+      if (cnt != 0) {
+        const int pos = fc.span.tile_at(fc.j + i) * kPagedTile;
+        page = __ldg(a.view.table + fc.b * a.view.table_stride + (pos >> a.view.page_shift));
       }
-    }
-    ++issued;
-    f.i += W;
+    };
+    bases();
     settle();
-  };
-  settle();
-#pragma unroll
-  for (int s = 0; s < S; ++s) fetch();
+    int s = 0, issued = 0;
+    uint32_t phase = 1, idle = 0;     // a fresh stage counts as released
+    while (__any_sync(0xffffffffu, cnt != 0)) {
+      const bool go = cnt != 0 && mbar_try(L::empty + 8 * (lane * S + s), phase);
+      if (go) {
+        const bool ok = page >= 0 && page < a.view.n_pages;
+        const int pos = fc.span.tile_at(fc.j + i) * kPagedTile;
+        const bool full = pos + kPagedTile <= fc.span.n && (pos >= fc.span.lo || pos + kPagedTile <= a.sinks);
+        const uint32_t bar = L::full + 8 * (lane * S + s), st = stage_addr(lane, s);
+        sts32(L::info + 4 * (lane * S + s), (uint32_t)pos | (full && ok ? 1u : 0u) | (ok ? 0u : 2u));
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(ok ? L::stage : 0u) : "memory");
+        if (ok) {
+          const uint64_t pg = (uint32_t)page;
+          const uint32_t row = pos & row_mask;
+          bulk_g2s(st + L::k_off, kb + pg * a.k_page_bytes + row * k_row_bytes(KF), 32 * k_row_bytes(KF), bar);
+          if (polar) bulk_g2s(st + L::kn_off, kn + pg * a.kn_page_bytes + row * 4, 128, bar);
+          bulk_g2s(st + L::v_off, vb + pg * a.v_page_bytes + row * v_row_bytes(VB), 32 * v_row_bytes(VB), bar);
+          bulk_g2s(st + L::vn_off, vn + pg * a.vn_page_bytes + row * 4, 128, bar);
+        } else {
+          atomicExch(a.view.status, 1);
+        }
+        ++issued;
+        if (++s == S) {
+          s = 0;
+          phase ^= 1u;
+        }
+        i += W;
+        settle();
+      }
+      __syncwarp();
+      if (__any_sync(0xffffffffu, go)) {
+        idle = 0;
+      } else {
+        if (lds32(L::flag) != 0) break;
+        if (++idle == kSpin) {
+          sts32(L::flag, 1);
+          if (lane == 0) atomicExch(a.view.status, 3);
+          break;
+        }
+        __nanosleep(100);
+      }
+    }
+    // every copy has landed before the CTA may end (bounded; the consumers have seen to it in all but the failed case)
+    for (int n = max(0, issued - S); n < issued; ++n) mbar_wait(L::full + 8 * (lane * S + n % S), (n / S) & 1);
+    return;
+  }
 
   // this thread's rows of a tile: key row of n-group ng: k_row0 + 2 ng; value rows of its ng-th pair: v_row0 + 2 ng, v_row1 + 2 ng
   constexpr bool kSwap = VB == 4;
   const int k_row0 = 8 * (g >> 1) + ((g & 1) ^ (kSwap ? (g >> 1) & 1 : 0));
   const int v_row0 = 8 * t4 + (kSwap ? t4 & 1 : 0), v_row1 = 8 * t4 + 1 - (kSwap ? t4 & 1 : 0);
-  const uint32_t lane4 = lane * 4;
-  float* nrm = reinterpret_cast<float*>(smem + L::norms) + warp * 96;
-  const int nrm_at = kSwap ? lane ^ ((lane >> 3) & 1) : lane;      // the place of position `lane` in that order
-  const uint8_t* table = smem + L::table;
-  auto k_lut = [&](uint32_t off) { return *reinterpret_cast<const uint32_t*>(table + off); };
-  auto v_lut = [&](uint32_t off) { return *reinterpret_cast<const uint32_t*>(table + L::v_entry + off); };
-  // byte j of a word as a table offset: byte 1 = the code pair, byte 0 = the lane's copy
-  auto byte_off = [&](uint32_t w, int j) {
-    return L::entry == 256 ? __byte_perm(w, lane4, 0x5504 | (j << 4))
-                           : ((j == 0 ? w << 7 : w >> (8 * j - 7)) & 0x7F80u) | lane4;
+  const uint32_t nrm = L::norms + warp * 384;
+  const uint32_t nrm_at = nrm + 4 * (kSwap ? lane ^ ((lane >> 3) & 1) : lane);      // the place of position `lane` in that order
+  uint32_t lut_lane;                                     // table address of entry 0 in this lane's copy; opaque, so that
+  asm("add.u32 %0, %1, %2;" : "=r"(lut_lane) : "r"(lane4), "n"(L::table));   // an address stays one logic operation
+  auto k_lut = [&](uint32_t at) { return lut<0>(at); };
+  auto v_lut = [&](uint32_t at) { return lut<L::v_entry>(at); };
+  // byte j of a word (a pair of 4-bit codes) as a table address
+  auto byte_at = [&](uint32_t w, int j) {
+    return L::entry == 256 ? __byte_perm(w, lut_lane, 0x7604 | (j << 4))
+                           : ((j == 0 ? w << 7 : w >> (8 * j - 7)) & 0x7F80u) | lut_lane;
   };
-  // 6-bit field i of a word as a table offset
-  auto field_off = [&](uint32_t w, int i) {
+  // 6-bit field i of a word as a table address
+  auto field_at = [&](uint32_t w, int i) {
     constexpr int sh = L::entry == 256 ? 8 : 7;
-    return ((6 * i >= sh ? w >> (6 * i - sh) : w << (sh - 6 * i)) & (0x3Fu << sh)) | lane4;
+    return ((6 * i >= sh ? w >> (6 * i - sh) : w << (sh - 6 * i)) & (0x3Fu << sh)) | lut_lane;
   };
 
-  while (run < run_end) {
-    const int cnt = (int)min((int64_t)(cur.span.tiles - cur.j), run_end - run);
-    const int b = cur.b, kvh = cur.group / rg_per_head, r0 = (cur.group % rg_per_head) * kPagedRows;
+  uint32_t st = stage_addr(warp, 0);
+  int us = 0;                        // stage of the tile consumed next
+  uint32_t phase = 0;
+  int i = warp;
+  // the group's query rows, four elements of row `warp` per lane: fetched a group ahead
+  auto load_query = [&](const Cursor& c, float (&x)[4]) {
+    const int kvh = rg_per_head == 1 ? c.group : c.group / rg_per_head, rr = (c.group - kvh * rg_per_head) * kPagedRows + warp;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = warp < kPagedRows && rr < a.n_rep
+                 ? load_elem(a.q, a.q_dtype, c.b * a.q_batch_stride + (kvh * a.n_rep + rr) * a.q_head_stride + lane * 4 + j) : 0.f;
+  };
+  static_assert(W >= kPagedRows, "a warp per query row");
+  float xq[4];
+  load_query(cur, xq);
+  while (true) {
+    const int cnt = cur.count_to(end);
+    const int b = cur.b, kvh = rg_per_head == 1 ? cur.group : cur.group / rg_per_head;
+    const int r0 = (cur.group - kvh * rg_per_head) * kPagedRows;
     const int nr = min(kPagedRows, a.n_rep - r0), h0 = kvh * a.n_rep + r0;
     // ---------------- query fragments ----------------
-    for (int r = warp; r < kPagedRows; r += W) {
-      float x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x[j] = r < nr ? load_elem(a.q, a.q_dtype, b * a.q_batch_stride + (h0 + r) * a.q_head_stride + lane * 4 + j) : 0.f;
+    if (warp < kPagedRows) {
+      const int r = warp;
+      float x[4] = {xq[0], xq[1], xq[2], xq[3]};
       if (!dense(KF)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] *= sign_at(a.k.signs, lane * 4 + j);
@@ -309,49 +404,55 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       const int ex = top > 0.f && top < INFINITY ? 9 - (((__float_as_int(top) >> 23) & 255) - 126) : 0;
       const int up1 = ex / 2, up2 = ex - up1;           // two steps: each factor is a normal number
       const float f1 = __int_as_float((127 + up1) << 23), f2 = __int_as_float((127 + up2) << 23);
-      if (lane == 0) q_post_s[r] = tb.k_post * __int_as_float((127 - up1) << 23) * __int_as_float((127 - up2) << 23);
+      if (lane == 0)
+        sts_f32(L::q_post + 4 * r, tb.k_post * __int_as_float((127 - up1) << 23) * __int_as_float((127 - up2) << 23));
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         uint32_t hi, lo;
         split_pair<KF == KF_BF16>(x[j] * f1 * f2, x[j + 1] * f1 * f2, hi, lo);
         int ks, t, up;
         query_slot<KF>(lane * 4 + j, ks, t, up);
-        uint32_t* at = reinterpret_cast<uint32_t*>(smem + L::q) + (ks * 32 + r * 4 + t) * 4 + 2 * up;
-        at[0] = hi;
-        at[1] = lo;
+        const uint32_t at = L::q + ((ks * 32 + r * 4 + t) * 4 + 2 * up) * 4;
+        sts32(at, hi);
+        sts32(at + 4, lo);
       }
     }
-    __syncthreads();
+    consumer_barrier<W>();
     uint32_t aq[8][4];
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
-      const uint4 w = *reinterpret_cast<const uint4*>(smem + L::q + (ks * 32 + lane) * 16);
+      const uint4 w = lds128(L::q + (ks * 32 + lane) * 16);
       aq[ks][0] = w.x; aq[ks][1] = w.y; aq[ks][2] = w.z; aq[ks][3] = w.w;
     }
-    const float post = q_post_s[g];
+    const float post = lds_f32(L::q_post + 4 * g);
+    const bool last = cur.j + cnt < cur.span.tiles;       // the run ends inside this group
+    Cursor nx = cur;
+    if (!last) nx.next_group(a);
+    const bool more = !last && !nx.at(end);
+    if (more) load_query(nx, xq);
 
     float o[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    for (int i = warp; i < cnt; i += W) {
-      const int s = used % S;
-      if (!mbar_wait(bar0 + 8 * s, (used / S) & 1)) {      // gave up: everything this CTA produces from here on is NaN
-        gave_up_s = 1;
-        if (lane == 0) atomicExch(a.view.status, 3);
+    for (; i < cnt; i += W) {
+      if (!mbar_wait(L::full + 8 * (warp * S + us), phase)) {      // gave up: everything this CTA produces from here on is NaN
+        if (lane == 0) {
+          sts32(L::flag, 1);
+          atomicExch(a.view.status, 3);
+        }
         break;
       }
-      ++used;
-      const uint8_t* st = smem + L::ring + (warp * S + s) * L::stage_bytes;
-      const int p0 = cur.span.tile_at(cur.j + i) * kPagedTile;
-      const bool full = p0 + kPagedTile <= cur.span.n && (p0 >= cur.span.lo || p0 + kPagedTile <= a.sinks);
+      const uint32_t info = lds32(L::info + 4 * (warp * S + us));
+      const int p0 = info & ~31u;
+      const bool full = info & 1u;
       {   // norms: lane = position
         const bool seen = full || cur.span.sees(p0 + lane, a.sinks);
-        const float vn = seen ? *reinterpret_cast<const float*>(st + L::vn_off + lane4) : 0.f;
-        if (!dense(KF)) nrm[nrm_at] = *reinterpret_cast<const float*>(st + L::kn_off + lane4);
-        nrm[32 + nrm_at] = lg2(fmaxf(vn, 1e-26f));
-        nrm[64 + nrm_at] = vn;
+        const float vn = seen ? lds_f32(st + L::vn_off + lane4) : 0.f;
+        if (!dense(KF)) sts32(nrm_at, lds32(st + L::kn_off + lane4));
+        sts_f32(nrm_at + 128, lg2(fmaxf(vn, 1e-26f)));
+        sts_f32(nrm_at + 256, vn);
         __syncwarp();
       }
       // ---------------- scores ----------------
@@ -359,52 +460,115 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
 #pragma unroll
       for (int ng = 0; ng < 4; ++ng) {
         sc[ng][0] = sc[ng][1] = sc[ng][2] = sc[ng][3] = 0.f;
-        const uint8_t* row = st + L::k_off + (k_row0 + 2 * ng) * k_row_bytes(KF);
+        const uint32_t row = st + L::k_off + (k_row0 + 2 * ng) * k_row_bytes(KF);
         if (dense(KF)) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
-            const uint4 w = *reinterpret_cast<const uint4*>(row + t4 * 16 + it * 64);
+            const uint4 w = lds128(row + t4 * 16 + it * 64);
             mma<KF == KF_BF16>(sc[ng], aq[2 * it], w.x, w.y);
             mma<KF == KF_BF16>(sc[ng], aq[2 * it + 1], w.z, w.w);
           }
         } else if (KF == KF_P4) {
-          const uint4 w4 = *reinterpret_cast<const uint4*>(row + t4 * 16);
+          const uint4 w4 = lds128(row + t4 * 16);
           const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            mma<false>(sc[ng], aq[2 * k], k_lut(byte_off(w[k], 0)), k_lut(byte_off(w[k], 1)));
-            mma<false>(sc[ng], aq[2 * k + 1], k_lut(byte_off(w[k], 2)), k_lut(byte_off(w[k], 3)));
+            mma<false>(sc[ng], aq[2 * k], k_lut(byte_at(w[k], 0)), k_lut(byte_at(w[k], 1)));
+            mma<false>(sc[ng], aq[2 * k + 1], k_lut(byte_at(w[k], 2)), k_lut(byte_at(w[k], 3)));
           }
         } else {
-          const uint32_t* words = reinterpret_cast<const uint32_t*>(row);
           uint32_t w[3];
 #pragma unroll
-          for (int k = 0; k < 3; ++k) w[k] = words[3 * t4 + k];
-          const uint32_t w12 = words[12] >> (6 * t4);
+          for (int k = 0; k < 3; ++k) w[k] = lds32(row + 12 * t4 + 4 * k);
+          const uint32_t w12 = lds32(row + 48) >> (6 * t4);
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const int p = 2 * ks, p1 = 2 * ks + 1;
-            mma<false>(sc[ng], aq[ks], k_lut(field_off(w[p / 5], p % 5)),
-                       p1 < 15 ? k_lut(field_off(w[p1 < 15 ? p1 / 5 : 0], p1 % 5)) : k_lut(field_off(w12, 0)));
+            mma<false>(sc[ng], aq[ks], k_lut(field_at(w[p / 5], p % 5)),
+                       p1 < 15 ? k_lut(field_at(w[p1 < 15 ? p1 / 5 : 0], p1 % 5)) : k_lut(field_at(w12, 0)));
           }
         }
       }
+      // value fragments of one k-step (two position pairs per thread)
+      auto load_values = [&](int half, uint32_t (&af)[8][4]) {
+        uint32_t off[2][16];          // table addresses of the 16 slots, for the two position pairs of this k-step
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int ng = 2 * half + p;
+          const uint32_t r0p = st + L::v_off + (v_row0 + 2 * ng) * v_row_bytes(VB);
+          const uint32_t r1p = st + L::v_off + (v_row1 + 2 * ng) * v_row_bytes(VB);
+          if (VB == 4) {
+            const uint2 x = lds64(r0p + 8 * g), y = lds64(r1p + 8 * g);
+            const uint32_t xs[2] = {x.x, x.y}, ys[2] = {y.x, y.y};
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t ev = (xs[w] & 0x0F0F0F0Fu) | ((ys[w] << 4) & 0xF0F0F0F0u);     // even elements
+              const uint32_t od = ((xs[w] >> 4) & 0x0F0F0F0Fu) | (ys[w] & 0xF0F0F0F0u);     // odd elements
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                off[p][8 * w + 2 * k] = byte_at(ev, k);
+                off[p][8 * w + 2 * k + 1] = byte_at(od, k);
+              }
+            }
+          } else {
+            constexpr uint32_t kEven = 0707070707u;             // codes 0, 2, 4, 6, 8 of a word
+            const int shb = 15 * (g & 1), shc = 3 * g;
+            const uint32_t wb = 32 + 4 * (g >> 1);
+            const uint32_t xa = lds32(r0p + 4 * g), ya = lds32(r1p + 4 * g), xb = lds32(r0p + wb) >> shb,
+                           yb = lds32(r1p + wb) >> shb, xc = lds32(r0p + 48) >> shc, yc = lds32(r1p + 48) >> shc;
+            // complementary masks (one logic operation); bits behind the fields are cut off by field_at
+            const uint32_t ea = (xa & kEven) | ((ya << 3) & ~kEven), oa = ((xa >> 3) & kEven) | (ya & ~kEven);
+            const uint32_t eb = (xb & kEven) | ((yb << 3) & ~kEven), ob = ((xb >> 3) & kEven) | (yb & ~kEven);
+            const uint32_t ec = (xc & kEven) | ((yc << 3) & ~kEven);
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+              off[p][2 * k] = field_at(ea, k);
+              off[p][2 * k + 1] = field_at(oa, k);
+            }
+            off[p][10] = field_at(eb, 0);
+            off[p][11] = field_at(ob, 0);
+            off[p][12] = field_at(eb, 1);
+            off[p][13] = field_at(ob, 1);
+            off[p][14] = field_at(eb, 2);
+            off[p][15] = field_at(ec, 0);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          af[j][0] = v_lut(off[0][2 * j]);
+          af[j][1] = v_lut(off[0][2 * j + 1]);
+          af[j][2] = v_lut(off[1][2 * j]);
+          af[j][3] = v_lut(off[1][2 * j + 1]);
+        }
+      };
+      // the first half's lookups wait for nothing: they fill the time the score products and the softmax take
+      uint32_t af0[8][4];
+      load_values(0, af0);
       // ---------------- softmax: head g, positions 8 t4 + 2 ng + c in this tile's order ----------------
-      const bool missing = (bad >> s) & 1u;
+      const bool missing = info & 2u;
       float kn[8], lv[8], vn[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!dense(KF)) *reinterpret_cast<float4*>(kn + 4 * h) = *reinterpret_cast<const float4*>(nrm + 8 * t4 + 4 * h);
-        *reinterpret_cast<float4*>(lv + 4 * h) = *reinterpret_cast<const float4*>(nrm + 32 + 8 * t4 + 4 * h);
-        *reinterpret_cast<float4*>(vn + 4 * h) = *reinterpret_cast<const float4*>(nrm + 64 + 8 * t4 + 4 * h);
+        const uint32_t at = nrm + 32 * t4 + 16 * h;
+        const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + 128), z = lds128(at + 256);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          kn[4 * h + k] = __uint_as_float(xs[k]);
+          lv[4 * h + k] = __uint_as_float(ys[k]);
+          vn[4 * h + k] = __uint_as_float(zs[k]);
+        }
       }
       float s2[8], top = -INFINITY;
+      const float2 post2 = make_float2(post, post);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float raw = sc[k >> 1][k & 1] + sc[k >> 1][(k & 1) + 2];
-        s2[k] = raw * (dense(KF) ? post : kn[k] * post);
+      for (int k = 0; k < 8; k += 2) {       // high part and residual of the query, scale, key norm
+        float2 x = mul2(add2(make_float2(sc[k >> 1][0], sc[k >> 1][1]), make_float2(sc[k >> 1][2], sc[k >> 1][3])), post2);
+        if (!dense(KF)) x = mul2(x, make_float2(kn[k], kn[k + 1]));
+        s2[k] = x.x;
+        s2[k + 1] = x.y;
       }
-      if (!full || missing) {
+      if (!full) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int pos = p0 + ((k & 1) ? v_row1 : v_row0) + (k & 6);
@@ -413,7 +577,10 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, s2[k] + lv[k]);
+      for (int k = 0; k < 8; k += 2) {
+        const float2 x = add2(make_float2(s2[k], s2[k + 1]), make_float2(lv[k], lv[k + 1]));
+        top = fmaxf(top, fmaxf(x.x, x.y));
+      }
       if (__any_sync(0xffffffffu, top > m_run + kRescale)) {       // also for the first visible tile
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -432,64 +599,29 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       uint32_t pb[4];
 #pragma unroll
       for (int ng = 0; ng < 4; ++ng) {
-        const float e0 = paged_ex2(s2[2 * ng] - m_use), e1 = paged_ex2(s2[2 * ng + 1] - m_use);
-        l_run += e0 + e1;
-        const __half2 h = __floats2half2_rn(e0 * vn[2 * ng], e1 * vn[2 * ng + 1]);
+        const float2 d = add2(make_float2(s2[2 * ng], s2[2 * ng + 1]), make_float2(-m_use, -m_use));
+        const float2 e = make_float2(paged_ex2(d.x), paged_ex2(d.y));
+        l_run += e.x + e.y;
+        const float2 w = mul2(e, make_float2(vn[2 * ng], vn[2 * ng + 1]));
+        const __half2 h = __floats2half2_rn(w.x, w.y);
         pb[ng] = *reinterpret_cast<const uint32_t*>(&h);
       }
       // ---------------- values ----------------
+      uint32_t af1[8][4];
+      load_values(1, af1);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t off[2][16];          // table offsets of the 16 slots, for the two position pairs of this k-step
+      for (int j = 0; j < 8; ++j) mma<false>(o[j], af0[j], pb[0], pb[1]);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int ng = 2 * half + p;
-          const uint8_t* r0p = st + L::v_off + (v_row0 + 2 * ng) * v_row_bytes(VB);
-          const uint8_t* r1p = st + L::v_off + (v_row1 + 2 * ng) * v_row_bytes(VB);
-          if (VB == 4) {
-            const uint2 x = *reinterpret_cast<const uint2*>(r0p + 8 * g), y = *reinterpret_cast<const uint2*>(r1p + 8 * g);
-            const uint32_t xs[2] = {x.x, x.y}, ys[2] = {y.x, y.y};
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const uint32_t ev = (xs[w] & 0x0F0F0F0Fu) | ((ys[w] << 4) & 0xF0F0F0F0u);     // even elements
-              const uint32_t od = ((xs[w] >> 4) & 0x0F0F0F0Fu) | (ys[w] & 0xF0F0F0F0u);     // odd elements
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                off[p][8 * w + 2 * k] = byte_off(ev, k);
-                off[p][8 * w + 2 * k + 1] = byte_off(od, k);
-              }
-            }
-          } else {
-            const uint32_t *xw = reinterpret_cast<const uint32_t*>(r0p), *yw = reinterpret_cast<const uint32_t*>(r1p);
-            constexpr uint32_t kEven = 0707070707u;      // codes 0, 2, 4, 6, 8 of a word
-            const int shb = 15 * (g & 1), shc = 3 * g;
-            const uint32_t xa = xw[g], ya = yw[g], xb = xw[8 + (g >> 1)] >> shb, yb = yw[8 + (g >> 1)] >> shb,
-                           xc = xw[12] >> shc, yc = yw[12] >> shc;
-            const uint32_t ea = (xa & kEven) | ((ya << 3) & (kEven << 3)), oa = ((xa >> 3) & kEven) | (ya & (kEven << 3));
-            const uint32_t eb = (xb & kEven) | ((yb << 3) & (kEven << 3)), ob = ((xb >> 3) & kEven) | (yb & (kEven << 3));
-            const uint32_t ec = (xc & 7u) | ((yc & 7u) << 3);
-#pragma unroll
-            for (int k = 0; k < 5; ++k) {
-              off[p][2 * k] = field_off(ea, k);
-              off[p][2 * k + 1] = field_off(oa, k);
-            }
-            off[p][10] = field_off(eb, 0);
-            off[p][11] = field_off(ob, 0);
-            off[p][12] = field_off(eb, 1);
-            off[p][13] = field_off(ob, 1);
-            off[p][14] = field_off(eb, 2);
-            off[p][15] = field_off(ec, 0);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t af[4] = {v_lut(off[0][2 * j]), v_lut(off[0][2 * j + 1]), v_lut(off[1][2 * j]), v_lut(off[1][2 * j + 1])};
-          mma<false>(o[j], af, pb[2 * half], pb[2 * half + 1]);
-        }
-      }
+      for (int j = 0; j < 8; ++j) mma<false>(o[j], af1[j], pb[2], pb[3]);
       __syncwarp();            // every lane is done with the stage (and with the norms)
-      fetch();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(L::empty + 8 * (warp * S + us)) : "memory");
+      if (++us == S) {
+        us = 0;
+        phase ^= 1u;
+      }
+      st = stage_addr(warp, us);
     }
+    i -= cnt;                  // the warp's first tile of the next group
 
     // ---------------- the warps meet ----------------
     // the upper half of the warps hands its state to the lower half, which hands rows to one warp per head
@@ -497,18 +629,18 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
     if (warp >= HW) {
-      float* to = reinterpret_cast<float*>(smem + L::xch) + (warp - HW) * 34 * 32 + lane;
+      const uint32_t to = L::xch + (warp - HW) * 34 * 128 + lane4;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) to[(4 * j + c) * 32] = o[j][c];
-      to[32 * 32] = m_run;
-      to[33 * 32] = l_run;
+        for (int c = 0; c < 4; ++c) sts_f32(to + (4 * j + c) * 128, o[j][c]);
+      sts_f32(to + 32 * 128, m_run);
+      sts_f32(to + 33 * 128, l_run);
     }
-    __syncthreads();
+    consumer_barrier<W>();
     if (warp < HW && warp + HW < W) {
-      const float* from = reinterpret_cast<const float*>(smem + L::xch) + warp * 34 * 32;
-      const float m2 = from[32 * 32 + lane], l2 = from[33 * 32 + lane];
+      const uint32_t from = L::xch + warp * 34 * 128 + lane4;
+      const float m2 = lds_f32(from + 32 * 128), l2 = lds_f32(from + 33 * 128);
       const float mx = fmaxf(m_run, m2);
       // a state that saw nothing has m = -inf; one that met a missing page then has l = NaN, which must live on
       const float fa = m_run == -INFINITY ? 1.f : paged_ex2(m_run - mx), fb = m2 == -INFINITY ? 1.f : paged_ex2(m2 - mx);
@@ -520,39 +652,43 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          o[j][c] = o[j][c] * ((c & 1) ? fa1 : fa0) + from[(4 * j + c) * 32 + lane] * ((c & 1) ? fb1 : fb0);
+          o[j][c] = o[j][c] * ((c & 1) ? fa1 : fa0) + lds_f32(from + (4 * j + c) * 128) * ((c & 1) ? fb1 : fb0);
     }
-    __syncthreads();
+    consumer_barrier<W>();
     if (warp < HW) {
-      float* to = reinterpret_cast<float*>(smem + L::xch) + warp * kPagedRows * L::xch_row;
+      const uint32_t to = L::xch + warp * kPagedRows * L::xch_row * 4;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) to[(2 * t4 + (c & 1)) * L::xch_row + (2 * j + (c >> 1)) * 8 + g] = o[j][c];
+        for (int c = 0; c < 4; ++c) sts_f32(to + ((2 * t4 + (c & 1)) * L::xch_row + (2 * j + (c >> 1)) * 8 + g) * 4, o[j][c]);
       if (t4 == 0) {
-        m_s[warp][g] = m_run;
-        l_s[warp][g] = l_run;
+        sts_f32(L::ml + (warp * 8 + g) * 4, m_run);
+        sts_f32(L::ml + ((W + warp) * 8 + g) * 4, l_run);
       }
     }
-    __syncthreads();
-    for (int r = warp; r < nr; r += W) {
+    consumer_barrier<W>();
+    const bool gave_up = lds32(L::flag) != 0;
+    if (warp < nr) {
+      const int r = warp;
       float mx = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-      int at[4];
+      uint32_t at[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         int gg, sl;
         value_slot<VB>(lane * 4 + j, gg, sl);
-        at[j] = sl * 8 + gg;
+        at[j] = L::xch + (r * L::xch_row + sl * 8 + gg) * 4;
       }
-      for (int w = 0; w < HW; ++w) mx = fmaxf(mx, m_s[w][r]);
-      for (int w = 0; w < HW; ++w) {
-        const float fw = m_s[w][r] == -INFINITY ? 1.f : paged_ex2(m_s[w][r] - mx);
-        l += l_s[w][r] * fw;
-        const float* from = reinterpret_cast<const float*>(smem + L::xch) + (w * kPagedRows + r) * L::xch_row;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += from[at[j]] * fw;
+      for (int w = 0; w < HW; ++w) mx = fmaxf(mx, lds_f32(L::ml + (w * 8 + r) * 4));
+#pragma unroll
+      for (int w = 0; w < HW; ++w) {
+        const float mw = lds_f32(L::ml + (w * 8 + r) * 4);
+        const float fw = mw == -INFINITY ? 1.f : paged_ex2(mw - mx);
+        l += lds_f32(L::ml + ((W + w) * 8 + r) * 4) * fw;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += lds_f32(at[j] + w * kPagedRows * L::xch_row * 4) * fw;
       }
-      if (gave_up_s) l = __int_as_float(0x7fc00000);
+      if (gave_up) l = __int_as_float(0x7fc00000);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] *= tb.v_post;
       if (cnt == cur.span.tiles) {
@@ -567,13 +703,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         }
       }
     }
-    __syncthreads();
-    if (gave_up_s) {           // every warp leaves together; its copies still in flight land first (bounded)
-      for (; used < issued; ++used) mbar_wait(bar0 + 8 * (used % S), (used / S) & 1);
-      return;
-    }
-    run += cnt;
-    if (cur.j + cnt == cur.span.tiles) cur.next_group(a);
+    if (gave_up || !more) return;      // all warps agree: the flag is read behind a barrier that every writer passed
+    cur = nx;
+    // the next group's first stores to q, xch and ml come behind a barrier that every reader above has passed
   }
 }
 
@@ -631,12 +763,14 @@ int launch(PagedDecodeArgs& a, const MmaTables& tb, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(L::end - kBase));
     if (e != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
   a.min_tiles = W;
-  paged_mma_kernel<KF, VB, W, S><<<a.ctas, W * 32, L::total, st>>>(a, tb);
+  a.group_cost = W;
+  paged_mma_kernel<KF, VB, W, S><<<a.ctas, (W + 1) * 32, L::end - kBase, st>>>(a, tb);
   const int rc = check_launch("tq_paged_decode");
   return rc ? rc : launch_paged_merge(a, kDim, st);
 }
@@ -649,6 +783,10 @@ bool paged_mma_supported(const PagedDecodeArgs& a, int dim) {
   if (!aligned16(a.v.data) || a.v.page_stride % 4 || a.v.head_stride % 4) return false;
   if (!aligned16(a.v.norms) || a.v.norm_page_stride % 4 || a.v.norm_head_stride % 4) return false;
   if (!aligned16(a.k.data)) return false;
+  // page distances travel as 32-bit byte counts
+  if (a.k.page_stride >= (1ll << 30) || a.v.page_stride >= (1ll << 30) || a.k.norm_page_stride >= (1ll << 30) ||
+      a.v.norm_page_stride >= (1ll << 30))
+    return false;
   if (a.k.format == TQ_KV_DENSE) return a.k.dtype != TQ_F32 && a.k.page_stride % 8 == 0 && a.k.head_stride % 8 == 0;
   return (a.k.bits == 3 || a.k.bits == 4) && a.k.page_stride % 4 == 0 && a.k.head_stride % 4 == 0 && aligned16(a.k.norms) &&
          a.k.norm_page_stride % 4 == 0 && a.k.norm_head_stride % 4 == 0;
@@ -662,6 +800,10 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st) {
   memcpy(tb.v_c16, vb.c16, sizeof(tb.v_c16));
   tb.v_post = 1.0f / vb.beta;
   tb.k_post = a.scale_log2;
+  a.k_page_bytes = (uint32_t)(a.k.page_stride * (a.k.format == TQ_KV_DENSE ? 2 : 4));
+  a.v_page_bytes = (uint32_t)(a.v.page_stride * 4);
+  a.kn_page_bytes = (uint32_t)(a.k.norm_page_stride * 4);
+  a.vn_page_bytes = (uint32_t)(a.v.norm_page_stride * 4);
   if (a.k.format == TQ_KV_POLAR) {
     ScaledBook kb;
     scale_book(a.k.cent.v, 1 << a.k.bits, &kb);
@@ -673,8 +815,8 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st) {
     if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2>(a, tb, st) : launch<KF_BF16, 4, 8, 2>(a, tb, st);
     return v3 ? launch<KF_F16, 3, 8, 2>(a, tb, st) : launch<KF_F16, 4, 8, 2>(a, tb, st);
   }
-  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 12, 4>(a, tb, st) : launch<KF_P3, 4, 12, 2>(a, tb, st);
-  return v3 ? launch<KF_P4, 3, 12, 2>(a, tb, st) : launch<KF_P4, 4, 12, 2>(a, tb, st);
+  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 4>(a, tb, st) : launch<KF_P3, 4, 11, 2>(a, tb, st);
+  return v3 ? launch<KF_P4, 3, 11, 2>(a, tb, st) : launch<KF_P4, 4, 11, 2>(a, tb, st);
 }
 
 }  // namespace tq
