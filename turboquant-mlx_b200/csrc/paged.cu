@@ -29,6 +29,7 @@ int paged_status_ptr(int** out) {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kTile = 32;            // positions per tile of the general kernel: one per lane
 constexpr int kMaxCtas = 256;        // of a decode launch (one per SM)
 
 // ---- general decode -----------------------------------------------------------------------------------
@@ -95,7 +96,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
       for (int j = 0; j < EPL; ++j) o[r][j] = 0.f;
     }
     for (int i = warp; i < cnt; i += kWarps) {
-      const int p0 = cur.span.tile_at(cur.j + i) * kPagedTile, pos = p0 + lane;
+      const int p0 = cur.span.tile_at(cur.j + i) * kTile, pos = p0 + lane;
       const int page = a.view.page_of(b, p0);
       const int row = p0 & ((1 << a.view.page_shift) - 1);
       if (page < 0 && lane == 0) atomicExch(a.view.status, 1);
@@ -147,7 +148,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
       if (page >= 0) {
         const uint32_t* vr = reinterpret_cast<const uint32_t*>(a.v.data) + page * a.v.page_stride + kvh * a.v.head_stride +
                              (int64_t)row * vpd;
-        for (int k = 0; k < kPagedTile; ++k) {
+        for (int k = 0; k < kTile; ++k) {
           if (!cur.span.sees(p0 + k, a.sinks)) continue;
           const float4 wa = *reinterpret_cast<const float4*>(pw + k * kPagedRows);
           const float4 wb = *reinterpret_cast<const float4*>(pw + k * kPagedRows + 4);
@@ -350,8 +351,8 @@ int check_paged_params(const tq_paged_params* p) {
              "struct_bytes %d does not match this library (%zu)", p->struct_bytes, sizeof(tq_paged_params));
   TQ_REQUIRE(p->dim >= 32 && p->dim <= 256 && !(p->dim & (p->dim - 1)), TQ_ERR_BAD_DIM,
              "dim must be a power of 2 in [32, 256], got %d", p->dim);
-  TQ_REQUIRE(p->page_size >= kPagedTile && p->page_size <= (1 << 20) && !(p->page_size & (p->page_size - 1)), TQ_ERR_BAD_ARG,
-             "page_size must be a power of 2, at least %d, got %d", kPagedTile, p->page_size);
+  TQ_REQUIRE(p->page_size >= kMinPage && p->page_size <= (1 << 20) && !(p->page_size & (p->page_size - 1)), TQ_ERR_BAD_ARG,
+             "page_size must be a power of 2, at least %d, got %d", kMinPage, p->page_size);
   TQ_REQUIRE(p->batch > 0 && p->batch <= (1 << 20) && p->n_kv_heads > 0 && p->n_kv_heads <= (1 << 16), TQ_ERR_BAD_ARG,
              "batch and n_kv_heads must be positive (at most 2^20 and 2^16)");
   TQ_REQUIRE(p->n_pages > 0 && p->n_pages < (1ll << 31), TQ_ERR_BAD_ARG, "n_pages must be in [1, 2^31), got %lld",
@@ -461,6 +462,7 @@ extern "C" int tq_paged_decode(const tq_paged_params* p) {
   a.ctas = num_sms() < kMaxCtas ? num_sms() : kMaxCtas;
   cudaStream_t st = (cudaStream_t)p->stream;
   if (paged_mma_supported(a, p->dim)) return launch_paged_mma(a, st);
+  a.tile_shift = 5;
   a.min_tiles = kWarps;
   a.group_cost = 2;
   switch (p->dim) {

@@ -4,9 +4,9 @@
 // positions [i * page, (i + 1) * page) of sequence b.  Pages may be anywhere in the pool and may be shared
 // between sequences (forks), so nothing here assumes an order.
 //
-// The unit of decode work is a tile: 32 consecutive positions of one (sequence, kv head, group of up to 8
-// query heads), which never straddles a page (page sizes are powers of two, 32 at least).  A sequence has
-// only the tiles that its newest token sees: all of them, or with a sliding window the tiles of the first
+// The unit of decode work is a tile: 32 or 64 consecutive positions (the kernel's choice) of one (sequence, kv head,
+// group of up to 8 query heads), which lies in one page, or in two of 32 positions (page sizes are powers of two, 32
+// at least).  A sequence has only the tiles that its newest token sees: all of them, or with a sliding window the tiles of the first
 // `sinks` positions and those from position len - window on.  The tiles of a launch, numbered sequence by
 // sequence, group by group, are cut into runs of equal cost, one per CTA, whatever the lengths of the
 // sequences: a ragged batch loads every SM alike, and a single long sequence is split as finely as it needs.
@@ -20,9 +20,9 @@
 
 namespace tq {
 
-constexpr int kPagedTile = 32;       // positions per tile
+constexpr int kMinPage = 32;         // positions of the smallest page
 constexpr int kPagedRows = 8;        // query heads per group
-constexpr int kPlanEntries = 512;    // prefix entries of a CTA's plan (each covers ceil(batch / 512) sequences)
+constexpr int kPlanEntries = 256;    // prefix entries of a CTA's plan (each covers ceil(batch / 256) sequences)
 constexpr float kPagedLog2e = 1.4426950408889634f;
 
 struct PagedHalf {                   // the K or the V half of a pool
@@ -59,6 +59,7 @@ struct PagedDecodeArgs {
   int batch, n_q_heads, n_kv_heads, n_rep, groups;     // groups = n_kv_heads * ceil(n_rep / 8)
   const int* lens;
   int window, sinks;                 // window 0: every position is visible
+  int tile_shift;                    // tiles have 1 << tile_shift positions
   const void* q;
   int q_dtype, out_dtype;
   int64_t q_batch_stride, q_head_stride;
@@ -85,9 +86,9 @@ __device__ __forceinline__ SeqSpan span_of(const PagedDecodeArgs& a, int b) {
   SeqSpan s;
   s.n = min(max(__ldg(a.lens + b), 0), a.view.capacity());
   s.lo = a.window > 0 ? max(0, s.n - a.window) : 0;
-  const int full = (s.n + kPagedTile - 1) / kPagedTile;
-  s.st = s.lo > 0 ? (int)min(((int64_t)a.sinks + kPagedTile - 1) / kPagedTile, (int64_t)full) : 0;
-  s.wt = max(s.lo / kPagedTile, s.st);
+  const int full = (int)(((int64_t)s.n + (1 << a.tile_shift) - 1) >> a.tile_shift);
+  s.st = s.lo > 0 ? (int)min(((int64_t)a.sinks + (1 << a.tile_shift) - 1) >> a.tile_shift, (int64_t)full) : 0;
+  s.wt = max(s.lo >> a.tile_shift, s.st);
   s.tiles = s.st + full - s.wt;
   return s;
 }

@@ -48,7 +48,7 @@ struct MmaTables {
 constexpr uint32_t kBase = 1024;
 constexpr uint32_t kEnd = 228 * 1024;
 constexpr uint32_t up16(uint32_t x) { return (x + 15) & ~15u; }
-template <int KF, int VB, int W, int S>
+template <int KF, int VB, int W, int S, int H>
 struct Layout {
   static constexpr uint32_t entry = dense(KF) ? 128 : 256;              // bytes between table entries (K and V side by side)
   static constexpr uint32_t v_entry = dense(KF) ? 0 : 128;
@@ -56,10 +56,11 @@ struct Layout {
   static constexpr uint32_t table_bytes = entries * entry;
   static constexpr uint32_t table = table_bytes > 16384 ? table_bytes : 16384, table_end = table + table_bytes;
   static constexpr uint32_t k_off = 0;
-  static constexpr uint32_t kn_off = 32 * k_row_bytes(KF);
-  static constexpr uint32_t v_off = kn_off + (dense(KF) ? 0 : 128);
-  static constexpr uint32_t vn_off = v_off + 32 * v_row_bytes(VB);
-  static constexpr uint32_t stage = vn_off + 128;
+  static constexpr uint32_t tile = 32 * H;                              // positions of a tile
+  static constexpr uint32_t kn_off = tile * k_row_bytes(KF);
+  static constexpr uint32_t v_off = kn_off + (dense(KF) ? 0 : tile * 4);
+  static constexpr uint32_t vn_off = v_off + tile * v_row_bytes(VB);
+  static constexpr uint32_t stage = vn_off + tile * 4;
   // below the table: barriers, scalars, the plan; what does not fit goes behind the table, ring stages fill both sides
   static constexpr uint32_t full = kBase, empty = full + W * S * 8;     // mbarriers of the ring stages
   static constexpr uint32_t info = empty + W * S * 8;                   // per stage: first position of its tile | flags
@@ -68,7 +69,7 @@ struct Layout {
   static constexpr uint32_t flag = ml + 2 * W * 32;
   static constexpr uint32_t prefix = flag + 16;
   static constexpr uint32_t norms = up16(prefix + (kPlanEntries + 1) * 4);   // per warp: key norms, log2 value norms, value norms
-  static constexpr uint32_t q = norms + W * 3 * 32 * 4;                 // query fragments [k-step][lane][4]
+  static constexpr uint32_t q = norms + W * 3 * tile * 4;                 // query fragments [k-step][lane][4]
   static constexpr uint32_t small_end = q + 8 * 32 * 16;
   static constexpr int xch_warps = (W + 1) / 2;
   static constexpr uint32_t xch_row = kDim + 4;                         // padded: conflict-free stores
@@ -226,10 +227,10 @@ __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
 }
 __device__ __forceinline__ void sts_f32(uint32_t addr, float v) { sts32(addr, __float_as_uint(v)); }
 
-template <int KF, int VB, int W, int S>
+template <int KF, int VB, int W, int S, int H>
 __global__ void __launch_bounds__((W + 1) * 32, 1)
 paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constant__ MmaTables tb) {
-  using L = Layout<KF, VB, W, S>;
+  using L = Layout<KF, VB, W, S, H>;
   extern __shared__ __align__(1024) uint8_t smem[];       // shared address kBase
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -275,7 +276,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     const bool polar = !dense(KF);
     const int row_mask = (1 << a.view.page_shift) - 1;
     Cursor fc = cur;                  // the piece the lane's next tile is in
-    int i = lane, cnt = lane < W ? cur.count_to(end) : 0, page = 0;       // cnt 0: the lane has no tile left
+    int i = lane, cnt = lane < W ? cur.count_to(end) : 0;       // cnt 0: the lane has no tile left
+    int page[H];
+    const bool small_page = H == 2 && a.view.page_shift == 5;
     const uint8_t *kb = nullptr, *vb = nullptr, *kn = nullptr, *vn = nullptr;      // the group's head in page 0
     auto bases = [&]() {
       const int head = rg_per_head == 1 ? fc.group : fc.group / rg_per_head;
@@ -296,8 +299,11 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         if (cnt != 0) bases();
       }
       if (cnt != 0) {
-        const int pos = fc.span.tile_at(fc.j + i) * kPagedTile;
-        page = __ldg(a.view.table + fc.b * a.view.table_stride + (pos >> a.view.page_shift));
+        const int pos = fc.span.tile_at(fc.j + i) * L::tile;
+        const int* entry = a.view.table + fc.b * a.view.table_stride + (pos >> a.view.page_shift);
+        page[0] = __ldg(entry);
+        // pages of 32 under tiles of 64: the second half has an entry of its own, if the sequence reaches it
+        if (H == 2 && small_page) page[H - 1] = pos + 32 < fc.span.n ? __ldg(entry + 1) : -1;
       }
     };
     bases();
@@ -307,21 +313,40 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     while (__any_sync(0xffffffffu, cnt != 0)) {
       const bool go = cnt != 0 && mbar_try(L::empty + 8 * (lane * S + s), phase);
       if (go) {
-        const bool ok = page >= 0 && page < a.view.n_pages;
-        const int pos = fc.span.tile_at(fc.j + i) * kPagedTile;
-        const bool full = pos + kPagedTile <= fc.span.n && (pos >= fc.span.lo || pos + kPagedTile <= a.sinks);
+        const int pos = fc.span.tile_at(fc.j + i) * L::tile;
         const uint32_t bar = L::full + 8 * (lane * S + s), st = stage_addr(lane, s);
-        sts32(L::info + 4 * (lane * S + s), (uint32_t)pos | (full && ok ? 1u : 0u) | (ok ? 0u : 2u));
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(ok ? L::stage : 0u) : "memory");
-        if (ok) {
-          const uint64_t pg = (uint32_t)page;
-          const uint32_t row = pos & row_mask;
-          bulk_g2s(st + L::k_off, kb + pg * a.k_page_bytes + row * k_row_bytes(KF), 32 * k_row_bytes(KF), bar);
-          if (polar) bulk_g2s(st + L::kn_off, kn + pg * a.kn_page_bytes + row * 4, 128, bar);
-          bulk_g2s(st + L::v_off, vb + pg * a.v_page_bytes + row * v_row_bytes(VB), 32 * v_row_bytes(VB), bar);
-          bulk_g2s(st + L::vn_off, vn + pg * a.vn_page_bytes + row * 4, 128, bar);
+        // copies `n` positions from row `row` of page `pg` behind position `at` of the stage
+        auto copy = [&](uint32_t pg, uint32_t row, uint32_t at, uint32_t n) {
+          bulk_g2s(st + L::k_off + at * k_row_bytes(KF), kb + (uint64_t)pg * a.k_page_bytes + row * k_row_bytes(KF), n * k_row_bytes(KF), bar);
+          if (polar) bulk_g2s(st + L::kn_off + at * 4, kn + (uint64_t)pg * a.kn_page_bytes + row * 4, n * 4, bar);
+          bulk_g2s(st + L::v_off + at * v_row_bytes(VB), vb + (uint64_t)pg * a.v_page_bytes + row * v_row_bytes(VB), n * v_row_bytes(VB), bar);
+          bulk_g2s(st + L::vn_off + at * 4, vn + (uint64_t)pg * a.vn_page_bytes + row * 4, n * 4, bar);
+        };
+        const bool full = pos + (int)L::tile <= fc.span.n && (pos >= fc.span.lo || pos + (int)L::tile <= a.sinks);
+        if (!small_page) {
+          const bool ok = page[0] >= 0 && page[0] < a.view.n_pages;
+          sts32(L::info + 4 * (lane * S + s), (uint32_t)pos | (ok ? (full ? 1u : 0u) : 6u));
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(ok ? L::stage : 0u) : "memory");
+          if (ok) copy(page[0], pos & row_mask, 0, L::tile);
+          else atomicExch(a.view.status, 1);
         } else {
-          atomicExch(a.view.status, 1);
+          // a half that the token does not see needs no page; one that it sees and that has none is missing
+          uint32_t flags = full ? 1u : 0u, have = 0;
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            const int p = pos + 32 * h;
+            const bool seen = p < fc.span.n && (p + 32 > fc.span.lo || p < a.sinks);
+            const bool ok = page[h] >= 0 && page[h] < a.view.n_pages;
+            if (seen && ok) have |= 1u << h;
+            if (seen && !ok) flags = (flags & ~1u) | (2u << h);
+          }
+          if (flags & 6u) atomicExch(a.view.status, 1);
+          sts32(L::info + 4 * (lane * S + s), (uint32_t)pos | flags);
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                       "r"((uint32_t)__popc(have) * (L::stage / H)) : "memory");
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            if ((have >> h) & 1u) copy(page[h], 0, 32 * h, 32);
         }
         ++issued;
         if (++s == S) {
@@ -353,7 +378,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   constexpr bool kSwap = VB == 4;
   const int k_row0 = 8 * (g >> 1) + ((g & 1) ^ (kSwap ? (g >> 1) & 1 : 0));
   const int v_row0 = 8 * t4 + (kSwap ? t4 & 1 : 0), v_row1 = 8 * t4 + 1 - (kSwap ? t4 & 1 : 0);
-  const uint32_t nrm = L::norms + warp * 384;
+  const uint32_t nrm = L::norms + warp * 3 * L::tile * 4;      // [3][tile]
   const uint32_t nrm_at = nrm + 4 * (kSwap ? lane ^ ((lane >> 3) & 1) : lane);      // the place of position `lane` in that order
   uint32_t lut_lane;                                     // table address of entry 0 in this lane's copy; opaque, so that
   asm("add.u32 %0, %1, %2;" : "=r"(lut_lane) : "r"(lane4), "n"(L::table));   // an address stays one logic operation
@@ -374,16 +399,20 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   int us = 0;                        // stage of the tile consumed next
   uint32_t phase = 0;
   int i = warp;
-  // the group's query rows, four elements of row `warp` per lane: fetched a group ahead
-  auto load_query = [&](const Cursor& c, float (&x)[4]) {
-    const int kvh = rg_per_head == 1 ? c.group : c.group / rg_per_head, rr = (c.group - kvh * rg_per_head) * kPagedRows + warp;
+  // the group's query rows, four elements of rows warp, warp + W per lane: fetched a group ahead
+  constexpr int kRpw = (kPagedRows + W - 1) / W;
+  auto load_query = [&](const Cursor& c, float (&x)[kRpw][4]) {
+    const int kvh = rg_per_head == 1 ? c.group : c.group / rg_per_head;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x[j] = warp < kPagedRows && rr < a.n_rep
-                 ? load_elem(a.q, a.q_dtype, c.b * a.q_batch_stride + (kvh * a.n_rep + rr) * a.q_head_stride + lane * 4 + j) : 0.f;
+    for (int k = 0; k < kRpw; ++k) {
+      const int r = warp + k * W, rr = (c.group - kvh * rg_per_head) * kPagedRows + r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[k][j] = r < kPagedRows && rr < a.n_rep
+                      ? load_elem(a.q, a.q_dtype, c.b * a.q_batch_stride + (kvh * a.n_rep + rr) * a.q_head_stride + lane * 4 + j) : 0.f;
+    }
   };
-  static_assert(W >= kPagedRows, "a warp per query row");
-  float xq[4];
+  float xq[kRpw][4];
   load_query(cur, xq);
   while (true) {
     const int cnt = cur.count_to(end);
@@ -391,9 +420,11 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     const int r0 = (cur.group - kvh * rg_per_head) * kPagedRows;
     const int nr = min(kPagedRows, a.n_rep - r0), h0 = kvh * a.n_rep + r0;
     // ---------------- query fragments ----------------
-    if (warp < kPagedRows) {
-      const int r = warp;
-      float x[4] = {xq[0], xq[1], xq[2], xq[3]};
+#pragma unroll
+    for (int k = 0; k < kRpw; ++k) {
+      const int r = warp + k * W;
+      if (r >= kPagedRows) break;
+      float x[4] = {xq[k][0], xq[k][1], xq[k][2], xq[k][3]};
       if (!dense(KF)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] *= sign_at(a.k.signs, lane * 4 + j);
@@ -447,20 +478,21 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       const uint32_t info = lds32(L::info + 4 * (warp * S + us));
       const int p0 = info & ~31u;
       const bool full = info & 1u;
-      {   // norms: lane = position
-        const bool seen = full || cur.span.sees(p0 + lane, a.sinks);
-        const float vn = seen ? lds_f32(st + L::vn_off + lane4) : 0.f;
-        if (!dense(KF)) sts32(nrm_at, lds32(st + L::kn_off + lane4));
-        sts_f32(nrm_at + 128, lg2(fmaxf(vn, 1e-26f)));
-        sts_f32(nrm_at + 256, vn);
-        __syncwarp();
-      }
-      // ---------------- scores ----------------
-      float sc[4][4];
 #pragma unroll
-      for (int ng = 0; ng < 4; ++ng) {
+      for (int h = 0; h < H; ++h) {   // norms: lane = position
+        const bool seen = full || cur.span.sees(p0 + 32 * h + lane, a.sinks);
+        const float vn = seen ? lds_f32(st + L::vn_off + lane4 + 128 * h) : 0.f;
+        if (!dense(KF)) sts32(nrm_at + 128 * h, lds32(st + L::kn_off + lane4 + 128 * h));
+        sts_f32(nrm_at + 128 * h + L::tile * 4, lg2(fmaxf(vn, 1e-26f)));
+        sts_f32(nrm_at + 128 * h + L::tile * 8, vn);
+      }
+      __syncwarp();
+      // ---------------- scores ----------------
+      float sc[4 * H][4];
+#pragma unroll
+      for (int ng = 0; ng < 4 * H; ++ng) {
         sc[ng][0] = sc[ng][1] = sc[ng][2] = sc[ng][3] = 0.f;
-        const uint32_t row = st + L::k_off + (k_row0 + 2 * ng) * k_row_bytes(KF);
+        const uint32_t row = st + L::k_off + (32 * (ng >> 2) + k_row0 + 2 * (ng & 3)) * k_row_bytes(KF);
         if (dense(KF)) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
@@ -490,13 +522,13 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         }
       }
       // value fragments of one k-step (two position pairs per thread)
-      auto load_values = [&](int half, uint32_t (&af)[8][4]) {
+      auto load_values = [&](int step, uint32_t (&af)[8][4]) {
         uint32_t off[2][16];          // table addresses of the 16 slots, for the two position pairs of this k-step
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int ng = 2 * half + p;
-          const uint32_t r0p = st + L::v_off + (v_row0 + 2 * ng) * v_row_bytes(VB);
-          const uint32_t r1p = st + L::v_off + (v_row1 + 2 * ng) * v_row_bytes(VB);
+          const int vrow = 32 * (step >> 1) + 4 * (step & 1) + 2 * p;
+          const uint32_t r0p = st + L::v_off + (v_row0 + vrow) * v_row_bytes(VB);
+          const uint32_t r1p = st + L::v_off + (v_row1 + vrow) * v_row_bytes(VB);
           if (VB == 4) {
             const uint2 x = lds64(r0p + 8 * g), y = lds64(r1p + 8 * g);
             const uint32_t xs[2] = {x.x, x.y}, ys[2] = {y.x, y.y};
@@ -541,45 +573,39 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           af[j][3] = v_lut(off[1][2 * j + 1]);
         }
       };
-      // the first half's lookups wait for nothing: they fill the time the score products and the softmax take
+      // the first step's lookups wait for nothing: they fill the time the score products and the softmax take
       uint32_t af0[8][4];
       load_values(0, af0);
-      // ---------------- softmax: head g, positions 8 t4 + 2 ng + c in this tile's order ----------------
-      const bool missing = info & 2u;
-      float kn[8], lv[8], vn[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t at = nrm + 32 * t4 + 16 * h;
-        const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + 128), z = lds128(at + 256);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          kn[4 * h + k] = __uint_as_float(xs[k]);
-          lv[4 * h + k] = __uint_as_float(ys[k]);
-          vn[4 * h + k] = __uint_as_float(zs[k]);
-        }
-      }
-      float s2[8], top = -INFINITY;
+      // ---------------- softmax: head g, positions 32 h + 8 t4 + 2 (ng & 3) + c in this tile's order ----------------
+      float s2[8 * H], vn[8 * H], top = -INFINITY;
       const float2 post2 = make_float2(post, post);
 #pragma unroll
-      for (int k = 0; k < 8; k += 2) {       // high part and residual of the query, scale, key norm
-        float2 x = mul2(add2(make_float2(sc[k >> 1][0], sc[k >> 1][1]), make_float2(sc[k >> 1][2], sc[k >> 1][3])), post2);
-        if (!dense(KF)) x = mul2(x, make_float2(kn[k], kn[k + 1]));
-        s2[k] = x.x;
-        s2[k + 1] = x.y;
-      }
-      if (!full) {
+      for (int q4 = 0; q4 < 2 * H; ++q4) {       // four positions at a time: high part and residual of the query, scale, key norm
+        const uint32_t at = nrm + 128 * (q4 >> 1) + 32 * t4 + 16 * (q4 & 1);
+        const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + L::tile * 4), z = lds128(at + L::tile * 8);
+        const float kn[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
+        const float lv[4] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w)};
+        vn[4 * q4] = __uint_as_float(z.x);
+        vn[4 * q4 + 1] = __uint_as_float(z.y);
+        vn[4 * q4 + 2] = __uint_as_float(z.z);
+        vn[4 * q4 + 3] = __uint_as_float(z.w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int pos = p0 + ((k & 1) ? v_row1 : v_row0) + (k & 6);
-          if (missing) s2[k] = __int_as_float(0x7fc00000);
-          else if (!cur.span.sees(pos, a.sinks)) s2[k] = -INFINITY;
+        for (int k = 0; k < 4; k += 2) {
+          const float (&c)[4] = sc[2 * q4 + k / 2];
+          float2 v = mul2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), post2);
+          if (!dense(KF)) v = mul2(v, make_float2(kn[k], kn[k + 1]));
+          if (!full) {
+            const int h = q4 >> 1, pos = p0 + 32 * h + 4 * (q4 & 1) + k;
+            const bool missing = (info >> (1 + h)) & 1u;
+            if (!cur.span.sees(pos + v_row0, a.sinks)) v.x = -INFINITY;
+            if (!cur.span.sees(pos + v_row1, a.sinks)) v.y = -INFINITY;
+            if (missing) v.x = v.y = __int_as_float(0x7fc00000);
+          }
+          s2[4 * q4 + k] = v.x;
+          s2[4 * q4 + k + 1] = v.y;
+          const float2 u = add2(v, make_float2(lv[k], lv[k + 1]));
+          top = fmaxf(top, fmaxf(u.x, u.y));
         }
-      }
-#pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        const float2 x = add2(make_float2(s2[k], s2[k + 1]), make_float2(lv[k], lv[k + 1]));
-        top = fmaxf(top, fmaxf(x.x, x.y));
       }
       if (__any_sync(0xffffffffu, top > m_run + kRescale)) {       // also for the first visible tile
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -596,9 +622,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         }
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
-      uint32_t pb[4];
+      uint32_t pb[4 * H];
 #pragma unroll
-      for (int ng = 0; ng < 4; ++ng) {
+      for (int ng = 0; ng < 4 * H; ++ng) {
         const float2 d = add2(make_float2(s2[2 * ng], s2[2 * ng + 1]), make_float2(-m_use, -m_use));
         const float2 e = make_float2(paged_ex2(d.x), paged_ex2(d.y));
         l_run += e.x + e.y;
@@ -607,12 +633,17 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         pb[ng] = *reinterpret_cast<const uint32_t*>(&h);
       }
       // ---------------- values ----------------
-      uint32_t af1[8][4];
-      load_values(1, af1);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mma<false>(o[j], af0[j], pb[0], pb[1]);
+      for (int step = 0; step < 2 * H; ++step) {
+        uint32_t af1[8][4];
+        if (step + 1 < 2 * H) load_values(step + 1, af1);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mma<false>(o[j], af1[j], pb[2], pb[3]);
+        for (int j = 0; j < 8; ++j) mma<false>(o[j], af0[j], pb[2 * step], pb[2 * step + 1]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) af0[j][c] = af1[j][c];
+      }
       __syncwarp();            // every lane is done with the stage (and with the norms)
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(L::empty + 8 * (warp * S + us)) : "memory");
       if (++us == S) {
@@ -668,8 +699,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     }
     consumer_barrier<W>();
     const bool gave_up = lds32(L::flag) != 0;
-    if (warp < nr) {
-      const int r = warp;
+    for (int r = warp; r < nr; r += W) {
       float mx = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t at[4];
 #pragma unroll
@@ -756,21 +786,22 @@ void scale_book(const float* c, int n, ScaledBook* out) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int KF, int VB, int W, int S>
+template <int KF, int VB, int W, int S, int H>
 int launch(PagedDecodeArgs& a, const MmaTables& tb, cudaStream_t st) {
-  using L = Layout<KF, VB, W, S>;
+  using L = Layout<KF, VB, W, S, H>;
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)(L::end - kBase));
     if (e != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
+  a.tile_shift = H == 2 ? 6 : 5;
   a.min_tiles = W;
   a.group_cost = W;
-  paged_mma_kernel<KF, VB, W, S><<<a.ctas, (W + 1) * 32, L::end - kBase, st>>>(a, tb);
+  paged_mma_kernel<KF, VB, W, S, H><<<a.ctas, (W + 1) * 32, L::end - kBase, st>>>(a, tb);
   const int rc = check_launch("tq_paged_decode");
   return rc ? rc : launch_paged_merge(a, kDim, st);
 }
@@ -812,11 +843,11 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st) {
   }
   const bool v3 = a.v.bits == 3;
   if (a.k.format == TQ_KV_DENSE) {
-    if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2>(a, tb, st) : launch<KF_BF16, 4, 8, 2>(a, tb, st);
-    return v3 ? launch<KF_F16, 3, 8, 2>(a, tb, st) : launch<KF_F16, 4, 8, 2>(a, tb, st);
+    if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2, 1>(a, tb, st) : launch<KF_BF16, 4, 8, 2, 1>(a, tb, st);
+    return v3 ? launch<KF_F16, 3, 8, 2, 1>(a, tb, st) : launch<KF_F16, 4, 8, 2, 1>(a, tb, st);
   }
-  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 4>(a, tb, st) : launch<KF_P3, 4, 11, 2>(a, tb, st);
-  return v3 ? launch<KF_P4, 3, 11, 2>(a, tb, st) : launch<KF_P4, 4, 11, 2>(a, tb, st);
+  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 2, 2>(a, tb, st) : launch<KF_P3, 4, 7, 2, 2>(a, tb, st);
+  return v3 ? launch<KF_P4, 3, 7, 2, 2>(a, tb, st) : launch<KF_P4, 4, 7, 2, 2>(a, tb, st);
 }
 
 }  // namespace tq
