@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import weakref
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
@@ -71,6 +72,19 @@ class FlashParams(ctypes.Structure):
     ]
 
 
+def _layout(cls, prefix=""):
+    """struct-module format of a ctypes structure (native sizes, no implicit padding: the fields are checked to be
+    packed), so that a whole argument block is filled by one call."""
+    codes = {c_int32: "i", c_int64: "q", c_void_p: "Q", c_float: "f", POINTER(c_float): "Q"}
+    out, at = "", 0
+    for name, kind in cls._fields_:
+        assert getattr(cls, name).offset == at, f"{cls.__name__}.{name} is not packed"
+        at += ctypes.sizeof(kind)
+        out += _layout(kind) if issubclass(kind, ctypes.Structure) else codes[kind]
+    assert at == ctypes.sizeof(cls)
+    return out
+
+
 class PagedHalf(ctypes.Structure):
     """Mirror of `tq_paged_half` (include/tqb200.h)."""
 
@@ -101,6 +115,8 @@ class PagedParams(ctypes.Structure):
         ("k", PagedHalf), ("v", PagedHalf),
     ]
 
+
+PAGED_PARAMS = struct.Struct("=" + _layout(PagedParams))
 
 _lib = None
 
@@ -150,11 +166,11 @@ _SIGNATURES = {
     "tq_set_peer_wait_limit_ms": (c_int, [c_int]),
     "tq_peer_push": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p), c_int, c_uint32, c_void_p]),
     "tq_peer_wait": (c_int, [c_void_p, c_int, c_uint32, c_void_p, c_void_p]),
-    "tq_paged_append": (c_int, [POINTER(PagedParams)]),
+    "tq_paged_append": (c_int, [c_void_p]),
     "tq_paged_decode_workspace_bytes": (c_int64, [c_int]),
-    "tq_paged_decode": (c_int, [POINTER(PagedParams)]),
-    "tq_paged_dequantize": (c_int, [POINTER(PagedParams)]),
-    "tq_copy_pages": (c_int, [POINTER(c_void_p), POINTER(c_int64), c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "tq_paged_decode": (c_int, [c_void_p]),
+    "tq_paged_dequantize": (c_int, [c_void_p]),
+    "tq_copy_pages": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
     "tq_paged_status": (c_int, [POINTER(c_int), c_void_p]),
     "tq_prefill_sdpa_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                        c_int64, c_int64, c_int] + [c_int64] * 12

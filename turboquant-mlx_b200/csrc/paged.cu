@@ -56,6 +56,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
     kc_s[threadIdx.x] = a.k.cent.v[threadIdx.x];
     vc_s[threadIdx.x] = a.v.cent.v[threadIdx.x];
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   plan_costs(a, prefix);
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
@@ -203,79 +204,105 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
 }
 
 // ---- merge -----------------------------------------------------------------------------------------------
-// One block per (kv head and row group, sequence): joins the partial states of the CTAs that share the
-// group, warp r row r: m = max m_i, l = sum l_i 2^(m_i - m), acc likewise.  Groups of one CTA are already
-// written; a sequence without tiles gets zeros here.
-template <int EPL>
+// Joins the partial states of the CTAs that share a group: m = max m_i, l = sum l_i 2^(m_i - m), acc likewise.  Groups of
+// one CTA are already written; a sequence without tiles gets zeros here.  With many groups each has few parts: a block
+// takes a group, a warp a row (ROWS = 8).  With few groups each may have a hundred: a block takes one row, its warps
+// share the parts and meet in shared memory (ROWS = 1).  Whole call: 4 groups of 37 parts 23.4 us with ROWS = 8, 17.4
+// with 1; 128 groups of 2 or 3 parts 34.0 and 39.1 us.
+template <int EPL, int ROWS>
 __global__ void __launch_bounds__(kPagedRows * 32)
 paged_merge_kernel(const PagedDecodeArgs a) {
   constexpr int DIM = EPL * 32;
   constexpr int kBatch = 8;          // partial states whose rows a lane has in flight
+  constexpr int kShare = kPagedRows / ROWS;            // warps per row
   __shared__ int prefix[kPlanEntries + 1];
-  __shared__ float w_s[kPagedRows][kMaxCtas];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int group = blockIdx.x, rg_per_head = a.groups / a.n_kv_heads;
+  __shared__ float w_s[ROWS][kMaxCtas];
+  __shared__ float acc_s[kShare][DIM];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = ROWS == 1 ? warp : 0;
+  const int group = blockIdx.x / (kPagedRows / ROWS), rg_per_head = a.groups / a.n_kv_heads;
+  const int row = ROWS == 1 ? (int)blockIdx.x % kPagedRows : warp;
+  // The kernel in front has itself waited for what wrote the lengths, so the plan may be made before its end; its
+  // partial states, and the output, have to wait for it.
   plan_costs(a, prefix);
   const Plan plan = make_paged_plan(a, prefix);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int kvh = group / rg_per_head, r0 = (group % rg_per_head) * kPagedRows;
-  if (warp >= min(kPagedRows, a.n_rep - r0)) return;
-  const int head = kvh * a.n_rep + r0 + warp;
+  const bool live = row < min(kPagedRows, a.n_rep - r0);
+  const int head = kvh * a.n_rep + r0 + row;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
     const SeqSpan span = span_of(a, b);
     float v[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) v[j] = 0.f;
     if (span.tiles == 0) {
-      finish_row<EPL>(a, b, head, v, 0.f, lane);
+      if (live && share == 0) finish_row<EPL>(a, b, head, v, 0.f, lane);
       continue;
     }
     const int64_t first = (int64_t)cost_before(a, prefix, b) * a.groups + (int64_t)group * cost_of(a, span) + a.group_cost;
     const int c0 = plan.owner(first), c1 = plan.owner(first + span.tiles - 1);
     if (c0 == c1) continue;
     // the group's first CTA left its tail piece (slot 1), the others their head pieces (slot 0)
-    auto slot = [&](int c) { return a.part + ((int64_t)(2 * c + (c == c0)) * kPagedRows + warp) * (DIM + 2); };
+    auto slot = [&](int c) { return a.part + ((int64_t)(2 * c + (c == c0)) * kPagedRows + row) * (DIM + 2); };
     const int n = c1 - c0 + 1;
     float mx = -INFINITY, l = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      const float m = __ldcg(slot(c0 + i) + DIM);
-      w_s[warp][i] = m;
-      mx = fmaxf(mx, m);
-    }
-    mx = warp_max(mx);
-    for (int i = lane; i < n; i += 32) {
-      const float m = w_s[warp][i], li = __ldcg(slot(c0 + i) + DIM + 1);
-      const float f = m == -INFINITY ? 1.f : paged_ex2(m - mx);      // m = -inf: l is 0, or NaN (a missing page)
-      w_s[warp][i] = f;
-      l += li * f;
-    }
-    l = warp_sum(l);
-    __syncwarp();
-    for (int i0 = 0; i0 < n; i0 += kBatch) {
-      float x[kBatch][EPL];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const float* p = slot(c0 + min(i0 + k, n - 1)) + lane * EPL;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
+    float* w = w_s[ROWS == 1 ? 0 : warp];
+    if (live) {                        // every warp of a row works out all weights: no exchange, the parts are in the L2
+      for (int i = lane; i < n; i += 32) mx = fmaxf(mx, __ldcg(slot(c0 + i) + DIM));
+      mx = warp_max(mx);
+      for (int i = lane; i < n; i += 32) {
+        const float m = __ldcg(slot(c0 + i) + DIM), li = __ldcg(slot(c0 + i) + DIM + 1);
+        const float f = m == -INFINITY ? 1.f : paged_ex2(m - mx);      // m = -inf: l is 0, or NaN (a missing page)
+        w[i] = f;                      // warps of one row store the same value
+        l += li * f;
       }
+      l = warp_sum(l);
+      __syncwarp();
+      for (int i0 = share * kBatch; i0 < n; i0 += kBatch * kShare) {
+        float x[kBatch][EPL];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const float f = i0 + k < n ? w_s[warp][i0 + k] : 0.f;
+        for (int k = 0; k < kBatch; ++k) {
+          const float* p = slot(c0 + min(i0 + k, n - 1)) + lane * EPL;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j)
-          if (i0 + k < n) v[j] += x[k][j] * f;
+          for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float f = i0 + k < n ? w[i0 + k] : 0.f;
+#pragma unroll
+          for (int j = 0; j < EPL; ++j)
+            if (i0 + k < n) v[j] += x[k][j] * f;
+        }
       }
     }
-    finish_row<EPL>(a, b, head, v, l, lane);
-    __syncwarp();
+    if (ROWS == 1) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) acc_s[share][lane * EPL + j] = v[j];
+      __syncthreads();
+      if (share == 0) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          v[j] = 0.f;
+#pragma unroll
+          for (int s = 0; s < kShare; ++s) v[j] += acc_s[s][lane * EPL + j];
+        }
+      }
+    }
+    if (live && share == 0) finish_row<EPL>(a, b, head, v, l, lane);
+    if (ROWS == 1) __syncthreads();
+    else __syncwarp();
   }
 }
 
 template <int EPL>
 int launch_merge_t(const PagedDecodeArgs& a, cudaStream_t st) {
-  const dim3 grid(a.groups, a.batch < 32768 ? a.batch : 32768);
-  paged_merge_kernel<EPL><<<grid, kPagedRows * 32, 0, st>>>(a);
-  return check_launch("tq_paged_decode (merge)");
+  const unsigned batch = a.batch < 32768 ? a.batch : 32768;
+  if ((int64_t)a.groups * a.batch * kPagedRows >= a.ctas)       // at most about nine parts per group
+    return launch_dependent("tq_paged_decode (merge)", paged_merge_kernel<EPL, kPagedRows>, dim3(a.groups, batch), kPagedRows * 32,
+                            0, st, a);
+  return launch_dependent("tq_paged_decode (merge)", paged_merge_kernel<EPL, 1>, dim3(a.groups * kPagedRows, batch),
+                          kPagedRows * 32, 0, st, a);
 }
 
 template <int EPL>
@@ -290,8 +317,7 @@ int launch_general(const PagedDecodeArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
   }
-  paged_decode_general_kernel<EPL><<<a.ctas, kWarps * 32, smem, st>>>(a);
-  int rc = check_launch("tq_paged_decode (general)");
+  const int rc = launch_dependent("tq_paged_decode (general)", paged_decode_general_kernel<EPL>, dim3(a.ctas), kWarps * 32, smem, st, a);
   return rc ? rc : launch_merge_t<EPL>(a, st);
 }
 

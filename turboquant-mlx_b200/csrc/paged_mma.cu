@@ -15,9 +15,8 @@
 // At the end of a group the warps meet in shared memory; a group that lies in one CTA is finished there (butterfly,
 // signs, / dim / l), otherwise its partial state goes to the workspace and paged_merge_kernel joins it.
 //
-// Positions of a tile are dealt to MMA columns so that thread t of a quad owns 8 consecutive ones (norms come in two
-// 16-byte loads); with 4-bit values the two positions of a pair change places in every other block of 8, which halves
-// the bank conflicts of the 64-byte value rows.
+// Positions of a tile are dealt to MMA columns so that thread t of a quad owns 8 consecutive ones of each 32: norms come
+// in 16-byte loads, and the rows that the threads of a warp read together lie in different banks where they can.
 #include <cuda_fp16.h>
 #include <string.h>
 
@@ -236,7 +235,8 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   const int g = lane >> 2, t4 = lane & 3;
   const uint32_t lane4 = lane * 4;
   int* prefix = reinterpret_cast<int*>(smem + L::prefix - kBase);
-  if (smem_u32(smem) != kBase) {         // the layout above would not hold
+  if (smem_u32(smem) != kBase) {         // the layout above would not hold (the launcher has checked that it does)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0) atomicExch(a.view.status, 4);
     return;
   }
@@ -260,14 +260,25 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     }
     if (e < (1u << (2 * VB))) sts32(at + L::v_entry, (uint32_t)tb.v_c16[e & ((1 << VB) - 1)] | ((uint32_t)tb.v_c16[e >> VB] << 16));
   }
+  // Everything above overlaps the end of the kernel in front; everything below may read what that kernel wrote.  The
+  // merge is not let in early: its blocks beside the running ones cost more than their start (34 against 23 us for one
+  // sequence of 32768 tokens with 16-bit keys).
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   plan_costs(a, prefix);          // also the barrier behind the tables
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
   const int rg_per_head = a.groups / a.n_kv_heads;
-  Cursor cur, end;
-  cur.seek(a, prefix, plan.begin(cta));
-  end.seek(a, prefix, plan.begin(cta + 1));
+  // both ends of the run, found by a warp each (the exchange area is free until the first group ends)
+  Cursor* ends = reinterpret_cast<Cursor*>(smem + L::xch - kBase);
+  if (warp < 2) {
+    Cursor c;
+    c.seek(a, prefix, plan.begin(cta + warp));
+    if (lane == 0) ends[warp] = c;
+  }
+  __syncthreads();
+  Cursor cur = ends[0];
+  const Cursor end = ends[1];
   if (cur.at(end)) return;
 
   // ---------------- producer: lane w fetches for warp w ----------------
@@ -374,10 +385,13 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     return;
   }
 
-  // this thread's rows of a tile: key row of n-group ng: k_row0 + 2 ng; value rows of its ng-th pair: v_row0 + 2 ng, v_row1 + 2 ng
+  // Which position of a block of 32 column 2 t + c of n-group ng stands for: 8 t + (kNg ng + kC c), the places of two
+  // neighbouring positions exchanged for odd t with kSwap.  3-bit rows are 13 words long: with c 4 rows apart the key
+  // words of a load lie in 32 different banks; with 64-byte value rows the exchange halves the conflicts.
   constexpr bool kSwap = VB == 4;
-  const int k_row0 = 8 * (g >> 1) + ((g & 1) ^ (kSwap ? (g >> 1) & 1 : 0));
-  const int v_row0 = 8 * t4 + (kSwap ? t4 & 1 : 0), v_row1 = 8 * t4 + 1 - (kSwap ? t4 & 1 : 0);
+  constexpr int kNg = KF == KF_P3 && VB == 3 ? 1 : 2, kC = KF == KF_P3 && VB == 3 ? 4 : 1;
+  const int k_row0 = 8 * (g >> 1) + kC * ((g & 1) ^ (kSwap ? (g >> 1) & 1 : 0));
+  const int v_row0 = 8 * t4 + kC * (kSwap ? t4 & 1 : 0), v_row1 = 8 * t4 + kC * (1 - (kSwap ? t4 & 1 : 0));
   const uint32_t nrm = L::norms + warp * 3 * L::tile * 4;      // [3][tile]
   const uint32_t nrm_at = nrm + 4 * (kSwap ? lane ^ ((lane >> 3) & 1) : lane);      // the place of position `lane` in that order
   uint32_t lut_lane;                                     // table address of entry 0 in this lane's copy; opaque, so that
@@ -492,7 +506,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
 #pragma unroll
       for (int ng = 0; ng < 4 * H; ++ng) {
         sc[ng][0] = sc[ng][1] = sc[ng][2] = sc[ng][3] = 0.f;
-        const uint32_t row = st + L::k_off + (32 * (ng >> 2) + k_row0 + 2 * (ng & 3)) * k_row_bytes(KF);
+        const uint32_t row = st + L::k_off + (32 * (ng >> 2) + k_row0 + kNg * (ng & 3)) * k_row_bytes(KF);
         if (dense(KF)) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
@@ -526,7 +540,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         uint32_t off[2][16];          // table addresses of the 16 slots, for the two position pairs of this k-step
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int vrow = 32 * (step >> 1) + 4 * (step & 1) + 2 * p;
+          const int vrow = 32 * (step >> 1) + kNg * (2 * (step & 1) + p);
           const uint32_t r0p = st + L::v_off + (v_row0 + vrow) * v_row_bytes(VB);
           const uint32_t r1p = st + L::v_off + (v_row1 + vrow) * v_row_bytes(VB);
           if (VB == 4) {
@@ -576,34 +590,43 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       // the first step's lookups wait for nothing: they fill the time the score products and the softmax take
       uint32_t af0[8][4];
       load_values(0, af0);
-      // ---------------- softmax: head g, positions 32 h + 8 t4 + 2 (ng & 3) + c in this tile's order ----------------
-      float s2[8 * H], vn[8 * H], top = -INFINITY;
+      // ---------------- softmax: head g ----------------
+      float s2[8 * H], vn[8 * H], top = -INFINITY;       // [4 h + n-group][c]
       const float2 post2 = make_float2(post, post);
 #pragma unroll
-      for (int q4 = 0; q4 < 2 * H; ++q4) {       // four positions at a time: high part and residual of the query, scale, key norm
-        const uint32_t at = nrm + 128 * (q4 >> 1) + 32 * t4 + 16 * (q4 & 1);
-        const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + L::tile * 4), z = lds128(at + L::tile * 8);
-        const float kn[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
-        const float lv[4] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w)};
-        vn[4 * q4] = __uint_as_float(z.x);
-        vn[4 * q4 + 1] = __uint_as_float(z.y);
-        vn[4 * q4 + 2] = __uint_as_float(z.z);
-        vn[4 * q4 + 3] = __uint_as_float(z.w);
+      for (int h = 0; h < H; ++h) {
+        // norms of this thread's 8 positions of the block, in the order of the tile
+        float kn[8], lv[8], vo[8];
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          const float (&c)[4] = sc[2 * q4 + k / 2];
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t at = nrm + 128 * h + 32 * t4 + 16 * q;
+          const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + L::tile * 4), z = lds128(at + L::tile * 8);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            kn[4 * q + k] = __uint_as_float(xs[k]);
+            lv[4 * q + k] = __uint_as_float(ys[k]);
+            vo[4 * q + k] = __uint_as_float(zs[k]);
+          }
+        }
+#pragma unroll
+        for (int ng = 0; ng < 4; ++ng) {     // high part and residual of the query, scale, key norm
+          const int i0 = kNg * ng, i1 = kNg * ng + kC, to = 8 * h + 2 * ng;
+          const float (&c)[4] = sc[4 * h + ng];
           float2 v = mul2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), post2);
-          if (!dense(KF)) v = mul2(v, make_float2(kn[k], kn[k + 1]));
+          if (!dense(KF)) v = mul2(v, make_float2(kn[i0], kn[i1]));
           if (!full) {
-            const int h = q4 >> 1, pos = p0 + 32 * h + 4 * (q4 & 1) + k;
+            const int pos = p0 + 32 * h + kNg * ng;
             const bool missing = (info >> (1 + h)) & 1u;
             if (!cur.span.sees(pos + v_row0, a.sinks)) v.x = -INFINITY;
             if (!cur.span.sees(pos + v_row1, a.sinks)) v.y = -INFINITY;
             if (missing) v.x = v.y = __int_as_float(0x7fc00000);
           }
-          s2[4 * q4 + k] = v.x;
-          s2[4 * q4 + k + 1] = v.y;
-          const float2 u = add2(v, make_float2(lv[k], lv[k + 1]));
+          s2[to] = v.x;
+          s2[to + 1] = v.y;
+          vn[to] = vo[i0];
+          vn[to + 1] = vo[i1];
+          const float2 u = add2(v, make_float2(lv[i0], lv[i1]));
           top = fmaxf(top, fmaxf(u.x, u.y));
         }
       }
@@ -801,16 +824,28 @@ int launch(PagedDecodeArgs& a, const MmaTables& tb, cudaStream_t st) {
   a.tile_shift = H == 2 ? 6 : 5;
   a.min_tiles = W;
   a.group_cost = W;
-  paged_mma_kernel<KF, VB, W, S, H><<<a.ctas, (W + 1) * 32, L::end - kBase, st>>>(a, tb);
-  const int rc = check_launch("tq_paged_decode");
+  const int rc = launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
   return rc ? rc : launch_paged_merge(a, kDim, st);
 }
 
 }  // namespace
 
+// The layout of shared memory counts on where dynamic memory begins.
+bool base_holds() {
+  static int known[64] = {0};          // 1: holds, 2: does not
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!known[dev]) {
+    int v = 0;
+    known[dev] = cudaDeviceGetAttribute(&v, cudaDevAttrReservedSharedMemoryPerBlock, dev) == cudaSuccess && v == (int)kBase ? 1 : 2;
+  }
+  return known[dev] == 1;
+}
+
 // Queries in 32 bits ask for 32-bit weights and take the general kernel.
 bool paged_mma_supported(const PagedDecodeArgs& a, int dim) {
   if (dim != kDim || a.q_dtype == TQ_F32 || a.v.format != TQ_KV_POLAR || (a.v.bits != 3 && a.v.bits != 4)) return false;
+  if (!base_holds()) return false;
   if (!aligned16(a.v.data) || a.v.page_stride % 4 || a.v.head_stride % 4) return false;
   if (!aligned16(a.v.norms) || a.v.norm_page_stride % 4 || a.v.norm_head_stride % 4) return false;
   if (!aligned16(a.k.data)) return false;

@@ -17,6 +17,7 @@ A page id outside the pool is never followed: inserts skip the row, results beco
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -26,98 +27,93 @@ from .packing import VALS_PER_WORD, packed_dim
 __all__ = ["paged_append", "paged_decode", "paged_dequantize", "copy_pages", "paged_status"]
 
 _workspace_bytes: dict = {}      # (device index, dim) -> bytes: fixed by the SM count
-_ERR_CPU = "libtqb200 operates on CUDA tensors only (no CPU path)"
+_PACK = _lib.PAGED_PARAMS.pack   # tq_paged_params in one call: a launch's host time counts when its kernel takes 10 us
+_SIZE = _lib.PAGED_PARAMS.size
+_FORMATS = {torch.float32: _lib.TQ_F32, torch.float16: _lib.TQ_F16, torch.bfloat16: _lib.TQ_BF16}
+_addressof = ctypes.addressof
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class _on:
-    """The current device is `dev` inside the block (free when it already is)."""
-
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(fn, params: bytes, index: int) -> None:
+    """One C call with device `index` current."""
+    if index == torch.cuda.current_device():
+        rc = fn(params)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(params)
+    if rc:
+        _lib.check(rc)
 
 
-def _half(H, desc: dict, what: str, dim: int | None, dev, encode: bool):
-    """Fill a tq_paged_half from a pool dict; returns (pages, heads, page, dim)."""
+def _dtype(t: torch.Tensor) -> int:
+    code = _FORMATS.get(t.dtype)
+    return _lib.dtype_code(t.dtype) if code is None else code        # raises for anything else
+
+
+def _table(x, count: int, what: str, keep: list) -> int:
+    arr = _lib.host_floats(x)
+    if arr is None or len(arr) != count:
+        raise ValueError(f"{what}: {0 if arr is None else len(arr)} entries, {count} expected")
+    keep.append(arr)
+    return _addressof(arr)
+
+
+def _half(desc: dict, what: str, dim: int | None, index: int, encode: bool, keep: list):
+    """((pages, heads, page, dim), the tq_paged_half fields in front of `rows`) of a pool dict."""
     fmt = desc["format"]
     if fmt == "polar":
         packed, norms, bits = desc["packed"], desc["norms"], desc["bits"]
         if bits not in VALS_PER_WORD:
             raise ValueError(f"Unsupported bit width: {bits}. Use 1-4.")
-        signs = _lib.host_floats(desc["signs"])
         if dim is None:
-            dim = len(signs)
+            dim = desc["signs"].numel()
         shape, st, ns = packed.shape, packed.stride(), norms.stride()
-        if (packed.dtype is not torch.uint32 or len(shape) != 4 or st[3] != 1 or st[2] != shape[3]
-                or shape[3] != packed_dim(dim, bits)):
-            raise ValueError(f"{what}: packed must be (pages, heads, page, {packed_dim(dim, bits)}) uint32 with contiguous rows")
+        words = packed_dim(dim, bits)
+        if packed.dtype is not torch.uint32 or len(shape) != 4 or st[3] != 1 or st[2] != words or shape[3] != words:
+            raise ValueError(f"{what}: packed must be (pages, heads, page, {words}) uint32 with contiguous rows")
         if norms.dtype is not torch.float32 or norms.shape != shape[:3] or ns[2] != 1:
             raise ValueError(f"{what}: norms must be float32 {tuple(shape[:3])}, contiguous along the page")
-        if len(signs) != dim:
-            raise ValueError(f"{what}: {len(signs)} signs for dim {dim}")
-        if packed.device != dev or norms.device != dev:
-            raise ValueError(f"{what}: all tensors must be on {dev}")
-        H.format, H.bits = _lib.TQ_KV_POLAR, bits
-        H.data, H.norms = packed.data_ptr(), norms.data_ptr()
-        H.page_stride, H.head_stride = st[0], st[1]
-        H.norm_page_stride, H.norm_head_stride = ns[0], ns[1]
-        H.signs_host = signs
+        if packed.get_device() != index or norms.get_device() != index:
+            raise ValueError(f"{what}: all tensors must be on cuda:{index}")
+        signs = _table(desc["signs"], dim, what + ": signs", keep)
         levels = 1 << bits
-        if encode:
-            table = _lib.host_floats(desc["boundaries"])
-            if len(table) != levels - 1:
-                raise ValueError(f"{what}: {len(table)} boundaries for {bits} bits")
-            H.boundaries_host = table
-        else:
-            table = _lib.host_floats(desc["centroids"])
-            if len(table) != levels:
-                raise ValueError(f"{what}: {len(table)} centroids for {bits} bits")
-            H.centroids_host = table
-        return shape[0], shape[1], shape[2], dim
+        cents = 0 if encode else _table(desc["centroids"], levels, what + ": centroids", keep)
+        bounds = _table(desc["boundaries"], levels - 1, what + ": boundaries", keep) if encode else 0
+        return (shape[0], shape[1], shape[2], dim), (_lib.TQ_KV_POLAR, bits, 0), (
+            packed.data_ptr(), norms.data_ptr(), st[0], st[1], ns[0], ns[1], cents, bounds, signs)
     if fmt == "dense":
         data = desc["data"]
         shape, st = data.shape, data.stride()
         if len(shape) != 4 or st[3] != 1 or st[2] != shape[3] or (dim is not None and shape[3] != dim):
             raise ValueError(f"{what}: dense pages must be (pages, heads, page, dim) with contiguous rows")
-        if data.device != dev:
-            raise ValueError(f"{what}: all tensors must be on {dev}")
-        H.format, H.dtype, H.data = _lib.TQ_KV_DENSE, _lib.dtype_code(data.dtype), data.data_ptr()
-        H.page_stride, H.head_stride = st[0], st[1]
-        return shape[0], shape[1], shape[2], shape[3]
+        if data.get_device() != index:
+            raise ValueError(f"{what}: all tensors must be on cuda:{index}")
+        return tuple(shape), (_lib.TQ_KV_DENSE, 0, _dtype(data)), (data.data_ptr(), 0, st[0], st[1], 0, 0, 0, 0, 0)
     raise ValueError(f"{what}: unknown page format {fmt!r}")
 
 
-def _lens(t, what: str, batch: int, dev):
-    if t.dtype is not torch.int32 or t.shape != (batch,) or (batch > 1 and t.stride(0) != 1) or t.device != dev:
-        raise ValueError(f"{what} must be a contiguous int32 ({batch},) tensor on {dev}")
+_NO_ROWS = (0, 0, 0, 0)
+_NO_HALF = (0,) * 17
+
+
+def _lens(t, what: str, batch: int, index: int) -> int:
+    if t.dtype is not torch.int32 or t.shape != (batch,) or (batch > 1 and t.stride(0) != 1) or t.get_device() != index:
+        raise ValueError(f"{what} must be a contiguous int32 ({batch},) tensor on cuda:{index}")
     return t.data_ptr()
 
 
-def _common(P, page_table, seq_lens, what: str, dev):
-    """Table and lengths; returns the batch size."""
+def _pages(page_table, seq_lens, what: str, index: int):
+    """(batch, table address, its row stride, its width, address of the lengths)."""
     if not page_table.is_cuda or not seq_lens.is_cuda:
-        raise RuntimeError(_ERR_CPU)
-    if page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.stride(1) != 1 and page_table.shape[1] > 1:
-        raise ValueError("page_table must be an int32 (batch, width) tensor with contiguous rows")
-    if page_table.device != dev:
-        raise ValueError(f"page_table must be on {dev}")
+        raise RuntimeError("libtqb200 operates on CUDA tensors only (no CPU path)")
+    if page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.get_device() != index:
+        raise ValueError(f"page_table must be an int32 (batch, width) tensor on cuda:{index}")
     batch, width = page_table.shape
-    if batch < 1 or width < 1:
-        raise ValueError("page_table must have at least one sequence and one page")
-    P.struct_bytes = _PARAM_BYTES
-    P.batch, P.page_table, P.table_stride, P.table_width = batch, page_table.data_ptr(), page_table.stride(0), width
-    P.seq_lens = _lens(seq_lens, what, batch, dev)
-    return batch
-
-
-_PARAM_BYTES = ctypes.sizeof(_lib.PagedParams)
+    row, step = page_table.stride()
+    if batch < 1 or width < 1 or (step != 1 and width > 1):
+        raise ValueError("page_table must have at least one sequence and one page, and contiguous rows")
+    return batch, page_table.data_ptr(), row, width, _lens(seq_lens, what, batch, index)
 
 
 def paged_append(keys: torch.Tensor, values: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
@@ -130,17 +126,19 @@ def paged_append(keys: torch.Tensor, values: torch.Tensor, *, k: dict, v: dict, 
     are copied and need the pages' own type.  Two tokens of one call must not share a place (sequences that share a
     page must not both write it)."""
     _lib.require_cuda(keys, values)
-    dev = keys.device
+    index = keys.get_device()
     if keys.ndim != 4 or keys.shape != values.shape:
         raise ValueError(f"keys and values must be (batch, heads, tokens, dim) alike, got {tuple(keys.shape)} and {tuple(values.shape)}")
-    if values.device != dev:
-        raise ValueError(f"values must be on {dev}")
+    if values.get_device() != index:
+        raise ValueError(f"values must be on cuda:{index}")
     B, H, T, dim = keys.shape
-    P = _lib.PagedParams()
-    if _common(P, page_table, starts, "starts", dev) != B:
-        raise ValueError(f"page_table has {page_table.shape[0]} sequences, keys have {B}")
-    geo = _half(P.k, k, "keys", dim, dev, True)
-    if _half(P.v, v, "values", dim, dev, True) != geo:
+    batch, table, row, width, lens = _pages(page_table, starts, "starts", index)
+    if batch != B:
+        raise ValueError(f"page_table has {batch} sequences, keys have {B}")
+    keep: list = []
+    geo, k0, k1 = _half(k, "keys", dim, index, True, keep)
+    vgeo, v0, v1 = _half(v, "values", dim, index, True, keep)
+    if vgeo != geo:
         raise ValueError("the pools of keys and values must agree in pages, heads, page size and dim")
     if geo[1] != H:
         raise ValueError(f"the pool has {geo[1]} heads, the new rows {H}")
@@ -148,19 +146,18 @@ def paged_append(keys: torch.Tensor, values: torch.Tensor, *, k: dict, v: dict, 
         keys = keys.contiguous()
     if values.stride(3) != 1:
         values = values.contiguous()
-    for half, x in ((P.k, keys), (P.v, values)):
-        st = x.stride()
-        half.rows, half.rows_dtype = x.data_ptr(), _lib.dtype_code(x.dtype)
-        half.rows_batch_stride, half.rows_head_stride, half.rows_token_stride = st[0], st[1], st[2]
-    if P.k.format == _lib.TQ_KV_DENSE and P.k.rows_dtype != P.k.dtype or P.v.format == _lib.TQ_KV_DENSE and P.v.rows_dtype != P.v.dtype:
+    kt, vt = _dtype(keys), _dtype(values)
+    if k0[0] == _lib.TQ_KV_DENSE and kt != k0[2] or v0[0] == _lib.TQ_KV_DENSE and vt != v0[2]:
         raise ValueError("rows stored in dense pages must have the pages' dtype")
+    n = 0
     if counts is not None:
         _lib.require_cuda(counts)
-        P.counts = _lens(counts, "counts", B, dev)
-    P.n_kv_heads, P.dim, P.page_size, P.n_pages, P.tokens = H, dim, geo[2], geo[0], T
-    P.stream = torch.cuda.current_stream(dev).cuda_stream
-    with _on(dev):
-        _lib.check(_lib.lib().tq_paged_append(ctypes.byref(P)))
+        n = _lens(counts, "counts", B, index)
+    ks, vs = keys.stride(), values.stride()
+    _call(_lib.lib().tq_paged_append, _PACK(
+        _SIZE, B, 0, H, dim, geo[2], geo[0], table, row, lens, n, T, width, 0, 0, 0.0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+        _raw_stream(index), *k0, kt, *k1, keys.data_ptr(), ks[0], ks[1], ks[2], *v0, vt, *v1, values.data_ptr(), vs[0], vs[1], vs[2]),
+        index)
 
 
 def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor, seq_lens: torch.Tensor, attn_scale: float,
@@ -178,41 +175,40 @@ def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
 
     The weights are 16-bit in the tensor-core kernel (head_dim 128, 3 / 4-bit values, 16-bit or 3 / 4-bit keys, 16-bit
     queries); float32 queries and every other shape take the 32-bit kernel."""
-    _lib.require_cuda(q)
-    dev = q.device
+    if not q.is_cuda:
+        _lib.require_cuda(q)
+    index = q.get_device()
     if q.ndim != 3:
         raise ValueError(f"q must be (batch, heads, dim), got {tuple(q.shape)}")
     if q.stride(2) != 1:
         q = q.contiguous()
-    B, n_q, dim = q.shape
-    P = _lib.PagedParams()
-    if _common(P, page_table, seq_lens, "seq_lens", dev) != B:
-        raise ValueError(f"page_table has {page_table.shape[0]} sequences, q has {B}")
-    geo = _half(P.k, k, "keys", dim, dev, False)
-    if _half(P.v, v, "values", dim, dev, False) != geo:
+    B, n_q, dim = shape = q.shape
+    batch, table, row, width, lens = _pages(page_table, seq_lens, "seq_lens", index)
+    if batch != B:
+        raise ValueError(f"page_table has {batch} sequences, q has {B}")
+    keep: list = []
+    geo, k0, k1 = _half(k, "keys", dim, index, False, keep)
+    vgeo, v0, v1 = _half(v, "values", dim, index, False, keep)
+    if vgeo != geo:
         raise ValueError("the pools of keys and values must agree in pages, heads, page size and dim")
     if n_q == 0 or n_q % geo[1]:
         raise ValueError(f"n_q_heads ({n_q}) must equal n_kv_heads ({geo[1]}) * n_rep")
     if window < 0 or sinks < 0 or (sinks and not window):
         raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, and sinks need a window")
     if out is None:
-        out = torch.empty((B, n_q, dim), dtype=out_dtype or q.dtype, device=dev)
-    elif out.shape != (B, n_q, dim) or out.stride(2) != 1 or out.device != dev or (out_dtype or out.dtype) != out.dtype:
-        raise ValueError(f"out must be ({B}, {n_q}, {dim}) on {dev}, with a contiguous last dimension and of out_dtype")
-    need = paged_workspace_bytes(dev, dim)
+        out = q.new_empty(shape, dtype=out_dtype)
+    elif out.shape != shape or out.stride(2) != 1 or out.get_device() != index or (out_dtype or out.dtype) != out.dtype:
+        raise ValueError(f"out must be {tuple(shape)} on cuda:{index}, with a contiguous last dimension and of out_dtype")
+    need = _workspace_bytes.get((index, dim)) or paged_workspace_bytes(index, dim)
     if workspace is None:
-        workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
-    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.device != dev or workspace.numel() < need:
-        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {dev}")
-    st, so = q.stride(), out.stride()
-    P.n_q_heads, P.n_kv_heads, P.dim, P.page_size, P.n_pages = n_q, geo[1], dim, geo[2], geo[0]
-    P.q, P.q_dtype, P.q_batch_stride, P.q_head_stride = q.data_ptr(), _lib.dtype_code(q.dtype), st[0], st[1]
-    P.out, P.out_dtype, P.out_batch_stride, P.out_head_stride = out.data_ptr(), _lib.dtype_code(out.dtype), so[0], so[1]
-    P.attn_scale, P.window, P.sinks = attn_scale, min(window, 0x7fffffff), min(sinks, 0x7fffffff)
-    P.workspace, P.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    P.stream = torch.cuda.current_stream(dev).cuda_stream
-    with _on(dev):
-        _lib.check(_lib.lib().tq_paged_decode(ctypes.byref(P)))
+        workspace = q.new_empty((need,), dtype=torch.uint8)
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != index or workspace.numel() < need:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on cuda:{index}")
+    qs, os = q.stride(), out.stride()
+    _call(_lib.lib().tq_paged_decode, _PACK(
+        _SIZE, B, n_q, geo[1], dim, geo[2], geo[0], table, row, lens, 0, 0, width, _dtype(q), _dtype(out), attn_scale,
+        min(window, 0x7fffffff), min(sinks, 0x7fffffff), q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+        workspace.data_ptr(), workspace.numel(), _raw_stream(index), *k0, 0, *k1, *_NO_ROWS, *v0, 0, *v1, *_NO_ROWS), index)
     return out
 
 
@@ -233,35 +229,33 @@ def paged_dequantize(pool: dict, *, page_table: torch.Tensor, seq_lens: torch.Te
     and `packed_dequantize` give; rows at and behind seq_lens[b] are zero.  Dense pools are gathered as they are.
     `out` optionally names the contiguous tensor to write."""
     _lib.require_cuda(page_table)
-    dev = page_table.device
-    P = _lib.PagedParams()
-    B = _common(P, page_table, seq_lens, "seq_lens", dev)
-    n_pages, H, page, dim = _half(P.v, pool, "pages", None, dev, False)
+    index = page_table.get_device()
+    B, table, row, width, lens = _pages(page_table, seq_lens, "seq_lens", index)
+    keep: list = []
+    (n_pages, H, page, dim), v0, v1 = _half(pool, "pages", None, index, False, keep)
     if length < 0:
         raise ValueError(f"length must not be negative, got {length}")
     if out is None:
-        out = torch.empty((B, H, length, dim), dtype=dtype, device=dev)
-    elif out.shape != (B, H, length, dim) or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous ({B}, {H}, {length}, {dim}) tensor on {dev}")
-    P.n_kv_heads, P.dim, P.page_size, P.n_pages, P.tokens = H, dim, page, n_pages, length
-    P.out, P.out_dtype = out.data_ptr(), _lib.dtype_code(out.dtype)
-    P.stream = torch.cuda.current_stream(dev).cuda_stream
-    with _on(dev):
-        _lib.check(_lib.lib().tq_paged_dequantize(ctypes.byref(P)))
+        out = torch.empty((B, H, length, dim), dtype=dtype, device=page_table.device)
+    elif out.shape != (B, H, length, dim) or not out.is_contiguous() or out.get_device() != index:
+        raise ValueError(f"out must be a contiguous ({B}, {H}, {length}, {dim}) tensor on cuda:{index}")
+    _call(_lib.lib().tq_paged_dequantize, _PACK(
+        _SIZE, B, 0, H, dim, page, n_pages, table, row, lens, 0, length, width, 0, _dtype(out), 0.0, 0, 0, 0, 0, 0,
+        out.data_ptr(), 0, 0, 0, 0, _raw_stream(index), *_NO_HALF, *v0, 0, *v1, *_NO_ROWS), index)
     return out
 
 
-def _page_ids(ids, n_pages: int, what: str):
-    """int32 ids from a list or a CPU tensor (checked) or a CUDA tensor (its values are checked by the kernel)."""
+def _page_ids(ids, n_pages: int, what: str, index: int):
+    """int32 ids on the device, from a list or a CPU tensor (checked here) or a CUDA tensor (checked by the kernel)."""
     if isinstance(ids, torch.Tensor) and ids.is_cuda:
-        if ids.dtype is not torch.int32 or ids.ndim != 1 or not ids.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous one-dimensional int32 tensor")
+        if ids.dtype is not torch.int32 or ids.ndim != 1 or not ids.is_contiguous() or ids.get_device() != index:
+            raise ValueError(f"{what} must be a contiguous one-dimensional int32 tensor on cuda:{index}")
         return ids, None
     host = [int(i) for i in ids]
     bad = [i for i in host if not 0 <= i < n_pages]
     if bad:
         raise ValueError(f"{what}: page {bad[0]} is outside the pool of {n_pages}")
-    return torch.tensor(host, dtype=torch.int32), host
+    return torch.tensor(host, dtype=torch.int32, device=torch.device("cuda", index)), host
 
 
 def copy_pages(pools, src, dst) -> None:
@@ -273,32 +267,33 @@ def copy_pages(pools, src, dst) -> None:
     pools = list(pools)
     if not pools:
         return
-    _lib.require_cuda(*pools)
-    dev, n_pages = pools[0].device, pools[0].shape[0]
+    _lib.require_cuda(pools[0])
+    index, n_pages = pools[0].get_device(), pools[0].shape[0]
+    ptrs, sizes = [], []
     for t in pools:
-        if t.device != dev or t.shape[0] != n_pages or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError("pools must be contiguous, 16-byte aligned, of one device and one number of pages")
-    (src, hs), (dst, hd) = _page_ids(src, n_pages, "src"), _page_ids(dst, n_pages, "dst")
-    if src.numel() != dst.numel():
-        raise ValueError(f"{src.numel()} source and {dst.numel()} target pages")
+        at = t.data_ptr()
+        if t.get_device() != index or t.shape[0] != n_pages or not t.is_contiguous() or at % 16:
+            raise ValueError("pools must be contiguous CUDA tensors, 16-byte aligned, of one device and one number of pages")
+        ptrs.append(at)
+        sizes.append(t.nbytes)
+    (src, hs), (dst, hd) = _page_ids(src, n_pages, "src", index), _page_ids(dst, n_pages, "dst", index)
+    n_pairs = src.numel()
+    if n_pairs != dst.numel():
+        raise ValueError(f"{n_pairs} source and {dst.numel()} target pages")
     if hd is not None and len(set(hd)) != len(hd):
         raise ValueError("a target page is named twice")
     if hs is not None and hd is not None and set(hs) & set(hd):
         raise ValueError("a page is both read and written")
-    if n_pages == 0 or src.numel() == 0:
+    if n_pages == 0 or n_pairs == 0:
         return
-    sizes = [t.numel() // n_pages * t.element_size() for t in pools]
+    sizes = [s // n_pages for s in sizes]
     if any(s == 0 or s % 16 for s in sizes):
         raise ValueError("pages must be multiples of 16 bytes")
-    if src.device != dev:
-        src = src.to(dev)
-    if dst.device != dev:
-        dst = dst.to(dev)
-    n = len(pools)
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in pools])
-    with _on(dev):
-        _lib.check(_lib.lib().tq_copy_pages(ptrs, (ctypes.c_int64 * n)(*sizes), n, n_pages, src.data_ptr(), dst.data_ptr(),
-                                            src.numel(), torch.cuda.current_stream(dev).cuda_stream))
+    n = len(ptrs)
+    args = struct.pack(f"={n}Q{n}q", *ptrs, *sizes)
+    base = ctypes.cast(ctypes.c_char_p(args), ctypes.c_void_p).value
+    fn = _lib.lib().tq_copy_pages
+    _call(lambda _p: fn(base, base + 8 * n, n, n_pages, src.data_ptr(), dst.data_ptr(), n_pairs, _raw_stream(index)), args, index)
 
 
 def paged_status(device) -> int:
