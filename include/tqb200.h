@@ -439,7 +439,7 @@ typedef struct tq_paged_params {
   int64_t q_batch_stride, q_head_stride;
   void* out;
   int64_t out_batch_stride, out_head_stride;
-  void* workspace;               /* decode: tq_paged_decode_workspace_bytes(dim), 16-byte aligned, contents irrelevant */
+  void* workspace;               /* decode: tq_paged_decode_workspace_bytes(dim), 16-byte aligned (see tq_paged_decode) */
   int64_t workspace_bytes;
   void* stream;
   tq_paged_half k, v;            /* dequantize reads `v` */
@@ -449,8 +449,8 @@ typedef struct tq_paged_params {
  * quantized with tq_quantize's arithmetic (the same words), dense halves copied. */
 int tq_paged_append(const tq_paged_params* p);
 /* One query token per sequence (the last of seq_lens[b] positions) over the pages; a
- * sequence of length 0 gives zeros.  The workspace holds nothing between calls; calls
- * that may overlap need one each. */
+ * sequence of length 0 gives zeros.  The workspace must be zero the first time it is used;
+ * every call leaves it ready for the next one.  Calls that may overlap need one each. */
 int64_t tq_paged_decode_workspace_bytes(int dim);
 int tq_paged_decode(const tq_paged_params* p);
 /* Positions [0, tokens) of every sequence as dense rows (batch, heads, tokens, dim), contiguous;

@@ -1,4 +1,4 @@
-// Paged caches: argument checks, the general decode kernel, the merge of split groups, page copies.
+// Paged caches: argument checks, the general decode kernel, page copies.
 // (The tensor-core decode kernel is paged_mma.cu; insert and read-back are paged_rows.cu.)
 #include <math.h>
 #include <string.h>
@@ -30,7 +30,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kTile = 32;            // positions per tile of the general kernel: one per lane
-constexpr int kMaxCtas = 256;        // of a decode launch (one per SM)
 
 // ---- general decode -----------------------------------------------------------------------------------
 // out = sum_p softmax(scale * q . k_p) v_p in 32 bits on the CUDA cores, for every head dimension, code width
@@ -58,6 +57,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   plan_costs(a, prefix);
+  zero_empty(a, DIM);
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
@@ -188,121 +188,30 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
       if (cnt == cur.span.tiles) {
         finish_row<EPL>(a, b, h0 + warp, v, ls, lane);
       } else {
-        float* part = a.part + ((int64_t)(2 * cta + (cur.j == 0)) * kPagedRows + warp) * (DIM + 2);
+        float* part = part_of(a, cta, cur.j == 0 ? cta : -1, warp, DIM);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) part[lane * EPL + j] = v[j];
         if (lane == 0) {
           part[DIM] = mx;
           part[DIM + 1] = ls;
         }
+        __threadfence();
       }
     }
     __syncthreads();
+    if (cnt != cur.span.tiles) {
+      // where the group begins in the plan's numbering: from the end of this run, or from its beginning
+      const int64_t first = cur.j == 0 ? plan.begin(cta + 1) - end.j : plan.begin(cta) - cur.j;
+      const int c0 = plan.owner(first), c1 = plan.owner(first + cur.span.tiles - 1);
+      __shared__ int last_s;
+      if (threadIdx.x == 0) last_s = last_part(a, c0, c1);
+      __syncthreads();
+      if (last_s && warp < nr) join_row<EPL>(a, c0, c1, warp, b, h0 + warp, lane);
+      __syncthreads();
+    }
     if (cur.j + cnt < cur.span.tiles) break;
     cur.next_group(a);
   }
-}
-
-// ---- merge -----------------------------------------------------------------------------------------------
-// Joins the partial states of the CTAs that share a group: m = max m_i, l = sum l_i 2^(m_i - m), acc likewise.  Groups of
-// one CTA are already written; a sequence without tiles gets zeros here.  With many groups each has few parts: a block
-// takes a group, a warp a row (ROWS = 8).  With few groups each may have a hundred: a block takes one row, its warps
-// share the parts and meet in shared memory (ROWS = 1).  Whole call: 4 groups of 37 parts 23.4 us with ROWS = 8, 17.4
-// with 1; 128 groups of 2 or 3 parts 34.0 and 39.1 us.
-template <int EPL, int ROWS>
-__global__ void __launch_bounds__(kPagedRows * 32)
-paged_merge_kernel(const PagedDecodeArgs a) {
-  constexpr int DIM = EPL * 32;
-  constexpr int kBatch = 8;          // partial states whose rows a lane has in flight
-  constexpr int kShare = kPagedRows / ROWS;            // warps per row
-  __shared__ int prefix[kPlanEntries + 1];
-  __shared__ float w_s[ROWS][kMaxCtas];
-  __shared__ float acc_s[kShare][DIM];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = ROWS == 1 ? warp : 0;
-  const int group = blockIdx.x / (kPagedRows / ROWS), rg_per_head = a.groups / a.n_kv_heads;
-  const int row = ROWS == 1 ? (int)blockIdx.x % kPagedRows : warp;
-  // The kernel in front has itself waited for what wrote the lengths, so the plan may be made before its end; its
-  // partial states, and the output, have to wait for it.
-  plan_costs(a, prefix);
-  const Plan plan = make_paged_plan(a, prefix);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int kvh = group / rg_per_head, r0 = (group % rg_per_head) * kPagedRows;
-  const bool live = row < min(kPagedRows, a.n_rep - r0);
-  const int head = kvh * a.n_rep + r0 + row;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const SeqSpan span = span_of(a, b);
-    float v[EPL];
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) v[j] = 0.f;
-    if (span.tiles == 0) {
-      if (live && share == 0) finish_row<EPL>(a, b, head, v, 0.f, lane);
-      continue;
-    }
-    const int64_t first = (int64_t)cost_before(a, prefix, b) * a.groups + (int64_t)group * cost_of(a, span) + a.group_cost;
-    const int c0 = plan.owner(first), c1 = plan.owner(first + span.tiles - 1);
-    if (c0 == c1) continue;
-    // the group's first CTA left its tail piece (slot 1), the others their head pieces (slot 0)
-    auto slot = [&](int c) { return a.part + ((int64_t)(2 * c + (c == c0)) * kPagedRows + row) * (DIM + 2); };
-    const int n = c1 - c0 + 1;
-    float mx = -INFINITY, l = 0.f;
-    float* w = w_s[ROWS == 1 ? 0 : warp];
-    if (live) {                        // every warp of a row works out all weights: no exchange, the parts are in the L2
-      for (int i = lane; i < n; i += 32) mx = fmaxf(mx, __ldcg(slot(c0 + i) + DIM));
-      mx = warp_max(mx);
-      for (int i = lane; i < n; i += 32) {
-        const float m = __ldcg(slot(c0 + i) + DIM), li = __ldcg(slot(c0 + i) + DIM + 1);
-        const float f = m == -INFINITY ? 1.f : paged_ex2(m - mx);      // m = -inf: l is 0, or NaN (a missing page)
-        w[i] = f;                      // warps of one row store the same value
-        l += li * f;
-      }
-      l = warp_sum(l);
-      __syncwarp();
-      for (int i0 = share * kBatch; i0 < n; i0 += kBatch * kShare) {
-        float x[kBatch][EPL];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const float* p = slot(c0 + min(i0 + k, n - 1)) + lane * EPL;
-#pragma unroll
-          for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const float f = i0 + k < n ? w[i0 + k] : 0.f;
-#pragma unroll
-          for (int j = 0; j < EPL; ++j)
-            if (i0 + k < n) v[j] += x[k][j] * f;
-        }
-      }
-    }
-    if (ROWS == 1) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) acc_s[share][lane * EPL + j] = v[j];
-      __syncthreads();
-      if (share == 0) {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          v[j] = 0.f;
-#pragma unroll
-          for (int s = 0; s < kShare; ++s) v[j] += acc_s[s][lane * EPL + j];
-        }
-      }
-    }
-    if (live && share == 0) finish_row<EPL>(a, b, head, v, l, lane);
-    if (ROWS == 1) __syncthreads();
-    else __syncwarp();
-  }
-}
-
-template <int EPL>
-int launch_merge_t(const PagedDecodeArgs& a, cudaStream_t st) {
-  const unsigned batch = a.batch < 32768 ? a.batch : 32768;
-  if ((int64_t)a.groups * a.batch * kPagedRows >= a.ctas)       // at most about nine parts per group
-    return launch_dependent("tq_paged_decode (merge)", paged_merge_kernel<EPL, kPagedRows>, dim3(a.groups, batch), kPagedRows * 32,
-                            0, st, a);
-  return launch_dependent("tq_paged_decode (merge)", paged_merge_kernel<EPL, 1>, dim3(a.groups * kPagedRows, batch),
-                          kPagedRows * 32, 0, st, a);
 }
 
 template <int EPL>
@@ -317,8 +226,7 @@ int launch_general(const PagedDecodeArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
   }
-  const int rc = launch_dependent("tq_paged_decode (general)", paged_decode_general_kernel<EPL>, dim3(a.ctas), kWarps * 32, smem, st, a);
-  return rc ? rc : launch_merge_t<EPL>(a, st);
+  return launch_dependent("tq_paged_decode (general)", paged_decode_general_kernel<EPL>, dim3(a.ctas), kWarps * 32, smem, st, a);
 }
 
 // ---- page copies -------------------------------------------------------------------------------------------
@@ -360,15 +268,6 @@ copy_pages_kernel(const __grid_constant__ CopyArgs a) {
 }
 
 }  // namespace
-
-int launch_paged_merge(const PagedDecodeArgs& a, int dim, cudaStream_t st) {
-  switch (dim) {
-    case 32: return launch_merge_t<1>(a, st);
-    case 64: return launch_merge_t<2>(a, st);
-    case 128: return launch_merge_t<4>(a, st);
-    default: return launch_merge_t<8>(a, st);
-  }
-}
 
 // ---- host-side checks shared by the entry points ------------------------------------------------------------
 int check_paged_params(const tq_paged_params* p) {
@@ -441,7 +340,7 @@ int fill_page_view(const tq_paged_params* p, PageView* v) {
 using namespace tq;
 
 extern "C" int64_t tq_paged_decode_workspace_bytes(int dim) {
-  return (int64_t)2 * num_sms() * kPagedRows * (dim + 2) * (int64_t)sizeof(float);
+  return kMaxCtas * (int64_t)sizeof(int) + (int64_t)2 * num_sms() * kPagedRows * (dim + 4) * (int64_t)sizeof(float);
 }
 
 extern "C" int tq_paged_decode(const tq_paged_params* p) {
@@ -484,7 +383,8 @@ extern "C" int tq_paged_decode(const tq_paged_params* p) {
   a.out_batch_stride = p->out_batch_stride;
   a.out_head_stride = p->out_head_stride;
   a.scale_log2 = p->attn_scale * kPagedLog2e;
-  a.part = (float*)p->workspace;
+  a.counters = (int*)p->workspace;
+  a.part = (float*)(a.counters + kMaxCtas);
   a.ctas = num_sms() < kMaxCtas ? num_sms() : kMaxCtas;
   cudaStream_t st = (cudaStream_t)p->stream;
   if (paged_mma_supported(a, p->dim)) return launch_paged_mma(a, st);

@@ -13,7 +13,8 @@
 // Starting and finishing a group costs a CTA time too, so each group counts group_cost tiles more than it has
 // (a run that begins inside that lead begins at the group's first tile).  A CTA that holds all tiles of a
 // group writes its output; otherwise it leaves a partial state (m, l, acc) in one of its two slots of the
-// workspace, which the merge kernel joins.
+// workspace and counts itself in, and the CTA that completes the count joins the states and writes the output.
+// No CTA waits for another.
 #pragma once
 
 #include "common.cuh"
@@ -22,6 +23,7 @@ namespace tq {
 
 constexpr int kMinPage = 32;         // positions of the smallest page
 constexpr int kPagedRows = 8;        // query heads per group
+constexpr int kMaxCtas = 256;        // of a decode launch (one per SM)
 constexpr int kPlanEntries = 256;    // prefix entries of a CTA's plan (each covers ceil(batch / 256) sequences)
 constexpr float kPagedLog2e = 1.4426950408889634f;
 
@@ -67,7 +69,8 @@ struct PagedDecodeArgs {
   int64_t out_batch_stride, out_head_stride;
   float scale_log2;                  // attn_scale * log2(e)
   uint32_t k_page_bytes, v_page_bytes, kn_page_bytes, vn_page_bytes;   // tensor-core kernel: page distances
-  float* part;                       // [2 * ctas][8][dim + 2]: acc (rotated domain), m (log2 domain), l
+  int* counters;                     // [kMaxCtas], zero between calls: CTAs of the split group that begins in CTA c
+  float* part;                       // [2 * ctas][8][dim + 4]: acc (rotated domain), m (log2 domain), l, two unused
   int ctas, min_tiles, group_cost;   // grid of the main kernel; fewest tiles worth a CTA; what a group costs besides, in tiles
 };
 
@@ -245,9 +248,75 @@ __device__ __forceinline__ void finish_row(const PagedDecodeArgs& a, int b, int 
   for (int j = 0; j < EPL; ++j)
     store_elem(a.out, a.out_dtype, off + j, l == 0.f ? 0.f : v[j] * sign_at(a.v.signs, lane * EPL + j) * inv);
 }
+// Sequences without a tile get zeros, from the CTAs in turn.
+__device__ __forceinline__ void zero_empty(const PagedDecodeArgs& a, int dim) {
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (span_of(a, b).tiles != 0) continue;
+    for (int i = threadIdx.x; i < a.n_q_heads * dim; i += blockDim.x)
+      store_elem(a.out, a.out_dtype, b * a.out_batch_stride + i / dim * a.out_head_stride + i % dim, 0.f);
+  }
+}
+
+// Slot of CTA c's part of a group that begins in CTA c0: its tail piece (1) or its head piece (0).
+__device__ __forceinline__ float* part_of(const PagedDecodeArgs& a, int c, int c0, int row, int dim) {
+  return a.part + ((int64_t)(2 * c + (c == c0)) * kPagedRows + row) * (dim + 4);
+}
+
+// The CTA has stored its part of a split group (every storing thread has fenced, the block has met): counts it in and
+// says whether it was the last.  `first`: the group's first tile in the plan's numbering.  One thread.
+__device__ __forceinline__ bool last_part(const PagedDecodeArgs& a, int c0, int c1) {
+  int before;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + c0) : "memory");
+  if (before != c1 - c0) return false;
+  a.counters[c0] = 0;                // nobody else touches it before the next call
+  return true;
+}
+
+// Joins one row of the parts c0 .. c1 of a group: m = max m_i, l = sum l_i 2^(m_i - m), acc likewise; one warp.
+template <int EPL>
+__device__ __forceinline__ void join_row(const PagedDecodeArgs& a, int c0, int c1, int row, int b, int head, int lane) {
+  constexpr int DIM = EPL * 32;
+  constexpr int kBatch = EPL <= 4 ? 12 : 4;          // parts whose rows a lane has in flight
+  float mx = -INFINITY, l = 0.f, v[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) v[j] = 0.f;
+  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(part_of(a, c, c0, row, DIM) + DIM));
+  mx = warp_max(mx);
+  for (int cb = c0; cb <= c1; cb += 32) {            // 32 parts: lane i knows the weight of part cb + i
+    float f = 0.f;
+    if (cb + lane <= c1) {
+      const float* p = part_of(a, cb + lane, c0, row, DIM) + DIM;
+      const float m = __ldcg(p), li = __ldcg(p + 1);
+      f = m == -INFINITY ? 1.f : paged_ex2(m - mx);  // m = -inf: l is 0, or NaN (a missing page)
+      l += li * f;
+    }
+    const int n = min(32, c1 - cb + 1);
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+      float x[kBatch][EPL];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float* p = part_of(a, cb + min(i0 + k, n - 1), c0, row, DIM) + lane * EPL;
+        if (EPL == 4) {
+          const float4 w = __ldcg(reinterpret_cast<const float4*>(p));
+          x[k][0] = w.x; x[k][EPL > 1 ? 1 : 0] = w.y; x[k][EPL > 2 ? 2 : 0] = w.z; x[k][EPL > 3 ? 3 : 0] = w.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float w = __shfl_sync(0xffffffffu, f, min(i0 + k, n - 1));
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (i0 + k < n) v[j] += x[k][j] * w;
+      }
+    }
+  }
+  finish_row<EPL>(a, b, head, v, warp_sum(l), lane);
+}
 #endif  // __CUDACC__
 
-int launch_paged_merge(const PagedDecodeArgs& a, int dim, cudaStream_t st);
 bool paged_mma_supported(const PagedDecodeArgs& a, int dim);
 int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st);
 

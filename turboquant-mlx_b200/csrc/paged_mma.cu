@@ -13,7 +13,7 @@
 //   values : out^T += V^T P.  The codes of two neighbouring positions are interleaved bit by bit field first, so that one
 //            table entry is the pair of values the MMA wants side by side and nothing is permuted afterwards.
 // At the end of a group the warps meet in shared memory; a group that lies in one CTA is finished there (butterfly,
-// signs, / dim / l), otherwise its partial state goes to the workspace and paged_merge_kernel joins it.
+// signs, / dim / l), otherwise its partial state goes to the workspace and the CTA that is last joins the states.
 //
 // Positions of a tile are dealt to MMA columns so that thread t of a quad owns 8 consecutive ones of each 32: norms come
 // in 16-byte loads, and the rows that the threads of a warp read together lie in different banks where they can.
@@ -260,11 +260,10 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     }
     if (e < (1u << (2 * VB))) sts32(at + L::v_entry, (uint32_t)tb.v_c16[e & ((1 << VB) - 1)] | ((uint32_t)tb.v_c16[e >> VB] << 16));
   }
-  // Everything above overlaps the end of the kernel in front; everything below may read what that kernel wrote.  The
-  // merge is not let in early: its blocks beside the running ones cost more than their start (34 against 23 us for one
-  // sequence of 32768 tokens with 16-bit keys).
+  // Everything above overlaps the end of the kernel in front; everything below may read what that kernel wrote.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   plan_costs(a, prefix);          // also the barrier behind the tables
+  zero_empty(a, kDim);
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
@@ -428,6 +427,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   };
   float xq[kRpw][4];
   load_query(cur, xq);
+  bool gave_up = false;              // a bounded wait failed: no more tiles, NaN for every group still to come
   while (true) {
     const int cnt = cur.count_to(end);
     const int b = cur.b, kvh = rg_per_head == 1 ? cur.group : cur.group / rg_per_head;
@@ -481,7 +481,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    for (; i < cnt; i += W) {
+    for (; i < cnt && !gave_up; i += W) {
       if (!mbar_wait(L::full + 8 * (warp * S + us), phase)) {      // gave up: everything this CTA produces from here on is NaN
         if (lane == 0) {
           sts32(L::flag, 1);
@@ -721,7 +721,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       }
     }
     consumer_barrier<W>();
-    const bool gave_up = lds32(L::flag) != 0;
+    gave_up = lds32(L::flag) != 0;   // read behind a barrier that every writer has passed: all warps agree
     for (int r = warp; r < nr; r += W) {
       float mx = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t at[4];
@@ -747,16 +747,26 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       if (cnt == cur.span.tiles) {
         finish_row<4>(a, b, h0 + r, v, l, lane);
       } else {
-        float* part = a.part + ((int64_t)(2 * cta + (cur.j == 0)) * kPagedRows + r) * (kDim + 2);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) part[lane * 4 + j] = v[j];
+        float* part = part_of(a, cta, cur.j == 0 ? cta : -1, r, kDim);
+        *reinterpret_cast<float4*>(part + lane * 4) = make_float4(v[0], v[1], v[2], v[3]);
         if (lane == 0) {
           part[kDim] = mx;
           part[kDim + 1] = l;
         }
+        __threadfence();
       }
     }
-    if (gave_up || !more) return;      // all warps agree: the flag is read behind a barrier that every writer passed
+    if (cnt != cur.span.tiles) {
+      // where the group begins in the plan's numbering: from the end of this run, or from its beginning
+      const int64_t first = cur.j == 0 ? plan.begin(cta + 1) - end.j : plan.begin(cta) - cur.j;
+      const int c0 = plan.owner(first), c1 = plan.owner(first + cur.span.tiles - 1);
+      consumer_barrier<W>();           // the whole part is on its way
+      if (threadIdx.x == 0) sts32(L::flag + 4, last_part(a, c0, c1));
+      consumer_barrier<W>();
+      if (lds32(L::flag + 4))
+        for (int r = warp; r < nr; r += W) join_row<4>(a, c0, c1, r, b, h0 + r, lane);
+    }
+    if (!more) return;
     cur = nx;
     // the next group's first stores to q, xch and ml come behind a barrier that every reader above has passed
   }
@@ -824,8 +834,7 @@ int launch(PagedDecodeArgs& a, const MmaTables& tb, cudaStream_t st) {
   a.tile_shift = H == 2 ? 6 : 5;
   a.min_tiles = W;
   a.group_cost = W;
-  const int rc = launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
-  return rc ? rc : launch_paged_merge(a, kDim, st);
+  return launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
 }
 
 }  // namespace

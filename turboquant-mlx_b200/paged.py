@@ -26,6 +26,7 @@ from .packing import VALS_PER_WORD, packed_dim
 
 __all__ = ["paged_append", "paged_decode", "paged_dequantize", "copy_pages", "paged_status"]
 
+_workspaces: dict = {}           # (device index, stream, dim) -> scratch of the calls made on it outside of captures
 _workspace_bytes: dict = {}      # (device index, dim) -> bytes: fixed by the SM count
 _PACK = _lib.PAGED_PARAMS.pack   # tq_paged_params in one call: a launch's host time counts when its kernel takes 10 us
 _SIZE = _lib.PAGED_PARAMS.size
@@ -169,9 +170,9 @@ def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
     window > 0: the token sees positions >= seq_lens[b] - window and the first `sinks` ones (it counts itself, as
     `create_causal_mask` does); pages outside both may have been freed.  A sequence of length 0 gives zeros.
     Lengths beyond the table are cut to it.  `out` optionally names the tensor to write (rows contiguous).
-    `workspace`: a uint8 tensor of `paged_workspace_bytes` on the device; without it each call allocates its own from
-    torch's caching allocator (inside a captured graph: from the graph's pool), so overlapping calls and captured
-    graphs never share one.
+    `workspace`: a zero-filled uint8 tensor of `paged_workspace_bytes` used by no other call that may be in flight
+    together with this one; every call leaves it ready for the next.  Without it the calls of a stream share one, and a
+    call captured in a CUDA graph gets one of its own from the graph's pool.
 
     The weights are 16-bit in the tensor-core kernel (head_dim 128, 3 / 4-bit values, 16-bit or 3 / 4-bit keys, 16-bit
     queries); float32 queries and every other shape take the 32-bit kernel."""
@@ -201,7 +202,12 @@ def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
         raise ValueError(f"out must be {tuple(shape)} on cuda:{index}, with a contiguous last dimension and of out_dtype")
     need = _workspace_bytes.get((index, dim)) or paged_workspace_bytes(index, dim)
     if workspace is None:
-        workspace = q.new_empty((need,), dtype=torch.uint8)
+        stream = _raw_stream(index)
+        workspace = _workspaces.get((index, stream, dim))
+        if workspace is None or torch.cuda.is_current_stream_capturing():
+            workspace = q.new_zeros((need,), dtype=torch.uint8)        # captured: zeroed again by every replay
+            if not torch.cuda.is_current_stream_capturing():
+                _workspaces[(index, stream, dim)] = workspace
     elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != index or workspace.numel() < need:
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on cuda:{index}")
     qs, os = q.stride(), out.stride()
