@@ -263,6 +263,67 @@ def test_append_extreme_rows(tq, dev):
         assert torch.equal(pool.packed[1, 0, :6].view(torch.int32), w.view(torch.int32)) and torch.equal(pool.norms[1, 0, :6], n)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_append_extreme_rows_of_a_prompt(tq, dev, dtype):
+    """A prompt's worth of zero, subnormal, huge, infinite, NaN and border rows: the words of the contiguous quantizer."""
+    dim, page, n = 128, 64, 100
+    table = torch.tensor([[3, 1]], dtype=torch.int32, device=dev)
+    k, v = pr.Pool(tq, 1, 4, 2, page, dim, 3, dev), pr.Pool(tq, 2, 4, 2, page, dim, 4, dev)
+    x = torch.randn((2, n, dim), generator=torch.Generator().manual_seed(4))
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3] = 0, x[:, 1] * 1e-6, x[:, 2] * 1e4, x[:, 3] * 1e-3
+    x[:, 4, 7], x[:, 5, 9], x[:, 6, 127] = float("inf"), float("nan"), -float("inf")
+    x[:, 7] = k.quant.signs.cpu()                       # rotates onto one axis
+    x[:, 8] = 0
+    x[:, 8, 64] = 1                                      # rotates to equal magnitudes
+    if dtype == torch.bfloat16:
+        x[:, 9], x[:, 10], x[:, 11] = x[:, 9] * 1e-38, x[:, 10] * 1e18, x[:, 11] * 1e30
+    x = x.to(dtype).to(dev)
+    tq.paged_append(x[None], x[None], k=k.desc, v=v.desc, page_table=table, starts=torch.zeros(1, dtype=torch.int32, device=dev))
+    for pool in (k, v):
+        w, nn = tq.fused_quantize(x.reshape(-1, dim), pool.quant.signs, pool.quant.boundaries, dim, pool.bits)
+        w, nn = w.view(torch.int32).view(2, n, -1), nn.view(2, n)
+        got = pool.packed.view(torch.int32)[[3, 1]].transpose(0, 1).flatten(1, 2)[:, :n]
+        assert torch.equal(got, w)
+        assert torch.equal(pool.norms[[3, 1]].transpose(0, 1).flatten(1, 2)[:, :n].nan_to_num(7.0), nn.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("bits", [3, 4])
+def test_append_other_codebooks(tq, dev, bits):
+    """Borders that are uneven, nearly equal or all alike: the count of borders below, whatever the kernel."""
+    dim, page, n, levels = 128, 32, 40, 1 << bits
+    x = torch.randn((1, 1, n, dim), generator=torch.Generator().manual_seed(5)).half().to(dev)
+    for seed, borders in enumerate((torch.linspace(-3, 3, levels - 1) ** 3, torch.linspace(-1e-4, 1e-4, levels - 1),
+                                    torch.zeros(levels - 1), torch.linspace(0.1, 0.11, levels - 1))):
+        k, v = pr.Pool(tq, 1, 3, 1, page, dim, bits, dev), pr.Pool(tq, 2, 3, 1, page, dim, bits, dev)
+        borders = borders.to(dev)
+        k.desc["boundaries"] = v.desc["boundaries"] = borders
+        tq.paged_append(x, x, k=k.desc, v=v.desc, page_table=torch.tensor([[2, 0]], dtype=torch.int32, device=dev),
+                        starts=torch.zeros(1, dtype=torch.int32, device=dev))
+        for pool in (k, v):
+            w, _ = tq.fused_quantize(x[0, 0], pool.quant.signs, borders, dim, bits)
+            got = pool.packed.view(torch.int32)[[2, 0], 0].flatten(0, 1)[:n]
+            assert torch.equal(got, w.view(torch.int32)), seed
+
+
+def test_append_bad_places_in_a_prompt(tq, dev):
+    """One page of a prompt outside the pool: its tokens are skipped, the others stored, neighbours untouched."""
+    page, dim, n = 32, 128, 90
+    k, v = pr.Pool(tq, 1, 4, 1, page, dim, 3, dev), pr.Pool(tq, 2, 4, 1, page, dim, 4, dev)
+    x = torch.randn((1, 1, n, dim), device=dev, dtype=torch.float16)
+    before = [(p.packed.view(torch.int32).clone(), p.norms.clone()) for p in (k, v)]
+    tq.paged_append(x, x, k=k.desc, v=v.desc, page_table=torch.tensor([[2, 9, 0]], dtype=torch.int32, device=dev),
+                    starts=torch.tensor([5], dtype=torch.int32, device=dev))
+    assert tq.paged_status(dev) in (1, 2)
+    pos = torch.arange(5, 5 + n, device=dev)
+    keep = (pos // page) != 1
+    for pool, (words, norms) in zip((k, v), before):
+        w, nn = tq.fused_quantize(x[0, 0], pool.quant.signs, pool.quant.boundaries, dim, pool.bits)
+        pg = torch.tensor([2, 9, 0], device=dev)[pos[keep] // page]
+        words[pg, 0, pos[keep] % page] = w.view(torch.int32)[keep]
+        norms[pg, 0, pos[keep] % page] = nn[keep]
+        assert torch.equal(pool.packed.view(torch.int32), words) and torch.equal(pool.norms, norms)
+
+
 def test_append_bad_places_are_skipped(tq, dev):
     """Pages outside the pool and positions behind the table are reported and not followed."""
     page, dim = 32, 128
