@@ -122,6 +122,14 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+// The 32 sign bits of a stretch of elements, laid out for 16-bit pairs: the even element of pair k at bit k, the odd one at
+// 16 + k, so that one shift and one mask put a pair's signs at bits 15 and 31.
+__device__ __forceinline__ uint32_t spread_signs(uint32_t w) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) r |= (((w >> (2 * k)) & 1u) << k) | (((w >> (2 * k + 1)) & 1u) << (16 + k));
+  return r;
+}
 // Raw butterfly of a vector of 128 spread over two threads (q = 0, 1): v[i] holds elements i and i + 32 of the thread's
 // 64, so that the stages 1 .. 16 are packed; the same sums and differences as a sequential butterfly (a - b as
 // fma(b, -1, a): one rounding, the same).
@@ -174,38 +182,33 @@ __host__ __device__ inline float bucket_float(float x, float mul, float add) {
 #endif
 }
 
+// Encodes 16 tokens of one head (n of them real).  rows / norms: where each token's words and norm go; `together`: the
+// rows are one stretch of memory.
 template <typename T, int BITS>
-__device__ __forceinline__ void encode_tokens(const AppendHalf& s, const BucketMap& map, uint32_t tab_lane,
-                                              uint32_t* stage, uint32_t* const* rows, float* const* norms, int b, int head,
-                                              int t0, int n, int lane) {
+__device__ __forceinline__ void encode_tokens(const AppendHalf& s, const BucketMap& map, uint32_t tab_lane, const uint32_t (&spread)[2],
+                                              uint32_t* stage, uint32_t* const* rows, float* const* norms, bool together,
+                                              const uint16_t* src0, int n, int lane) {
   constexpr int PD = packed_words(128, BITS);
   const int q = lane & 1, vs = lane >> 1;
-  const int t = t0 + min(vs, n - 1);                       // lanes behind the last token repeat it and store nothing
-  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(s.x) + b * s.batch_stride +
-                                                    head * s.head_stride + t * s.token_stride) + 8 * q;
+  // lanes behind the last token repeat it and store nothing
+  const uint4* src = reinterpret_cast<const uint4*>(src0 + min(vs, n - 1) * s.token_stride) + 8 * q;
   f2 x[32];
-  {
-    const uint32_t sw[2] = {s.h.signs.w[2 * q], s.h.signs.w[2 * q + 1]};        // bit e set: element e changes sign
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint4 wa = __ldg(src + c), wb = __ldg(src + 4 + c);                  // elements 8 c .. and 32 + 8 c ..
-      const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+  for (int c = 0; c < 4; ++c) {
+    const uint4 wa = __ldg(src + c), wb = __ldg(src + 4 + c);                  // elements 8 c .. and 32 + 8 c ..
+    const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int e = 8 * c + 2 * k;
-        float a0, a1, b0, b1;
-        if (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-          const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ua[k]));
-          const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&ub[k]));
-          a0 = fa.x; a1 = fa.y; b0 = fb.x; b1 = fb.y;
-        } else {
-          a0 = __uint_as_float(ua[k] << 16); a1 = __uint_as_float(ua[k] & 0xffff0000u);
-          b0 = __uint_as_float(ub[k] << 16); b1 = __uint_as_float(ub[k] & 0xffff0000u);
-        }
-        x[e] = pack2(__uint_as_float(__float_as_uint(a0) ^ ((sw[0] << (31 - e)) & 0x80000000u)),
-                     __uint_as_float(__float_as_uint(b0) ^ ((sw[1] << (31 - e)) & 0x80000000u)));
-        x[e + 1] = pack2(__uint_as_float(__float_as_uint(a1) ^ ((sw[0] << (30 - e)) & 0x80000000u)),
-                         __uint_as_float(__float_as_uint(b1) ^ ((sw[1] << (30 - e)) & 0x80000000u)));
+    for (int k = 0; k < 4; ++k) {
+      const int e = 8 * c + 2 * k;
+      const uint32_t fa = ua[k] ^ ((spread[0] << (15 - e / 2)) & 0x80008000u);        // signs of the pair
+      const uint32_t fb = ub[k] ^ ((spread[1] << (15 - e / 2)) & 0x80008000u);
+      if (std::is_same<T, __half>::value) {
+        const __half2 ha = *reinterpret_cast<const __half2*>(&fa), hb = *reinterpret_cast<const __half2*>(&fb);
+        x[e] = pack2(__low2float(ha), __low2float(hb));
+        x[e + 1] = pack2(__high2float(ha), __high2float(hb));
+      } else {
+        x[e] = pack2(__uint_as_float(fa << 16), __uint_as_float(fb << 16));
+        x[e + 1] = pack2(__uint_as_float(fa & 0xffff0000u), __uint_as_float(fb & 0xffff0000u));
       }
     }
   }
@@ -254,20 +257,33 @@ __device__ __forceinline__ void encode_tokens(const AppendHalf& s, const BucketM
   }
   if (BITS == 4) {
     if (vs < n) {
-      uint32_t* to = rows[vs] + DW * q;                     // rows are 16-byte aligned, or the launcher takes the other kernel
-      *reinterpret_cast<uint4*>(to) = make_uint4(dense[0], dense[1], dense[2], dense[3]);
-      *reinterpret_cast<uint4*>(to + 4) = make_uint4(dense[DW - 4], dense[DW - 3], dense[DW - 2], dense[DW - 1]);
+      uint4* to = reinterpret_cast<uint4*>(rows[vs] + DW * q);
+      to[0] = make_uint4(dense[0], dense[1], dense[2], dense[3]);
+      to[1] = make_uint4(dense[DW - 4], dense[DW - 3], dense[DW - 2], dense[DW - 1]);
     }
   } else {
-    // the vector's 384-bit string -> thirteen 30-bit words; the warp's rows are mostly one stretch of memory
-    uint32_t* ds = stage + vs * 13;
+    // this thread's 192 bits -> 30-bit words: the first thread's are words 0 .. 5 and the low 12 bits of word 6, the
+    // second's the high 18 bits of word 6 and words 7 .. 12
+    const uint32_t low12 = __shfl_xor_sync(0xffffffffu, dense[DW - 1] >> 20, 1);
+    uint32_t* to = stage + vs * PD;
 #pragma unroll
-    for (int w = 0; w < DW; ++w) ds[DW * q + w] = dense[w];
-    if (q == 0) ds[12] = 0;
+    for (int k = 0; k < 6; ++k) {
+      const int b0 = 30 * k, b1 = 18 + 30 * k;               // first bit of word k (first thread), of word 7 + k (second)
+      const uint32_t w0 = __funnelshift_r(dense[b0 >> 5], (b0 >> 5) + 1 < DW ? dense[((b0 >> 5) + 1) % DW] : 0u, b0 & 31);
+      const uint32_t w1 = __funnelshift_r(dense[b1 >> 5], (b1 >> 5) + 1 < DW ? dense[((b1 >> 5) + 1) % DW] : 0u, b1 & 31);
+      to[q ? 7 + k : k] = (q ? w1 : w0) & 0x3fffffffu;
+    }
+    if (q) to[6] = low12 | ((dense[0] & 0x3ffffu) << 12);
     __syncwarp();
-    for (int i = lane; i < n * PD; i += 32) {
-      const int r = i / PD, w = i - r * PD, bit = 30 * w, dw = bit >> 5;
-      rows[r][w] = __funnelshift_r(stage[r * 13 + dw], dw < 12 ? stage[r * 13 + dw + 1] : 0u, bit & 31) & 0x3fffffffu;
+    if (together) {
+      uint32_t* dst = rows[0];
+#pragma unroll
+      for (int k = 0; k < (kSplitTokens * PD + 31) / 32; ++k) {
+        const int i = 32 * k + lane;
+        if (i < n * PD) dst[i] = stage[i];
+      }
+    } else {
+      for (int i = lane; i < n * PD; i += 32) rows[i / PD][i % PD] = stage[i];
     }
   }
   if (q == 0 && vs < n) *norms[vs] = nrm;
@@ -277,20 +293,18 @@ __device__ __forceinline__ void encode_tokens(const AppendHalf& s, const BucketM
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32, 2)
 paged_append_split_kernel(const __grid_constant__ SplitArgs p) {
-  __shared__ __align__(256) uint2 table[kBuckets * 32];
+  __shared__ __align__(256) uint2 table[2][kBuckets * 32];
   __shared__ uint32_t stage_s[kWarps][kSplitTokens * 13];
   __shared__ uint32_t* rows_s[kWarps][kSplitTokens];
   __shared__ float* norms_s[kWarps][kSplitTokens];
   const AppendArgs& a = p.a;
-  const int which = blockIdx.y;
-  const AppendHalf& s = a.half[which];
-  const BucketMap& map = p.map[which];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (s.h.format == TQ_KV_POLAR)
-    for (int i = threadIdx.x; i < kBuckets * 32; i += kWarps * 32)
-      table[i] = make_uint2(__float_as_uint(map.thr[i >> 5]), map.below[i >> 5]);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & 1;
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+    if (a.half[which].h.format == TQ_KV_POLAR)
+      for (int i = threadIdx.x; i < kBuckets * 32; i += kWarps * 32)
+        table[which][i] = make_uint2(__float_as_uint(p.map[which].thr[i >> 5]), p.map[which].below[i >> 5]);
   __syncthreads();
-  const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table) + lane * 8;
   const int chunks = (a.tokens + kSplitTokens - 1) / kSplitTokens;
   const int64_t units = (int64_t)a.batch * a.heads * chunks;
   for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
@@ -299,50 +313,56 @@ paged_append_split_kernel(const __grid_constant__ SplitArgs p) {
     const int count = min(a.tokens, a.counts ? __ldg(a.counts + b) : a.tokens);
     const int n = min(kSplitTokens, count - t0);
     if (n <= 0) continue;
-    if (lane < n) {
-      int row = 0;
-      const int page = append_place(a, b, t0 + lane, &row);
-      uint32_t* to = nullptr;
-      if (page >= 0) {
-        if (s.h.format == TQ_KV_DENSE)
-          to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(s.h.data) + page * s.h.page_stride +
-                                           head * s.h.head_stride + (int64_t)row * 128);
+    int row = 0;
+    const int page = append_place(a, b, t0 + min(lane, n - 1), &row);        // lane = token
+    const bool all = __all_sync(0xffffffffu, page >= 0);
+    const bool together = __all_sync(0xffffffffu, page == __shfl_sync(0xffffffffu, page, 0));
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      const AppendHalf& s = a.half[which];
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(s.x) + b * s.batch_stride + head * s.head_stride + t0 * s.token_stride;
+      if (lane < kSplitTokens) {
+        uint32_t* to = nullptr;
+        if (page >= 0) {
+          if (s.h.format == TQ_KV_DENSE)
+            to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(s.h.data) + page * s.h.page_stride +
+                                             head * s.h.head_stride + (int64_t)row * 128);
+          else
+            to = reinterpret_cast<uint32_t*>(s.h.data) + page * s.h.page_stride + head * s.h.head_stride +
+                 row * packed_words(128, s.h.bits);
+          norms_s[warp][lane] = s.h.norms + page * s.h.norm_page_stride + head * s.h.norm_head_stride + row;
+        }
+        rows_s[warp][lane] = to;
+      }
+      __syncwarp();
+      if (s.h.format == TQ_KV_DENSE) {
+        for (int i = lane; i < n * 16; i += 32) {          // 16 chunks of 16 bytes per row
+          const int r = i >> 4, c = i & 15;
+          uint4* to = reinterpret_cast<uint4*>(rows_s[warp][r]);
+          if (to) to[c] = __ldg(reinterpret_cast<const uint4*>(src + r * s.token_stride) + c);
+        }
+      } else if (all) {
+        const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table[which]) + lane * 8;
+        const uint32_t spread[2] = {spread_signs(s.h.signs.w[2 * q]), spread_signs(s.h.signs.w[2 * q + 1])};
+        if (s.h.bits == 3)
+          encode_tokens<T, 3>(s, p.map[which], tab_lane, spread, stage_s[warp], rows_s[warp], norms_s[warp], together, src, n, lane);
         else
-          to = reinterpret_cast<uint32_t*>(s.h.data) + page * s.h.page_stride + head * s.h.head_stride +
-               (int64_t)row * packed_words(128, s.h.bits);
-        norms_s[warp][lane] = s.h.norms + page * s.h.norm_page_stride + head * s.h.norm_head_stride + row;
-      }
-      rows_s[warp][lane] = to;
-    }
-    __syncwarp();
-    const bool all = __all_sync(0xffffffffu, lane >= n || rows_s[warp][lane < n ? lane : 0] != nullptr);
-    if (s.h.format == TQ_KV_DENSE) {
-      for (int i = lane; i < n * 16; i += 32) {          // 16 chunks of 16 bytes per row
-        const int r = i >> 4, c = i & 15;
-        uint4* to = reinterpret_cast<uint4*>(rows_s[warp][r]);
-        if (to)
-          to[c] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(s.x) + b * s.batch_stride +
-                                                       head * s.head_stride + (t0 + r) * s.token_stride) + c);
-      }
-    } else if (all) {
-      if (s.h.bits == 3) encode_tokens<T, 3>(s, map, tab_lane, stage_s[warp], rows_s[warp], norms_s[warp], b, head, t0, n, lane);
-      else encode_tokens<T, 4>(s, map, tab_lane, stage_s[warp], rows_s[warp], norms_s[warp], b, head, t0, n, lane);
-    } else {
-      // some token has no place (reported): the others one by one
-      for (int r = 0; r < n; ++r) {
-        if (rows_s[warp][r] == nullptr) continue;
-        uint8_t* idx = reinterpret_cast<uint8_t*>(stage_s[warp]);
-        int row = 0;
-        const int page = append_place(a, b, t0 + r, &row);
-        float x[4];
+          encode_tokens<T, 4>(s, p.map[which], tab_lane, spread, stage_s[warp], rows_s[warp], norms_s[warp], together, src, n, lane);
+      } else {
+        // some token has no place (reported): the others one by one
+        for (int r = 0; r < n; ++r) {
+          const int pg = __shfl_sync(0xffffffffu, page, r), rw = __shfl_sync(0xffffffffu, row, r);
+          if (pg < 0) continue;
+          float x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[j] = load_elem(s.x, s.x_dtype, b * s.batch_stride + head * s.head_stride + (t0 + r) * s.token_stride + lane * 4 + j);
-        if (s.h.bits == 3) encode_row<4, 3>(s, x, idx, page, head, row, lane);
-        else encode_row<4, 4>(s, x, idx, page, head, row, lane);
+          for (int j = 0; j < 4; ++j) x[j] = load_elem(src, s.x_dtype, r * s.token_stride + lane * 4 + j);
+          uint8_t* idx = reinterpret_cast<uint8_t*>(stage_s[warp]);
+          if (s.h.bits == 3) encode_row<4, 3>(s, x, idx, pg, head, rw, lane);
+          else encode_row<4, 4>(s, x, idx, pg, head, rw, lane);
+        }
       }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
@@ -380,8 +400,8 @@ bool split_supported(const AppendHalf& s, BucketMap* map) {
 
 int launch_append_split(const SplitArgs& p, cudaStream_t st) {
   const int64_t units = (int64_t)p.a.batch * p.a.heads * ((p.a.tokens + kSplitTokens - 1) / kSplitTokens);
-  const int64_t blocks = (units + kWarps - 1) / kWarps, cap = (int64_t)num_sms() * 4;
-  const dim3 grid((unsigned)(blocks < cap ? blocks : cap), 2);
+  const int64_t blocks = (units + kWarps - 1) / kWarps, cap = (int64_t)num_sms() * 2;
+  const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
   if (p.a.half[0].x_dtype == TQ_F16) paged_append_split_kernel<__half><<<grid, kWarps * 32, 0, st>>>(p);
   else paged_append_split_kernel<__nv_bfloat16><<<grid, kWarps * 32, 0, st>>>(p);
   return check_launch("tq_paged_append (split)");
@@ -470,7 +490,7 @@ paged_read_split_kernel(const __grid_constant__ ReadArgs a) {
   __syncthreads();
   const uint32_t tab = (uint32_t)__cvta_generic_to_shared(dyn) + (lane & 15) * 8;
   const uint32_t out_at = (uint32_t)__cvta_generic_to_shared(out_s);
-  const uint32_t sw[2] = {a.h.signs.w[2 * q], a.h.signs.w[2 * q + 1]};
+  const uint32_t spread[2] = {spread_signs(a.h.signs.w[2 * q]), spread_signs(a.h.signs.w[2 * q + 1])};
   const f2 s2 = pack2(a.s, a.s);
   const int64_t chunks = (a.length + kReadRows - 1) / kReadRows, units = (int64_t)a.batch * a.heads * chunks;
   for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
@@ -479,7 +499,14 @@ paged_read_split_kernel(const __grid_constant__ ReadArgs a) {
     const int n = min(__ldg(a.lens + b), a.view.capacity());
     const int pos = p0 + vs;
     const int last = (int)min((int64_t)kReadRows, a.length - p0);                  // rows of this chunk in the output
-    int page = pos < n && vs < last ? a.view.page_of(b, pos) : -1;
+    uint4* out = reinterpret_cast<uint4*>(a.out) + (bh * a.length + p0) * 16;
+    if (p0 >= n) {                       // the whole chunk lies behind the sequence
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (2 * k + (lane >> 4) < last) out[k * 32 + lane] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const int page = pos < n && vs < last ? a.view.page_of(b, pos) : -1;
     const bool missing = pos < n && vs < last && page < 0;
     if (missing && q == 0) atomicExch(a.view.status, 1);
     uint32_t dense[DW + 1];
@@ -539,11 +566,18 @@ paged_read_split_kernel(const __grid_constant__ ReadArgs a) {
       }
     }
     butterfly_pairs(x, q);
+    // a row behind the sequence has norm 0 and no signs: zeros; one without a page is NaN
     const float nq = missing ? __int_as_float(0x7fc00000) : nrm;
     const f2 n2 = pack2(nq, nq);
+    const uint32_t fl[2] = {page >= 0 ? spread[0] : 0u, page >= 0 ? spread[1] : 0u};
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] = mul2(mul2(x[i], s2), n2);
-    const bool live = page >= 0;
+    // (the centroids of a row of norm 0 may be negative: x * 0 = -0; adding 0 clears it)
+    const f2 zero2 = pack2(0.f, 0.f);
+    if (__any_sync(0xffffffffu, page < 0)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = page < 0 ? add2(x[i], zero2) : x[i];
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -561,16 +595,13 @@ paged_read_split_kernel(const __grid_constant__ ReadArgs a) {
             const __nv_bfloat162 v = __floats2bfloat162_rn(y0, y1);
             h = *reinterpret_cast<const uint32_t*>(&v);
           }
-          // signs of elements e and e + 1: bits 15 and 31
-          const uint32_t flip = ((sw[half] >> e) & 1u) << 15 | ((sw[half] >> (e + 1)) & 1u) << 31;
-          pk[k] = live || missing ? h ^ (missing ? 0u : flip) : 0u;
+          pk[k] = h ^ ((fl[half] << (15 - e / 2)) & 0x80008000u);      // signs of elements e and e + 1
         }
         const int chunk = 8 * q + 4 * half + c;              // 16-byte chunk of the row; places are swizzled against conflicts
         const uint32_t at = out_at + vs * 256 + (chunk & 8) * 16 + ((chunk & 7) ^ ((2 * vs + q) & 7)) * 16;
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
       }
     __syncwarp();
-    uint4* out = reinterpret_cast<uint4*>(a.out) + (bh * a.length + p0) * 16;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int r = 2 * k + (lane >> 4), chunk = lane & 15;
