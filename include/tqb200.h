@@ -454,7 +454,8 @@ int tq_paged_append(const tq_paged_params* p);
 int64_t tq_paged_decode_workspace_bytes(int dim);
 int tq_paged_decode(const tq_paged_params* p);
 /* Positions [0, tokens) of every sequence as dense rows (batch, heads, tokens, dim), contiguous;
- * rows at and behind seq_lens[b] are zero.  tq_dequantize's arithmetic (the same bits). */
+ * rows at and behind seq_lens[b] are zero, and so are rows whose table entry is -1 (a page
+ * freed behind a window).  tq_dequantize's arithmetic (the same bits). */
 int tq_paged_dequantize(const tq_paged_params* p);
 /* Copies page src[i] to page dst[i] in each of n_pools arrays of n_pages pages (page_bytes[j]
  * bytes per page, multiples of 16, 16-byte aligned).  src / dst are device arrays; no page may be

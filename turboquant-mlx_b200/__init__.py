@@ -25,6 +25,7 @@ from .kernels import (
     prefill_attention,
 )
 from .paged import paged_append, paged_decode, paged_dequantize, copy_pages, paged_status
+from .paged_cache import PagedSequences, PagedTurboQuantCache, make_paged_caches
 from .fused_attention import turboquant_attention
 from .packing import pack_indices, unpack_indices, packed_dim
 from .rotation import (

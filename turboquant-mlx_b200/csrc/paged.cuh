@@ -48,9 +48,10 @@ struct PageView {
     const int64_t c = (int64_t)table_width << page_shift;
     return c > 0x7fffffe0 ? 0x7fffffe0 : (int)c;
   }
+  __device__ __forceinline__ int entry(int b, int pos) const { return __ldg(table + b * table_stride + (pos >> page_shift)); }
   // Pool page of position `pos` of sequence b, -1 when the table names none in the pool.
   __device__ __forceinline__ int page_of(int b, int pos) const {
-    const int id = __ldg(table + b * table_stride + (pos >> page_shift));
+    const int id = entry(b, pos);
     return id >= 0 && id < n_pages ? id : -1;
   }
 };

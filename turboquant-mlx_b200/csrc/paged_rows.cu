@@ -250,10 +250,15 @@ __device__ __forceinline__ void encode_tokens(const AppendHalf& s, const BucketM
     const uint32_t at = (__float_as_uint(bucket_float(v, map.mul, map.add)) << 8) + tab_lane;     // 2^23's exponent is shifted out
     uint32_t thr, below;
     asm("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(thr), "=r"(below) : "r"(at));
-    const uint32_t code = below + (v > __uint_as_float(thr) ? 1u : 0u);
     const int bit = i * BITS, w = bit >> 5, sh = bit & 31;
-    dense[w] += code << sh;                                 // fields never overlap: + is |
-    if (sh + BITS > 32) dense[w + 1] += code >> (32 - sh);
+    if (sh + BITS > 32) {                                   // the code straddles two words
+      const uint32_t code = below + (v > __uint_as_float(thr) ? 1u : 0u);
+      dense[w] += code << sh;
+      dense[w + 1] += code >> (32 - sh);
+    } else {                                                // fields never overlap: + is |
+      dense[w] += below << sh;
+      if (v > __uint_as_float(thr)) dense[w] += 1u << sh;
+    }
   }
   if (BITS == 4) {
     if (vs < n) {
@@ -297,6 +302,8 @@ paged_append_split_kernel(const __grid_constant__ SplitArgs p) {
   __shared__ uint32_t stage_s[kWarps][kSplitTokens * 13];
   __shared__ uint32_t* rows_s[kWarps][kSplitTokens];
   __shared__ float* norms_s[kWarps][kSplitTokens];
+  constexpr int kEntries = 256;
+  __shared__ int prefix[kEntries + 1];
   const AppendArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane & 1;
 #pragma unroll
@@ -305,20 +312,58 @@ paged_append_split_kernel(const __grid_constant__ SplitArgs p) {
       for (int i = threadIdx.x; i < kBuckets * 32; i += kWarps * 32)
         table[which][i] = make_uint2(__float_as_uint(p.map[which].thr[i >> 5]), p.map[which].below[i >> 5]);
   __syncthreads();
-  const int chunks = (a.tokens + kSplitTokens - 1) / kSplitTokens;
-  const int64_t units = (int64_t)a.batch * a.heads * chunks;
+  // Units of work: (sequence, half, head, 16 tokens), only those that exist: prefix[e] = chunks of 16 tokens in the
+  // sequences in front of entry e (kEntries entries of `per` sequences each).
+  const int per = (a.batch + kEntries - 1) / kEntries, entries = (a.batch + per - 1) / per;
+  auto chunks_of = [&](int b) {
+    const int count = min(a.tokens, a.counts ? __ldg(a.counts + b) : a.tokens);
+    return (max(count, 0) + kSplitTokens - 1) / kSplitTokens;
+  };
+  for (int e = threadIdx.x; e < entries; e += kWarps * 32) {
+    int c = 0;
+    for (int b = e * per; b < min(a.batch, (e + 1) * per); ++b) c += chunks_of(b);
+    prefix[e + 1] = c;
+  }
+  if (threadIdx.x == 0) prefix[0] = 0;
+  __syncthreads();
+  if (warp == 0)
+    for (int e0 = 1, carry = 0; e0 <= entries; e0 += 32) {
+      const int e = e0 + lane;
+      int c = e <= entries ? prefix[e] : 0;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, c, k);
+        if (lane >= k) c += o;
+      }
+      c += carry;
+      if (e <= entries) prefix[e] = c;
+      carry = __shfl_sync(0xffffffffu, c, 31);
+    }
+  __syncthreads();
+  const int rows2 = 2 * a.heads;
+  const int64_t units = (int64_t)prefix[entries] * rows2;
   for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
-    const int64_t bh = u / chunks;
-    const int t0 = (int)(u - bh * chunks) * kSplitTokens, b = (int)(bh / a.heads), head = (int)(bh - (int64_t)b * a.heads);
+    int e = 0, hi = entries - 1;
+    while (e < hi) {                           // last entry that does not begin behind u
+      const int mid = (e + hi + 1) / 2;
+      if ((int64_t)prefix[mid] * rows2 <= u) e = mid;
+      else hi = mid - 1;
+    }
+    int64_t rest = u - (int64_t)prefix[e] * rows2;
+    int b = e * per, chunks = chunks_of(b);
+    while (rest >= (int64_t)chunks * rows2) {
+      rest -= (int64_t)chunks * rows2;
+      chunks = chunks_of(++b);
+    }
+    const int hr = (int)(rest / chunks), t0 = (int)(rest - (int64_t)hr * chunks) * kSplitTokens;
+    const int which = hr / a.heads, head = hr - which * a.heads;
     const int count = min(a.tokens, a.counts ? __ldg(a.counts + b) : a.tokens);
     const int n = min(kSplitTokens, count - t0);
-    if (n <= 0) continue;
     int row = 0;
     const int page = append_place(a, b, t0 + min(lane, n - 1), &row);        // lane = token
     const bool all = __all_sync(0xffffffffu, page >= 0);
     const bool together = __all_sync(0xffffffffu, page == __shfl_sync(0xffffffffu, page, 0));
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
+    {
       const AppendHalf& s = a.half[which];
       const uint16_t* src = reinterpret_cast<const uint16_t*>(s.x) + b * s.batch_stride + head * s.head_stride + t0 * s.token_stride;
       if (lane < kSplitTokens) {
@@ -399,7 +444,7 @@ bool split_supported(const AppendHalf& s, BucketMap* map) {
 }
 
 int launch_append_split(const SplitArgs& p, cudaStream_t st) {
-  const int64_t units = (int64_t)p.a.batch * p.a.heads * ((p.a.tokens + kSplitTokens - 1) / kSplitTokens);
+  const int64_t units = (int64_t)p.a.batch * 2 * p.a.heads * ((p.a.tokens + kSplitTokens - 1) / kSplitTokens);
   const int64_t blocks = (units + kWarps - 1) / kWarps, cap = (int64_t)num_sms() * 2;
   const unsigned grid = (unsigned)(blocks < cap ? blocks : cap);
   if (p.a.half[0].x_dtype == TQ_F16) paged_append_split_kernel<__half><<<grid, kWarps * 32, 0, st>>>(p);
@@ -420,7 +465,7 @@ struct ReadArgs {
 };
 
 // One warp per row, lane = EPL consecutive elements: ((butterfly(c * s) * s) * sign) * norm in the order of the
-// contiguous decoder, so both give the same bits.  Rows behind a sequence are zero.
+// contiguous decoder, so both give the same bits.  Rows behind a sequence, or of a page it does not hold, are zero.
 template <int EPL>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_read_kernel(const ReadArgs a) {
@@ -437,10 +482,11 @@ paged_read_kernel(const ReadArgs a) {
     const int pos = (int)(v - bh * a.length), b = (int)(bh / a.heads), head = (int)(bh - (int64_t)b * a.heads);
     const int64_t to = v * DIM + lane * EPL;
     const int n = min(__ldg(a.lens + b), a.view.capacity());
-    const int page = pos < n ? a.view.page_of(b, pos) : -1;
-    if (pos < n && page < 0 && lane == 0) atomicExch(a.view.status, 1);
-    if (page < 0) {                  // behind the sequence: zero; a page outside the pool: NaN
-      const float x = pos < n ? __int_as_float(0x7fc00000) : 0.f;
+    const int page = pos < n ? a.view.entry(b, pos) : -1;
+    const bool wrong = page < -1 || page >= a.view.n_pages;
+    if (wrong && lane == 0) atomicExch(a.view.status, 1);
+    if (page < 0 || wrong) {         // behind the sequence, or no page held: zero; a page outside the pool: NaN
+      const float x = wrong ? __int_as_float(0x7fc00000) : 0.f;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) store_elem(a.out, a.out_dtype, to + j, x);
       continue;
@@ -506,8 +552,9 @@ paged_read_split_kernel(const __grid_constant__ ReadArgs a) {
         if (2 * k + (lane >> 4) < last) out[k * 32 + lane] = make_uint4(0, 0, 0, 0);
       continue;
     }
-    const int page = pos < n && vs < last ? a.view.page_of(b, pos) : -1;
-    const bool missing = pos < n && vs < last && page < 0;
+    int page = pos < n && vs < last ? a.view.entry(b, pos) : -1;
+    const bool missing = page < -1 || page >= a.view.n_pages;        // outside the pool; -1: no page held, zeros
+    if (missing) page = -1;
     if (missing && q == 0) atomicExch(a.view.status, 1);
     uint32_t dense[DW + 1];
     float nrm = 0.f;
@@ -678,8 +725,8 @@ extern "C" int tq_paged_append(const tq_paged_params* p) {
   a.starts = p->seq_lens;
   a.counts = p->counts;
   cudaStream_t st = (cudaStream_t)p->stream;
-  // From 16 tokens on a warp's worth of neighbouring rows exists: two threads per vector (six prompts of 5000 tokens, 8
-  // heads, 3-bit: 68 us against 184 with a warp per row).
+  // From 16 tokens on a warp's worth of neighbouring rows exists: two threads per vector (six prompts of up to 5000
+  // tokens, 8 heads, 3-bit: 60 us against 184 with a warp per row).
   if (p->dim == 128 && a.tokens >= kSplitTokens && a.half[0].x_dtype == a.half[1].x_dtype) {
     SplitArgs sp;
     memset(&sp, 0, sizeof(sp));

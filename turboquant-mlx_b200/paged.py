@@ -232,7 +232,8 @@ def paged_workspace_bytes(device, dim: int) -> int:
 def paged_dequantize(pool: dict, *, page_table: torch.Tensor, seq_lens: torch.Tensor, length: int, dtype=torch.float16,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Positions [0, length) of every sequence as dense rows: (B, H, length, dim) in `dtype`, the bits `dequant_fp16`
-    and `packed_dequantize` give; rows at and behind seq_lens[b] are zero.  Dense pools are gathered as they are.
+    and `packed_dequantize` give; rows at and behind seq_lens[b], and of pages that the sequence no longer holds
+    (table entry -1), are zero.  Dense pools are gathered as they are.
     `out` optionally names the contiguous tensor to write."""
     _lib.require_cuda(page_table)
     index = page_table.get_device()

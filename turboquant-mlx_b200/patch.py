@@ -26,8 +26,11 @@ def _prefill_sdpa(queries, keys, values, scale, mask):
 def _patched_sdpa(queries, keys, values, cache, scale, mask, sinks=None):
     """Fused TurboQuant decode, affine-quantized decode, or the original attention."""
     from .cache import TurboQuantKVCache
+    from .paged_cache import PagedTurboQuantCache
     from .v_only_cache import VOnlyTurboQuantCache
 
+    if isinstance(cache, PagedTurboQuantCache):
+        return cache.attention(queries, scale, mask)
     is_decode = queries.shape[2] == 1
     if isinstance(cache, TurboQuantKVCache) and cache.offset > 0 and cache.fused and not cache.v_only:
         from .fused_attention import short_step_supported

@@ -114,7 +114,7 @@ class Qwen2Model:
 
     def decode_step(self, tok: torch.Tensor, caches, position: torch.Tensor) -> torch.Tensor:
         """One token per sequence, tok (B, 1), at the position held in the int32 device tensor
-        `position` (1,): logits (B, vocab).  Nothing here depends on a host-side length, so with caches
+        `position` (1,), or at one position per sequence (B,): logits (B, vocab).  Nothing here depends on a host-side length, so with caches
         in static decode mode (`enable_static_decode`) the whole step can be captured in a CUDA graph
         and replayed while the position advances on the device.  Same layer structure as `forward`,
         with the projections that share an input fused (17 launches per layer instead of ~35)."""
@@ -123,7 +123,7 @@ class Qwen2Model:
         D, nq, nkv = cfg.head_dim, cfg.n_q_heads, cfg.n_kv_heads
         half = D // 2
         x = self.emb[tok[:, 0]]
-        ang = position.to(torch.float32) * self.inv_freq
+        ang = position.to(torch.float32)[:, None, None] * self.inv_freq
         cos, sin = ang.cos().to(x.dtype), ang.sin().to(x.dtype)
         scale = 1.0 / math.sqrt(D)
         for lw, cache in zip(self.layers, caches):
@@ -205,3 +205,52 @@ class StaticDecoder:
     def close(self):
         for c in self.caches:
             c.disable_static_decode()
+
+
+class PagedDecoder:
+    """Greedy decoding of several sequences of different lengths over paged caches (`make_paged_caches`): prompts one by
+    one, then all sequences together, one CUDA-graph replay per token.  A step = embedding, all layers (insert at each
+    sequence's own position, attention over its own pages), logits, argmax, positions += 1; lengths, positions and page
+    tables are read on the device, and the pages of all tokens of a run are taken before it."""
+
+    def __init__(self, model: Qwen2Model, caches):
+        from . import patch
+        if base.scaled_dot_product_attention is not patch._patched_sdpa:
+            raise RuntimeError("paged caches are attended through the hook: call apply_patch() first")
+        self.model, self.caches, self.seqs = model, caches, caches[0].sequences
+
+    def prefill(self, prompt: torch.Tensor, seq: int | None = None):
+        """Run a prompt (L,) through the model, behind what `seq` already holds (default: a new sequence).  Returns
+        (sequence, next token (1, 1))."""
+        seq = self.seqs.add() if seq is None else seq
+        self.seqs.begin([seq], prompt.shape[0])
+        logits = self.model.forward(prompt[None], self.caches)
+        return seq, logits[:, -1].argmax(-1, keepdim=True)
+
+    def _step(self, tok):
+        tok.copy_(self.model.decode_step(tok, self.caches, self.seqs.starts).argmax(-1, keepdim=True))
+        self.seqs.advance_device()
+
+    def generate(self, ids, first_tok: torch.Tensor, n: int, use_graph: bool = True) -> torch.Tensor:
+        """n further tokens of the sequences `ids` after `first_tok` (B, 1): (B, n)."""
+        if n < 1:
+            return first_tok.new_empty((len(ids), 0))
+        self.seqs.begin(ids, 1, reserve=n - 1)
+        tok = first_tok.clone()
+        out = []
+        self._step(tok)                                   # eager: also the warm-up before a capture
+        out.append(tok.clone())
+        graph = None
+        if use_graph and n > 1:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self._step(tok)
+        while len(out) < n:
+            if graph is not None:
+                graph.replay()
+            else:
+                self._step(tok)
+            out.append(tok.clone())
+        self.seqs.advance(n - 1)
+        return torch.cat(out, dim=1)
