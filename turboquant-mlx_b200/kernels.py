@@ -724,20 +724,19 @@ def prefill_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.T
         raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, sinks need a window, "
                          "and a window needs causal attention")
     status = _lib.workspace(16, q.device, tag="prefill")
-    if window:
-        with torch.cuda.device(q.device):
-            _lib.check(_lib.lib().tq_prefill_sdpa_window(
-                _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
-                q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
-                v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1), out.stride(2),
-                float(scale), 1, min(int(window), 1 << 40), min(int(sinks), 1 << 40), _lib.ptr(status),
-                _lib.stream_ptr(q.device)))
+    L_ = _lib.lib()
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
+            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale), 1 if causal else 0)
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    if not window:
+        _lib.check(L_.tq_prefill_sdpa(*args, status.data_ptr(), stream))
         return out
-    _lib.check(_lib.lib().tq_prefill_sdpa(
-        _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(out), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
-        q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
-        v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1), out.stride(2),
-        float(scale), 1 if causal else 0, _lib.ptr(status), _lib.stream_ptr(q.device)))
+    args += (min(int(window), 1 << 40), min(int(sinks), 1 << 40), status.data_ptr(), stream)
+    if q.device.index == torch.cuda.current_device():
+        _lib.check(L_.tq_prefill_sdpa_window(*args))
+    else:
+        with torch.cuda.device(q.device):
+            _lib.check(L_.tq_prefill_sdpa_window(*args))
     return out
 
 

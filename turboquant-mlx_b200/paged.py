@@ -32,13 +32,16 @@ _PACK = _lib.PAGED_PARAMS.pack   # tq_paged_params in one call: a launch's host 
 _SIZE = _lib.PAGED_PARAMS.size
 _FORMATS = {torch.float32: _lib.TQ_F32, torch.float16: _lib.TQ_F16, torch.bfloat16: _lib.TQ_BF16}
 _addressof = ctypes.addressof
+_get_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_capturing = (torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing")
+              else torch.cuda.is_current_stream_capturing)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _call(fn, params: bytes, index: int) -> None:
     """One C call with device `index` current."""
-    if index == torch.cuda.current_device():
+    if index == _get_device():
         rc = fn(params)
     else:
         with torch.cuda.device(index):
@@ -197,24 +200,30 @@ def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
     if window < 0 or sinks < 0 or (sinks and not window):
         raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, and sinks need a window")
     if out is None:
-        out = q.new_empty(shape, dtype=out_dtype)
+        out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
     elif out.shape != shape or out.stride(2) != 1 or out.get_device() != index or (out_dtype or out.dtype) != out.dtype:
         raise ValueError(f"out must be {tuple(shape)} on cuda:{index}, with a contiguous last dimension and of out_dtype")
-    need = _workspace_bytes.get((index, dim)) or paged_workspace_bytes(index, dim)
-    if workspace is None:
-        stream = _raw_stream(index)
-        workspace = _workspaces.get((index, stream, dim))
-        if workspace is None or torch.cuda.is_current_stream_capturing():
-            workspace = q.new_zeros((need,), dtype=torch.uint8)        # captured: zeroed again by every replay
-            if not torch.cuda.is_current_stream_capturing():
-                _workspaces[(index, stream, dim)] = workspace
-    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != index or workspace.numel() < need:
-        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on cuda:{index}")
+    stream = _raw_stream(index)
+    if workspace is not None:
+        need = paged_workspace_bytes(index, dim)
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != index or workspace.numel() < need:
+            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on cuda:{index}")
+        scratch = (workspace.data_ptr(), workspace.numel())
+    elif _capturing():                                      # the graph's own, zeroed by every replay
+        workspace = torch.zeros((paged_workspace_bytes(index, dim),), dtype=torch.uint8, device=q.device)
+        scratch = (workspace.data_ptr(), workspace.numel())
+    else:
+        kept = _workspaces.get((index, stream, dim))
+        if kept is None:
+            need = paged_workspace_bytes(index, dim)
+            workspace = torch.zeros((need,), dtype=torch.uint8, device=q.device)
+            kept = _workspaces[(index, stream, dim)] = (workspace, (workspace.data_ptr(), need))
+        scratch = kept[1]
     qs, os = q.stride(), out.stride()
     _call(_lib.lib().tq_paged_decode, _PACK(
         _SIZE, B, n_q, geo[1], dim, geo[2], geo[0], table, row, lens, 0, 0, width, _dtype(q), _dtype(out), attn_scale,
         min(window, 0x7fffffff), min(sinks, 0x7fffffff), q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
-        workspace.data_ptr(), workspace.numel(), _raw_stream(index), *k0, 0, *k1, *_NO_ROWS, *v0, 0, *v1, *_NO_ROWS), index)
+        *scratch, stream, *k0, 0, *k1, *_NO_ROWS, *v0, 0, *v1, *_NO_ROWS), index)
     return out
 
 
@@ -274,15 +283,14 @@ def copy_pages(pools, src, dst) -> None:
     pools = list(pools)
     if not pools:
         return
+    T = torch.Tensor                                        # method descriptors in map: one call per tensor, nothing else
     _lib.require_cuda(pools[0])
     index, n_pages = pools[0].get_device(), pools[0].shape[0]
-    ptrs, sizes = [], []
-    for t in pools:
-        at = t.data_ptr()
-        if t.get_device() != index or t.shape[0] != n_pages or not t.is_contiguous() or at % 16:
-            raise ValueError("pools must be contiguous CUDA tensors, 16-byte aligned, of one device and one number of pages")
-        ptrs.append(at)
-        sizes.append(t.nbytes)
+    ptrs = list(map(T.data_ptr, pools))
+    if (set(map(T.get_device, pools)) != {index} or any([t.size(0) != n_pages for t in pools])
+            or not all(map(T.is_contiguous, pools)) or any([p & 15 for p in ptrs])):
+        raise ValueError("pools must be contiguous CUDA tensors, 16-byte aligned, of one device and one number of pages")
+    sizes = [t.nbytes for t in pools]
     (src, hs), (dst, hd) = _page_ids(src, n_pages, "src", index), _page_ids(dst, n_pages, "dst", index)
     n_pairs = src.numel()
     if n_pairs != dst.numel():
