@@ -47,28 +47,31 @@ struct MmaTables {
 constexpr uint32_t kBase = 1024;
 constexpr uint32_t kEnd = 228 * 1024;
 constexpr uint32_t up16(uint32_t x) { return (x + 15) & ~15u; }
-template <int KF, int VB, int W, int S, int H>
+template <int KF, int VB, int W, int S, int H, int P>
 struct Layout {
+  static constexpr int rings = W / P;                                   // P warps share a ring: each takes 32 H positions of its tiles
+  static_assert(W % P == 0, "whole rings");
   static constexpr uint32_t entry = dense(KF) ? 128 : 256;              // bytes between table entries (K and V side by side)
   static constexpr uint32_t v_entry = dense(KF) ? 0 : 128;
   static constexpr uint32_t entries = (KF == KF_P4 || VB == 4) ? 256 : 64;
   static constexpr uint32_t table_bytes = entries * entry;
   static constexpr uint32_t table = table_bytes > 16384 ? table_bytes : 16384, table_end = table + table_bytes;
   static constexpr uint32_t k_off = 0;
-  static constexpr uint32_t tile = 32 * H;                              // positions of a tile
+  static constexpr int blocks = H * P;                                  // blocks of 32 positions of a tile
+  static constexpr uint32_t tile = 32 * blocks;
   static constexpr uint32_t kn_off = tile * k_row_bytes(KF);
   static constexpr uint32_t v_off = kn_off + (dense(KF) ? 0 : tile * 4);
   static constexpr uint32_t vn_off = v_off + tile * v_row_bytes(VB);
   static constexpr uint32_t stage = vn_off + tile * 4;
   // below the table: barriers, scalars, the plan; what does not fit goes behind the table, ring stages fill both sides
-  static constexpr uint32_t full = kBase, empty = full + W * S * 8;     // mbarriers of the ring stages
-  static constexpr uint32_t info = empty + W * S * 8;                   // per stage: first position of its tile | flags
-  static constexpr uint32_t q_post = up16(info + W * S * 4);            // 8 floats
+  static constexpr uint32_t full = kBase, empty = full + rings * S * 8;     // mbarriers of the ring stages
+  static constexpr uint32_t info = empty + rings * S * 8;                   // per stage: first position of its tile | flags
+  static constexpr uint32_t q_post = up16(info + rings * S * 4);            // 8 floats
   static constexpr uint32_t ml = q_post + 32;                           // m, l of the warps that hand over rows: [2][W][8]
   static constexpr uint32_t flag = ml + 2 * W * 32;
   static constexpr uint32_t prefix = flag + 16;
   static constexpr uint32_t norms = up16(prefix + (kPlanEntries + 1) * 4);   // per warp: key norms, log2 value norms, value norms
-  static constexpr uint32_t q = norms + W * 3 * tile * 4;                 // query fragments [k-step][lane][4]
+  static constexpr uint32_t q = norms + W * 3 * 32 * H * 4;                 // query fragments [k-step][lane][4]
   static constexpr uint32_t small_end = q + 8 * 32 * 16;
   static constexpr int xch_warps = (W + 1) / 2;
   static constexpr uint32_t xch_row = kDim + 4;                         // padded: conflict-free stores
@@ -78,8 +81,8 @@ struct Layout {
   static constexpr uint32_t low = xch_low ? xch + xch_bytes : small_end;       // ring stages 0 .. low_stages - 1
   static constexpr uint32_t high = xch_low ? table_end : xch + xch_bytes;      // the others
   static constexpr int low_fit = (int)((table - low) / stage);
-  static constexpr int low_stages = low_fit < W * S ? low_fit : W * S;
-  static constexpr uint32_t end = high + (W * S - low_stages) * stage;
+  static constexpr int low_stages = low_fit < rings * S ? low_fit : rings * S;
+  static constexpr uint32_t end = high + (rings * S - low_stages) * stage;
   static_assert(small_end <= table, "the small arrays fit below the table");
   static_assert(xch_warps * 8 * xch_row * 4 <= xch_bytes, "row exchange fits");
   static_assert(low % 16 == 0 && high % 16 == 0 && stage % 16 == 0 && q % 16 == 0 && norms % 16 == 0, "alignment");
@@ -226,10 +229,10 @@ __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
 }
 __device__ __forceinline__ void sts_f32(uint32_t addr, float v) { sts32(addr, __float_as_uint(v)); }
 
-template <int KF, int VB, int W, int S, int H>
+template <int KF, int VB, int W, int S, int H, int P>
 __global__ void __launch_bounds__((W + 1) * 32, 1)
 paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constant__ MmaTables tb) {
-  using L = Layout<KF, VB, W, S, H>;
+  using L = Layout<KF, VB, W, S, H, P>;
   extern __shared__ __align__(1024) uint8_t smem[];       // shared address kBase
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -245,9 +248,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     return k < L::low_stages ? L::low + k * L::stage : L::high + (k - L::low_stages) * L::stage;
   };
   if (threadIdx.x == 0) sts32(L::flag, 0);
-  if (threadIdx.x < W * S) {
+  if (threadIdx.x < L::rings * S) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(L::full + 8 * threadIdx.x) : "memory");
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(L::empty + 8 * threadIdx.x) : "memory");
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(L::empty + 8 * threadIdx.x), "n"(P) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // pair tables, one copy per lane: K entry = (code of the lower element | code of the upper << bits), V entry =
@@ -280,15 +283,15 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   const Cursor end = ends[1];
   if (cur.at(end)) return;
 
-  // ---------------- producer: lane w fetches for warp w ----------------
-  // Each lane walks its warp's tiles on its own; the warp executes that walk once for all of them.
+  // ---------------- producer: lane r fetches for ring r ----------------
+  // Each lane walks its ring's tiles on its own; the warp executes that walk once for all of them.
   if (warp == W) {
     const bool polar = !dense(KF);
     const int row_mask = (1 << a.view.page_shift) - 1;
     Cursor fc = cur;                  // the piece the lane's next tile is in
-    int i = lane, cnt = lane < W ? cur.count_to(end) : 0;       // cnt 0: the lane has no tile left
-    int page[H];
-    const bool small_page = H == 2 && a.view.page_shift == 5;
+    int i = lane, cnt = lane < L::rings ? cur.count_to(end) : 0;       // cnt 0: the lane has no tile left
+    int page[L::blocks];
+    const bool small_page = L::blocks == 2 && a.view.page_shift == 5;
     const uint8_t *kb = nullptr, *vb = nullptr, *kn = nullptr, *vn = nullptr;      // the group's head in page 0
     auto bases = [&]() {
       const int head = rg_per_head == 1 ? fc.group : fc.group / rg_per_head;
@@ -313,7 +316,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         const int* entry = a.view.table + fc.b * a.view.table_stride + (pos >> a.view.page_shift);
         page[0] = __ldg(entry);
         // pages of 32 under tiles of 64: the second half has an entry of its own, if the sequence reaches it
-        if (H == 2 && small_page) page[H - 1] = pos + 32 < fc.span.n ? __ldg(entry + 1) : -1;
+        if (L::blocks == 2 && small_page) page[L::blocks - 1] = pos + 32 < fc.span.n ? __ldg(entry + 1) : -1;
       }
     };
     bases();
@@ -343,7 +346,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           // a half that the token does not see needs no page; one that it sees and that has none is missing
           uint32_t flags = full ? 1u : 0u, have = 0;
 #pragma unroll
-          for (int h = 0; h < H; ++h) {
+          for (int h = 0; h < L::blocks; ++h) {
             const int p = pos + 32 * h;
             const bool seen = p < fc.span.n && (p + 32 > fc.span.lo || p < a.sinks);
             const bool ok = page[h] >= 0 && page[h] < a.view.n_pages;
@@ -353,9 +356,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           if (flags & 6u) atomicExch(a.view.status, 1);
           sts32(L::info + 4 * (lane * S + s), (uint32_t)pos | flags);
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
-                       "r"((uint32_t)__popc(have) * (L::stage / H)) : "memory");
+                       "r"((uint32_t)__popc(have) * (L::stage / L::blocks)) : "memory");
 #pragma unroll
-          for (int h = 0; h < H; ++h)
+          for (int h = 0; h < L::blocks; ++h)
             if ((have >> h) & 1u) copy(page[h], 0, 32 * h, 32);
         }
         ++issued;
@@ -363,7 +366,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           s = 0;
           phase ^= 1u;
         }
-        i += W;
+        i += L::rings;
         settle();
       }
       __syncwarp();
@@ -391,7 +394,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   constexpr int kNg = KF == KF_P3 && VB == 3 ? 1 : 2, kC = KF == KF_P3 && VB == 3 ? 4 : 1;
   const int k_row0 = 8 * (g >> 1) + kC * ((g & 1) ^ (kSwap ? (g >> 1) & 1 : 0));
   const int v_row0 = 8 * t4 + kC * (kSwap ? t4 & 1 : 0), v_row1 = 8 * t4 + kC * (1 - (kSwap ? t4 & 1 : 0));
-  const uint32_t nrm = L::norms + warp * 3 * L::tile * 4;      // [3][tile]
+  const uint32_t nrm = L::norms + warp * 3 * 128 * H;          // [3][32 H]
   const uint32_t nrm_at = nrm + 4 * (kSwap ? lane ^ ((lane >> 3) & 1) : lane);      // the place of position `lane` in that order
   uint32_t lut_lane;                                     // table address of entry 0 in this lane's copy; opaque, so that
   asm("add.u32 %0, %1, %2;" : "=r"(lut_lane) : "r"(lane4), "n"(L::table));   // an address stays one logic operation
@@ -408,10 +411,11 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     return ((6 * i >= sh ? w >> (6 * i - sh) : w << (sh - 6 * i)) & (0x3Fu << sh)) | lut_lane;
   };
 
-  uint32_t st = stage_addr(warp, 0);
+  const int ring = warp / P, sub = H * (warp % P);             // the warp's ring; its first block of a tile
+  uint32_t st = stage_addr(ring, 0);
   int us = 0;                        // stage of the tile consumed next
   uint32_t phase = 0;
-  int i = warp;
+  int i = ring;
   // the group's query rows, four elements of rows warp, warp + W per lane: fetched a group ahead
   constexpr int kRpw = (kPagedRows + W - 1) / W;
   auto load_query = [&](const Cursor& c, float (&x)[kRpw][4]) {
@@ -481,24 +485,24 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    for (; i < cnt && !gave_up; i += W) {
-      if (!mbar_wait(L::full + 8 * (warp * S + us), phase)) {      // gave up: everything this CTA produces from here on is NaN
+    for (; i < cnt && !gave_up; i += L::rings) {
+      if (!mbar_wait(L::full + 8 * (ring * S + us), phase)) {      // gave up: everything this CTA produces from here on is NaN
         if (lane == 0) {
           sts32(L::flag, 1);
           atomicExch(a.view.status, 3);
         }
         break;
       }
-      const uint32_t info = lds32(L::info + 4 * (warp * S + us));
-      const int p0 = info & ~31u;
+      const uint32_t info = lds32(L::info + 4 * (ring * S + us));
+      const int p0 = (int)(info & ~31u) + 32 * sub;
       const bool full = info & 1u;
 #pragma unroll
       for (int h = 0; h < H; ++h) {   // norms: lane = position
         const bool seen = full || cur.span.sees(p0 + 32 * h + lane, a.sinks);
-        const float vn = seen ? lds_f32(st + L::vn_off + lane4 + 128 * h) : 0.f;
-        if (!dense(KF)) sts32(nrm_at + 128 * h, lds32(st + L::kn_off + lane4 + 128 * h));
-        sts_f32(nrm_at + 128 * h + L::tile * 4, lg2(fmaxf(vn, 1e-26f)));
-        sts_f32(nrm_at + 128 * h + L::tile * 8, vn);
+        const float vn = seen ? lds_f32(st + L::vn_off + lane4 + 128 * (sub + h)) : 0.f;
+        if (!dense(KF)) sts32(nrm_at + 128 * h, lds32(st + L::kn_off + lane4 + 128 * (sub + h)));
+        sts_f32(nrm_at + 128 * (H + h), lg2(fmaxf(vn, 1e-26f)));
+        sts_f32(nrm_at + 128 * (2 * H + h), vn);
       }
       __syncwarp();
       // ---------------- scores ----------------
@@ -506,7 +510,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
 #pragma unroll
       for (int ng = 0; ng < 4 * H; ++ng) {
         sc[ng][0] = sc[ng][1] = sc[ng][2] = sc[ng][3] = 0.f;
-        const uint32_t row = st + L::k_off + (32 * (ng >> 2) + k_row0 + kNg * (ng & 3)) * k_row_bytes(KF);
+        const uint32_t row = st + L::k_off + (32 * (sub + (ng >> 2)) + k_row0 + kNg * (ng & 3)) * k_row_bytes(KF);
         if (dense(KF)) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
@@ -540,7 +544,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         uint32_t off[2][16];          // table addresses of the 16 slots, for the two position pairs of this k-step
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int vrow = 32 * (step >> 1) + kNg * (2 * (step & 1) + p);
+          const int vrow = 32 * (sub + (step >> 1)) + kNg * (2 * (step & 1) + p);
           const uint32_t r0p = st + L::v_off + (v_row0 + vrow) * v_row_bytes(VB);
           const uint32_t r1p = st + L::v_off + (v_row1 + vrow) * v_row_bytes(VB);
           if (VB == 4) {
@@ -588,8 +592,6 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         }
       };
       // the first step's lookups wait for nothing: they fill the time the score products and the softmax take
-      uint32_t af0[8][4];
-      load_values(0, af0);
       // ---------------- softmax: head g ----------------
       float s2[8 * H], vn[8 * H], top = -INFINITY;       // [4 h + n-group][c]
       const float2 post2 = make_float2(post, post);
@@ -600,7 +602,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const uint32_t at = nrm + 128 * h + 32 * t4 + 16 * q;
-          const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + L::tile * 4), z = lds128(at + L::tile * 8);
+          const uint4 x = dense(KF) ? make_uint4(0, 0, 0, 0) : lds128(at), y = lds128(at + 128 * H), z = lds128(at + 256 * H);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -617,7 +619,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           if (!dense(KF)) v = mul2(v, make_float2(kn[i0], kn[i1]));
           if (!full) {
             const int pos = p0 + 32 * h + kNg * ng;
-            const bool missing = (info >> (1 + h)) & 1u;
+            const bool missing = (info >> (1 + sub + h)) & 1u;
             if (!cur.span.sees(pos + v_row0, a.sinks)) v.x = -INFINITY;
             if (!cur.span.sees(pos + v_row1, a.sinks)) v.y = -INFINITY;
             if (missing) v.x = v.y = __int_as_float(0x7fc00000);
@@ -658,22 +660,18 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       // ---------------- values ----------------
 #pragma unroll
       for (int step = 0; step < 2 * H; ++step) {
-        uint32_t af1[8][4];
-        if (step + 1 < 2 * H) load_values(step + 1, af1);
+        uint32_t af0[8][4];
+        load_values(step, af0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) mma<false>(o[j], af0[j], pb[2 * step], pb[2 * step + 1]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) af0[j][c] = af1[j][c];
       }
       __syncwarp();            // every lane is done with the stage (and with the norms)
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(L::empty + 8 * (warp * S + us)) : "memory");
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(L::empty + 8 * (ring * S + us)) : "memory");
       if (++us == S) {
         us = 0;
         phase ^= 1u;
       }
-      st = stage_addr(warp, us);
+      st = stage_addr(ring, us);
     }
     i -= cnt;                  // the warp's first tile of the next group
 
@@ -819,22 +817,22 @@ void scale_book(const float* c, int n, ScaledBook* out) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int KF, int VB, int W, int S, int H>
+template <int KF, int VB, int W, int S, int H, int P>
 int launch(PagedDecodeArgs& a, const MmaTables& tb, cudaStream_t st) {
-  using L = Layout<KF, VB, W, S, H>;
+  using L = Layout<KF, VB, W, S, H, P>;
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S, H, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)(L::end - kBase));
     if (e != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  a.tile_shift = H == 2 ? 6 : 5;
-  a.min_tiles = W;
-  a.group_cost = W;
-  return launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
+  a.tile_shift = L::blocks == 2 ? 6 : 5;
+  a.min_tiles = L::rings;
+  a.group_cost = L::rings;
+  return launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H, P>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
 }
 
 }  // namespace
@@ -887,11 +885,11 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st) {
   }
   const bool v3 = a.v.bits == 3;
   if (a.k.format == TQ_KV_DENSE) {
-    if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2, 1>(a, tb, st) : launch<KF_BF16, 4, 8, 2, 1>(a, tb, st);
-    return v3 ? launch<KF_F16, 3, 8, 2, 1>(a, tb, st) : launch<KF_F16, 4, 8, 2, 1>(a, tb, st);
+    if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2, 1, 1>(a, tb, st) : launch<KF_BF16, 4, 8, 2, 1, 1>(a, tb, st);
+    return v3 ? launch<KF_F16, 3, 8, 2, 1, 1>(a, tb, st) : launch<KF_F16, 4, 8, 2, 1, 1>(a, tb, st);
   }
-  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 2, 2>(a, tb, st) : launch<KF_P3, 4, 7, 2, 2>(a, tb, st);
-  return v3 ? launch<KF_P4, 3, 7, 2, 2>(a, tb, st) : launch<KF_P4, 4, 7, 2, 2>(a, tb, st);
+  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 2, 2, 1>(a, tb, st) : launch<KF_P3, 4, 7, 2, 2, 1>(a, tb, st);
+  return v3 ? launch<KF_P4, 3, 7, 2, 2, 1>(a, tb, st) : launch<KF_P4, 4, 7, 2, 2, 1>(a, tb, st);
 }
 
 }  // namespace tq
