@@ -47,7 +47,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
   float* q_s = dyn_s;                                   // [DIM][8]
   float* o_s = q_s + DIM * kPagedRows;                  // [kWarps][8][DIM]
   float* p_s = o_s + kWarps * kPagedRows * DIM;         // [kWarps][32][8]
-  __shared__ int prefix[kPlanEntries + 1];
+  __shared__ int prefix[kPlanInts];
   __shared__ float kc_s[16], vc_s[16];
   __shared__ float m_s[kWarps][kPagedRows], l_s[kWarps][kPagedRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -62,8 +62,8 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
   Cursor cur, end;
-  cur.seek(a, prefix, plan.begin(cta));
-  end.seek(a, prefix, plan.begin(cta + 1));
+  cur.seek_run(a, prefix, plan, cta, false, lane);
+  end.seek_run(a, prefix, plan, cta, true, lane);
   const int kvpw = vals_per_word(a.k.bits), kpd = packed_words(DIM, a.k.bits);
   const int vvpw = vals_per_word(a.v.bits), vpd = packed_words(DIM, a.v.bits);
   const uint32_t kmask = (1u << a.k.bits) - 1u, vmask = (1u << a.v.bits) - 1u;

@@ -11,7 +11,8 @@
 // sequence, group by group, are cut into runs of equal cost, one per CTA, whatever the lengths of the
 // sequences: a ragged batch loads every SM alike, and a single long sequence is split as finely as it needs.
 // Starting and finishing a group costs a CTA time too, so each group counts group_cost tiles more than it has
-// (a run that begins inside that lead begins at the group's first tile).  A CTA that holds all tiles of a
+// (a run that begins inside that lead begins at the group's first tile).  When there is a CTA for every group and
+// splitting would not save two rounds of a CTA's warps, each group gets one CTA instead.  A CTA that holds all tiles of a
 // group writes its output; otherwise it leaves a partial state (m, l, acc) in one of its two slots of the
 // workspace and counts itself in, and the CTA that completes the count joins the states and writes the output.
 // No CTA waits for another.
@@ -103,8 +104,10 @@ __device__ __forceinline__ int cost_of(const PagedDecodeArgs& a, const SeqSpan& 
 __device__ __forceinline__ int plan_stride(const PagedDecodeArgs& a) { return (a.batch + kPlanEntries - 1) / kPlanEntries; }
 __device__ __forceinline__ int plan_entries(const PagedDecodeArgs& a) { const int per = plan_stride(a); return (a.batch + per - 1) / per; }
 
-// prefix[e] = cost of one group in the sequences in front of entry e, prefix[n] = of all sequences.
-// Called by every thread of the block; `prefix` holds kPlanEntries + 1 ints.
+// prefix[e] = cost of one group in the sequences in front of entry e, prefix[n] = of all sequences; behind them the
+// largest cost of an entry and the number of entries that have any.  Called by every thread of the block; `prefix`
+// holds kPlanInts ints.
+constexpr int kPlanInts = kPlanEntries + 3;
 __device__ __forceinline__ void plan_costs(const PagedDecodeArgs& a, int* prefix) {
   const int per = plan_stride(a), n = plan_entries(a);
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
@@ -114,29 +117,36 @@ __device__ __forceinline__ void plan_costs(const PagedDecodeArgs& a, int* prefix
   }
   if (threadIdx.x == 0) prefix[0] = 0;
   __syncthreads();
-  if (n > 1) {
-    if (threadIdx.x < 32) {
-      int carry = 0;
-      for (int e0 = 1; e0 <= n; e0 += 32) {
-        const int e = e0 + threadIdx.x;
-        int t = e <= n ? prefix[e] : 0;
+  if (threadIdx.x < 32) {
+    int carry = 0, most = 0, some = 0;
+    for (int e0 = 1; e0 <= n; e0 += 32) {
+      const int e = e0 + threadIdx.x;
+      int t = e <= n ? prefix[e] : 0;
+      most = max(most, t);
+      some += t != 0;
 #pragma unroll
-        for (int k = 1; k < 32; k <<= 1) {
-          const int o = __shfl_up_sync(0xffffffffu, t, k);
-          if ((int)threadIdx.x >= k) t += o;
-        }
-        t += carry;
-        if (e <= n) prefix[e] = t;
-        carry = __shfl_sync(0xffffffffu, t, 31);
+      for (int k = 1; k < 32; k <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, t, k);
+        if ((int)threadIdx.x >= k) t += o;
       }
+      t += carry;
+      if (e <= n) prefix[e] = t;
+      carry = __shfl_sync(0xffffffffu, t, 31);
     }
-    __syncthreads();
+    most = __reduce_max_sync(0xffffffffu, most);
+    some = __reduce_add_sync(0xffffffffu, some);
+    if (threadIdx.x == 0) {
+      prefix[kPlanEntries + 1] = most;
+      prefix[kPlanEntries + 2] = some;
+    }
   }
+  __syncthreads();
 }
 
 struct Plan {
   int64_t total, q;    // cost of the launch; cost of a run (the first `r` runs have one more)
   int ctas, r;
+  bool whole;          // CTA c takes the c-th group that has tiles, whole
   __device__ __forceinline__ int64_t begin(int cta) const { return cta * q + min(cta, r); }
   // the CTA whose run holds point t of the numbering
   __device__ __forceinline__ int owner(int64_t t) const {
@@ -147,6 +157,20 @@ struct Plan {
 __device__ __forceinline__ Plan make_paged_plan(const PagedDecodeArgs& a, const int* prefix) {
   Plan p;
   p.total = (int64_t)prefix[plan_entries(a)] * a.groups;
+  const int most = prefix[kPlanEntries + 1] - a.group_cost, some = prefix[kPlanEntries + 2];
+  if (plan_stride(a) == 1 && (int64_t)some * a.groups <= a.ctas) {
+    // rounds of min_tiles tiles: the longest group alone, and an equal share of all
+    const int64_t tiles = p.total - (int64_t)some * a.groups * a.group_cost;
+    const int64_t share = (tiles + (int64_t)a.ctas * a.min_tiles - 1) / ((int64_t)a.ctas * a.min_tiles);
+    p.whole = (most + a.min_tiles - 1) / a.min_tiles <= share + 1;
+  } else {
+    p.whole = false;
+  }
+  if (p.whole) {
+    p.ctas = max(1, some * a.groups);
+    p.q = p.r = 0;
+    return p;
+  }
   p.ctas = p.total >= (int64_t)a.ctas * a.min_tiles ? a.ctas : max(1, (int)(p.total + a.min_tiles - 1) / a.min_tiles);
   if (p.total < (1ll << 31)) {           // 32-bit division is a tenth of the 64-bit one
     p.q = (uint32_t)p.total / (uint32_t)p.ctas;
@@ -201,6 +225,27 @@ struct Cursor {
       j = (int)(rest - (int64_t)group * cost);
     }
     j = max(0, j - a.group_cost);
+  }
+  // both ends of CTA `cta`'s run (one warp)
+  __device__ __forceinline__ void seek_run(const PagedDecodeArgs& a, const int* prefix, const Plan& plan, int cta, bool behind,
+                                           int lane) {
+    if (!plan.whole) {
+      seek(a, prefix, plan.begin(cta + behind));
+      return;
+    }
+    int k = cta / a.groups;                      // the k-th sequence that has tiles
+    for (int b0 = 0;; b0 += 32) {
+      const uint32_t some = __ballot_sync(0xffffffffu, b0 + lane < a.batch && prefix[b0 + lane + 1] != prefix[b0 + lane]);
+      if (k < __popc(some)) {
+        b = b0 + (int)__fns(some, 0, k + 1);
+        break;
+      }
+      k -= __popc(some);
+    }
+    group = cta % a.groups;
+    j = 0;
+    span = span_of(a, b);
+    if (behind) next_group(a);
   }
   // tiles from here to the end of the group, at most to `end`
   __device__ __forceinline__ int count_to(const Cursor& end) const {

@@ -70,7 +70,7 @@ struct Layout {
   static constexpr uint32_t ml = q_post + 32;                           // m, l of the warps that hand over rows: [2][W][8]
   static constexpr uint32_t flag = ml + 2 * W * 32;
   static constexpr uint32_t prefix = flag + 16;
-  static constexpr uint32_t norms = up16(prefix + (kPlanEntries + 1) * 4);   // per warp: key norms, log2 value norms, value norms
+  static constexpr uint32_t norms = up16(prefix + kPlanInts * 4);   // per warp: key norms, log2 value norms, value norms
   static constexpr uint32_t q = norms + W * 3 * 32 * H * 4;                 // query fragments [k-step][lane][4]
   static constexpr uint32_t small_end = q + 8 * 32 * 16;
   static constexpr int xch_warps = (W + 1) / 2;
@@ -275,7 +275,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   Cursor* ends = reinterpret_cast<Cursor*>(smem + L::xch - kBase);
   if (warp < 2) {
     Cursor c;
-    c.seek(a, prefix, plan.begin(cta + warp));
+    c.seek_run(a, prefix, plan, cta, warp == 1, lane);
     if (lane == 0) ends[warp] = c;
   }
   __syncthreads();
