@@ -56,7 +56,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
     vc_s[threadIdx.x] = a.v.cent.v[threadIdx.x];
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  plan_costs(a, prefix);
+  plan_costs(a, prefix, cost_early(a));
   zero_empty(a, DIM);
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
@@ -195,7 +195,6 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
           part[DIM] = mx;
           part[DIM + 1] = ls;
         }
-        __threadfence();
       }
     }
     __syncthreads();

@@ -108,11 +108,18 @@ __device__ __forceinline__ int plan_entries(const PagedDecodeArgs& a) { const in
 // largest cost of an entry and the number of entries that have any.  Called by every thread of the block; `prefix`
 // holds kPlanInts ints.
 constexpr int kPlanInts = kPlanEntries + 3;
-__device__ __forceinline__ void plan_costs(const PagedDecodeArgs& a, int* prefix) {
+// `early`: this thread's cost_early(), asked for ahead so that its load is on its way.
+__device__ __forceinline__ int cost_early(const PagedDecodeArgs& a) {
+  return (int)threadIdx.x < a.batch && plan_stride(a) == 1 ? cost_of(a, span_of(a, threadIdx.x)) : 0;
+}
+__device__ __forceinline__ void plan_costs(const PagedDecodeArgs& a, int* prefix, int early) {
   const int per = plan_stride(a), n = plan_entries(a);
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
-    int t = 0;
-    for (int b = e * per; b < min(a.batch, (e + 1) * per); ++b) t += cost_of(a, span_of(a, b));
+    int t = early;
+    if (per != 1 || e != (int)threadIdx.x) {
+      t = 0;
+      for (int b = e * per; b < min(a.batch, (e + 1) * per); ++b) t += cost_of(a, span_of(a, b));
+    }
     prefix[e + 1] = t;
   }
   if (threadIdx.x == 0) prefix[0] = 0;
@@ -308,8 +315,9 @@ __device__ __forceinline__ float* part_of(const PagedDecodeArgs& a, int c, int c
   return a.part + ((int64_t)(2 * c + (c == c0)) * kPagedRows + row) * (dim + 4);
 }
 
-// The CTA has stored its part of a split group (every storing thread has fenced, the block has met): counts it in and
-// says whether it was the last.  `first`: the group's first tile in the plan's numbering.  One thread.
+// The CTA has stored its part of a split group and its threads have met: counts it in and says whether it was the last
+// (release: everything before the meeting is visible to whoever sees the count; acquire: the others' parts are).  One
+// thread.
 __device__ __forceinline__ bool last_part(const PagedDecodeArgs& a, int c0, int c1) {
   int before;
   asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + c0) : "memory");
@@ -318,47 +326,63 @@ __device__ __forceinline__ bool last_part(const PagedDecodeArgs& a, int c0, int 
   return true;
 }
 
-// Joins one row of the parts c0 .. c1 of a group: m = max m_i, l = sum l_i 2^(m_i - m), acc likewise; one warp.
+// Joins one row of the parts c0 .. c1 of a group: m = max m_i, l = sum l_i 2^(m_i - m), acc likewise; one warp.  The
+// first rows are on their way while the weights are worked out.
 template <int EPL>
 __device__ __forceinline__ void join_row(const PagedDecodeArgs& a, int c0, int c1, int row, int b, int head, int lane) {
   constexpr int DIM = EPL * 32;
-  constexpr int kBatch = EPL <= 4 ? 12 : 4;          // parts whose rows a lane has in flight
-  float mx = -INFINITY, l = 0.f, v[EPL];
+  constexpr int kBatch = EPL <= 4 ? 16 : 8;          // parts whose rows a lane has in flight
+  constexpr int kOwn = kMaxCtas / 32;                // lane i keeps the states of parts i, i + 32, ...
+  const int n = c1 - c0 + 1;
+  float x[kBatch][EPL], m[kOwn], w[kOwn];
+  auto load = [&](int i0) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) v[j] = 0.f;
-  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(part_of(a, c, c0, row, DIM) + DIM));
-  mx = warp_max(mx);
-  for (int cb = c0; cb <= c1; cb += 32) {            // 32 parts: lane i knows the weight of part cb + i
-    float f = 0.f;
-    if (cb + lane <= c1) {
-      const float* p = part_of(a, cb + lane, c0, row, DIM) + DIM;
-      const float m = __ldcg(p), li = __ldcg(p + 1);
-      f = m == -INFINITY ? 1.f : paged_ex2(m - mx);  // m = -inf: l is 0, or NaN (a missing page)
-      l += li * f;
+    for (int k = 0; k < kBatch; ++k) {
+      const float* p = part_of(a, c0 + min(i0 + k, n - 1), c0, row, DIM) + lane * EPL;
+      if (EPL == 4) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
+        x[k][0] = f.x; x[k][EPL > 1 ? 1 : 0] = f.y; x[k][EPL > 2 ? 2 : 0] = f.z; x[k][EPL > 3 ? 3 : 0] = f.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
+      }
     }
-    const int n = min(32, c1 - cb + 1);
-    for (int i0 = 0; i0 < n; i0 += kBatch) {
-      float x[kBatch][EPL];
+  };
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const float* p = part_of(a, cb + min(i0 + k, n - 1), c0, row, DIM) + lane * EPL;
-        if (EPL == 4) {
-          const float4 w = __ldcg(reinterpret_cast<const float4*>(p));
-          x[k][0] = w.x; x[k][EPL > 1 ? 1 : 0] = w.y; x[k][EPL > 2 ? 2 : 0] = w.z; x[k][EPL > 3 ? 3 : 0] = w.w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < EPL; ++j) x[k][j] = __ldcg(p + j);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const float w = __shfl_sync(0xffffffffu, f, min(i0 + k, n - 1));
-#pragma unroll
-        for (int j = 0; j < EPL; ++j)
-          if (i0 + k < n) v[j] += x[k][j] * w;
-      }
+  for (int o = 0; o < kOwn; ++o) {
+    m[o] = -INFINITY;
+    w[o] = 0.f;
+    if (32 * o < n && 32 * o + lane < n) {
+      const float2 f = __ldcg(reinterpret_cast<const float2*>(part_of(a, c0 + 32 * o + lane, c0, row, DIM) + DIM));
+      m[o] = f.x;
+      w[o] = f.y;
     }
   }
+  load(0);
+  float mx = -INFINITY, l = 0.f, v[EPL];
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o) mx = fmaxf(mx, m[o]);
+  mx = warp_max(mx);
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o) {
+    const float f = m[o] == -INFINITY ? 1.f : paged_ex2(m[o] - mx);        // m = -inf: l is 0, or NaN (a missing page)
+    l += w[o] * f;
+    w[o] = f;
+  }
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) v[j] = 0.f;
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o)
+    for (int i0 = 32 * o; i0 < min(n, 32 * o + 32); i0 += kBatch) {
+      if (i0 > 0) load(i0);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float f = __shfl_sync(0xffffffffu, w[o], (i0 + k) & 31);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (i0 + k < n) v[j] += x[k][j] * f;
+      }
+    }
   finish_row<EPL>(a, b, head, v, warp_sum(l), lane);
 }
 #endif  // __CUDACC__

@@ -253,6 +253,10 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(L::empty + 8 * threadIdx.x), "n"(P) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // Everything above overlaps the end of the kernel in front; everything below may read what that kernel wrote.  (The
+  // tables could be built above, but while a kernel of this size runs in front there is no room on its SM to begin.)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int early = cost_early(a);       // a length is on its way while the tables are built
   // pair tables, one copy per lane: K entry = (code of the lower element | code of the upper << bits), V entry =
   // (code of the lower position | code of the upper << bits)
   for (uint32_t i = threadIdx.x; i < L::entries * 32; i += (W + 1) * 32) {
@@ -263,9 +267,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     }
     if (e < (1u << (2 * VB))) sts32(at + L::v_entry, (uint32_t)tb.v_c16[e & ((1 << VB) - 1)] | ((uint32_t)tb.v_c16[e >> VB] << 16));
   }
-  // Everything above overlaps the end of the kernel in front; everything below may read what that kernel wrote.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  plan_costs(a, prefix);          // also the barrier behind the tables
+  plan_costs(a, prefix, early);   // also the barrier behind the tables
   zero_empty(a, kDim);
   const Plan plan = make_paged_plan(a, prefix);
   const int cta = blockIdx.x;
@@ -751,7 +753,6 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           part[kDim] = mx;
           part[kDim + 1] = l;
         }
-        __threadfence();
       }
     }
     if (cnt != cur.span.tiles) {
