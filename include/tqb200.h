@@ -388,13 +388,22 @@ int tq_prefill_sdpa(const void* q, const void* k, const void* v, void* out, int 
  * j <= i + (seq_k - seq_q) with j > i + (seq_k - seq_q) - window or j < sinks.  Key tiles that no row of a query tile
  * sees are neither read nor computed, so the time follows the window, not the sequence.  No reference counterpart
  * (its mask helpers build such masks as arrays, cache.py:311-334). */
-int tq_prefill_sdpa_window(const void* q, const void* k, const void* v, void* out, int dtype, int batch,
-                           int n_q_heads, int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim,
-                           int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
-                           int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
-                           int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
-                           int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
-                           float attn_scale, int causal, int64_t window, int64_t sinks, int* status, void* stream);
+typedef struct tq_prefill_params {
+  int32_t struct_bytes;          /* sizeof(tq_prefill_params) */
+  int32_t dtype, batch, n_q_heads, n_kv_heads, dim;
+  int64_t seq_q, seq_k;
+  const void* q;                 /* strides in elements: batch, head, row */
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3];
+  int64_t window, sinks;
+  float attn_scale;
+  int32_t causal;
+  int* status;
+  void* stream;
+} tq_prefill_params;
+int tq_prefill_sdpa_window(const tq_prefill_params* p);
 
 /* ---- paged caches ------------------------------------------------------------
  * No reference counterpart (its caches are one array per layer).  A pool keeps the

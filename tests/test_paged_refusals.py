@@ -113,12 +113,18 @@ def test_copy_refusals(tq, ptr, nbytes, pages, pairs, code):
 def test_prompt_window_refusals(tq):
     L = tq._lib.lib()
 
-    def call(causal, window, sinks, scale=0.1):
-        one = ctypes.c_void_p(16)
-        return L.tq_prefill_sdpa_window(one, one, one, one, 1, 1, 2, 1, 4, 4, 128, *([1024] * 12), scale, causal, window, sinks, one, None)
+    def call(causal, window, sinks, scale=0.1, size=None):
+        P = tq._lib.PrefillParams()
+        P.struct_bytes = ctypes.sizeof(P) if size is None else size
+        P.dtype, P.batch, P.n_q_heads, P.n_kv_heads, P.dim, P.seq_q, P.seq_k = 1, 1, 2, 1, 128, 4, 4
+        P.q = P.k = P.v = P.out = P.status = 16
+        for name in ("q_strides", "k_strides", "v_strides", "o_strides"):
+            setattr(P, name, (ctypes.c_int64 * 3)(1024, 1024, 1024))
+        P.window, P.sinks, P.attn_scale, P.causal = window, sinks, scale, causal
+        return L.tq_prefill_sdpa_window(ctypes.byref(P))
 
     assert call(1, -1, 0) == -7 and call(1, 4, -1) == -7 and call(1, 0, 3) == -7 and call(0, 4, 0) == -8
-    assert call(1, 4, 0, scale=0.0) == -7
+    assert call(1, 4, 0, scale=0.0) == -7 and call(1, 4, 0, size=8) == -7 and L.tq_prefill_sdpa_window(None) == -7
 
 
 def test_wrappers_refuse_cpu_tensors(tq):

@@ -75,7 +75,7 @@ class FlashParams(ctypes.Structure):
 def _layout(cls, prefix=""):
     """struct-module format of a ctypes structure (native sizes, no implicit padding: the fields are checked to be
     packed), so that a whole argument block is filled by one call."""
-    codes = {c_int32: "i", c_int64: "q", c_void_p: "Q", c_float: "f", POINTER(c_float): "Q"}
+    codes = {c_int32: "i", c_int64: "q", c_void_p: "Q", c_float: "f", POINTER(c_float): "Q", c_int64 * 3: "3q"}
     out, at = "", 0
     for name, kind in cls._fields_:
         assert getattr(cls, name).offset == at, f"{cls.__name__}.{name} is not packed"
@@ -116,7 +116,21 @@ class PagedParams(ctypes.Structure):
     ]
 
 
+class PrefillParams(ctypes.Structure):
+    """Mirror of `tq_prefill_params` (include/tqb200.h)."""
+
+    _fields_ = [
+        ("struct_bytes", c_int32), ("dtype", c_int32), ("batch", c_int32), ("n_q_heads", c_int32), ("n_kv_heads", c_int32),
+        ("dim", c_int32), ("seq_q", c_int64), ("seq_k", c_int64),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p),
+        ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3), ("o_strides", c_int64 * 3),
+        ("window", c_int64), ("sinks", c_int64), ("attn_scale", c_float), ("causal", c_int32),
+        ("status", c_void_p), ("stream", c_void_p),
+    ]
+
+
 PAGED_PARAMS = struct.Struct("=" + _layout(PagedParams))
+PREFILL_PARAMS = struct.Struct("=" + _layout(PrefillParams))
 
 _lib = None
 
@@ -172,9 +186,7 @@ _SIGNATURES = {
     "tq_paged_dequantize": (c_int, [c_void_p]),
     "tq_copy_pages": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
     "tq_paged_status": (c_int, [POINTER(c_int), c_void_p]),
-    "tq_prefill_sdpa_window": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                                       c_int64, c_int64, c_int] + [c_int64] * 12
-                               + [c_float, c_int, c_int64, c_int64, c_void_p, c_void_p]),
+    "tq_prefill_sdpa_window": (c_int, [c_void_p]),
     "tq_prefill_sdpa": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                 c_int64, c_int64, c_int] + [c_int64] * 12 + [c_float, c_int, c_void_p, c_void_p]),
 }
@@ -225,8 +237,20 @@ def ptr(t: torch.Tensor | None) -> c_void_p:
     return c_void_p(t.data_ptr())
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def stream_handle(device=None) -> int:
+    """The current stream of a device as an integer."""
+    if isinstance(device, str):
+        device = torch.device(device)
+    index = device if isinstance(device, int) else getattr(device, "index", None)
+    return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
 def stream_ptr(device=None) -> c_void_p:
-    return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return c_void_p(stream_handle(device))
 
 
 # ---------------------------------------------------------------------------
@@ -284,7 +308,7 @@ def workspace(nbytes: int, device, tag: str = "flash") -> torch.Tensor | None:
     kernels never share it."""
     if nbytes <= 0:
         return None
-    key = (tag, str(device), torch.cuda.current_stream(device).cuda_stream)
+    key = (tag, str(device), stream_handle(device))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)

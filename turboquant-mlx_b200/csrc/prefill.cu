@@ -583,14 +583,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 }  // namespace tq
 
-extern "C" int tq_prefill_sdpa_window(const void* q, const void* k, const void* v, void* out, int dtype, int batch,
-                                      int n_q_heads, int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim,
-                                      int64_t q_batch_stride, int64_t q_head_stride, int64_t q_row_stride,
-                                      int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
-                                      int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
-                                      int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
-                                      float attn_scale, int causal, int64_t window, int64_t sinks, int* status,
-                                      void* stream) {
+static int prefill_sdpa(const void* q, const void* k, const void* v, void* out, int dtype, int batch, int n_q_heads,
+                        int n_kv_heads, int64_t seq_q, int64_t seq_k, int dim, int64_t q_batch_stride, int64_t q_head_stride,
+                        int64_t q_row_stride, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
+                        int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride, int64_t o_batch_stride,
+                        int64_t o_head_stride, int64_t o_row_stride, float attn_scale, int causal, int64_t window,
+                        int64_t sinks, int* status, void* stream) {
   using namespace tq;
   TQ_REQUIRE(window >= 0 && sinks >= 0, TQ_ERR_BAD_ARG, "window and sinks must not be negative");
   TQ_REQUIRE(window == 0 || causal, TQ_ERR_UNSUPPORTED, "a window needs causal attention");
@@ -655,8 +653,18 @@ extern "C" int tq_prefill_sdpa(const void* q, const void* k, const void* v, void
                                int64_t v_batch_stride, int64_t v_head_stride, int64_t v_row_stride,
                                int64_t o_batch_stride, int64_t o_head_stride, int64_t o_row_stride,
                                float attn_scale, int causal, int* status, void* stream) {
-  return tq_prefill_sdpa_window(q, k, v, out, dtype, batch, n_q_heads, n_kv_heads, seq_q, seq_k, dim, q_batch_stride,
-                                q_head_stride, q_row_stride, k_batch_stride, k_head_stride, k_row_stride, v_batch_stride,
-                                v_head_stride, v_row_stride, o_batch_stride, o_head_stride, o_row_stride, attn_scale,
-                                causal, 0, 0, status, stream);
+  return prefill_sdpa(q, k, v, out, dtype, batch, n_q_heads, n_kv_heads, seq_q, seq_k, dim, q_batch_stride, q_head_stride,
+                      q_row_stride, k_batch_stride, k_head_stride, k_row_stride, v_batch_stride, v_head_stride,
+                      v_row_stride, o_batch_stride, o_head_stride, o_row_stride, attn_scale, causal, 0, 0, status, stream);
+}
+
+extern "C" int tq_prefill_sdpa_window(const tq_prefill_params* p) {
+  using namespace tq;
+  TQ_REQUIRE(p != nullptr, TQ_ERR_BAD_ARG, "params pointer is NULL");
+  TQ_REQUIRE(p->struct_bytes == (int32_t)sizeof(tq_prefill_params), TQ_ERR_BAD_ARG,
+             "struct_bytes %d does not match this library (%zu)", p->struct_bytes, sizeof(tq_prefill_params));
+  return prefill_sdpa(p->q, p->k, p->v, p->out, p->dtype, p->batch, p->n_q_heads, p->n_kv_heads, p->seq_q, p->seq_k, p->dim,
+                      p->q_strides[0], p->q_strides[1], p->q_strides[2], p->k_strides[0], p->k_strides[1], p->k_strides[2],
+                      p->v_strides[0], p->v_strides[1], p->v_strides[2], p->o_strides[0], p->o_strides[1], p->o_strides[2],
+                      p->attn_scale, p->causal, p->window, p->sinks, p->status, p->stream);
 }

@@ -714,29 +714,31 @@ def prefill_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.T
         raise ValueError("keys and values must have the same (batch, heads, length)")
 
     def usable(t):
-        ok = t.stride(-1) == 1 and not any(st % 8 for st in t.stride()[:-1]) and t.data_ptr() % 16 == 0
-        return t if ok else t.contiguous()
+        st = t.stride()
+        return t if st[3] == 1 and not (st[0] | st[1] | st[2]) & 7 and not t.data_ptr() & 15 else t.contiguous()
 
     q, k, v = usable(queries), usable(keys), usable(values)
-    if out is None:
-        out = torch.empty((B, n_q, L, D), dtype=q.dtype, device=q.device)
     if window < 0 or sinks < 0 or (sinks and not window) or (window and not causal):
         raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, sinks need a window, "
                          "and a window needs causal attention")
-    status = _lib.workspace(16, q.device, tag="prefill")
-    L_ = _lib.lib()
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
-            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale), 1 if causal else 0)
-    stream = torch.cuda.current_stream(q.device).cuda_stream
+    if out is None:
+        out = torch.empty((B, n_q, L, D), dtype=q.dtype, device=q.device)
+    status = _lib.workspace(16, q.device, tag="prefill").data_ptr()
+    stream = _lib.stream_handle(q.device)
+    qs, ks, vs, os = q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3]
     if not window:
-        _lib.check(L_.tq_prefill_sdpa(*args, status.data_ptr(), stream))
+        _lib.check(_lib.lib().tq_prefill_sdpa(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
+            *qs, *ks, *vs, *os, float(scale), 1 if causal else 0, status, stream))
         return out
-    args += (min(int(window), 1 << 40), min(int(sinks), 1 << 40), status.data_ptr(), stream)
-    if q.device.index == torch.cuda.current_device():
-        _lib.check(L_.tq_prefill_sdpa_window(*args))
+    args = _lib.PREFILL_PARAMS.pack(
+        _lib.PREFILL_PARAMS.size, _lib.dtype_code(q.dtype), B, n_q, n_kv, D, L, S, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        out.data_ptr(), *qs, *ks, *vs, *os, min(int(window), 1 << 40), min(int(sinks), 1 << 40), scale, 1, status, stream)
+    if q.get_device() == torch.cuda.current_device():
+        _lib.check(_lib.lib().tq_prefill_sdpa_window(args))
     else:
         with torch.cuda.device(q.device):
-            _lib.check(L_.tq_prefill_sdpa_window(*args))
+            _lib.check(_lib.lib().tq_prefill_sdpa_window(args))
     return out
 
 

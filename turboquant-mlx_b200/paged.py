@@ -35,8 +35,7 @@ _addressof = ctypes.addressof
 _get_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _capturing = (torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing")
               else torch.cuda.is_current_stream_capturing)
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_raw_stream = _lib._raw_stream
 
 
 def _call(fn, params: bytes, index: int) -> None:
