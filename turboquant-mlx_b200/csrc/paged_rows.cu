@@ -340,22 +340,25 @@ paged_append_split_kernel(const __grid_constant__ SplitArgs p) {
       carry = __shfl_sync(0xffffffffu, c, 31);
     }
   __syncthreads();
-  const int rows2 = 2 * a.heads;
-  const int64_t units = (int64_t)prefix[entries] * rows2;
-  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
+  const uint32_t spread[2][2] = {
+      {spread_signs(a.half[0].h.signs.w[2 * q]), spread_signs(a.half[0].h.signs.w[2 * q + 1])},
+      {spread_signs(a.half[1].h.signs.w[2 * q]), spread_signs(a.half[1].h.signs.w[2 * q + 1])}};
+  const uint32_t rows2 = 2 * a.heads, units = (uint32_t)prefix[entries] * rows2;      // below 2^31: the launcher has checked
+  for (uint32_t u = blockIdx.x * kWarps + warp; u < units; u += gridDim.x * kWarps) {
     int e = 0, hi = entries - 1;
     while (e < hi) {                           // last entry that does not begin behind u
       const int mid = (e + hi + 1) / 2;
-      if ((int64_t)prefix[mid] * rows2 <= u) e = mid;
+      if ((uint32_t)prefix[mid] * rows2 <= u) e = mid;
       else hi = mid - 1;
     }
-    int64_t rest = u - (int64_t)prefix[e] * rows2;
-    int b = e * per, chunks = chunks_of(b);
-    while (rest >= (int64_t)chunks * rows2) {
-      rest -= (int64_t)chunks * rows2;
+    uint32_t rest = u - (uint32_t)prefix[e] * rows2;
+    int b = e * per;
+    uint32_t chunks = chunks_of(b);
+    while (rest >= chunks * rows2) {
+      rest -= chunks * rows2;
       chunks = chunks_of(++b);
     }
-    const int hr = (int)(rest / chunks), t0 = (int)(rest - (int64_t)hr * chunks) * kSplitTokens;
+    const int hr = (int)(rest / chunks), t0 = (int)(rest - (uint32_t)hr * chunks) * kSplitTokens;
     const int which = hr / a.heads, head = hr - which * a.heads;
     const int count = min(a.tokens, a.counts ? __ldg(a.counts + b) : a.tokens);
     const int n = min(kSplitTokens, count - t0);
@@ -388,11 +391,11 @@ paged_append_split_kernel(const __grid_constant__ SplitArgs p) {
         }
       } else if (all) {
         const uint32_t tab_lane = (uint32_t)__cvta_generic_to_shared(table[which]) + lane * 8;
-        const uint32_t spread[2] = {spread_signs(s.h.signs.w[2 * q]), spread_signs(s.h.signs.w[2 * q + 1])};
+        const uint32_t sg[2] = {which ? spread[1][0] : spread[0][0], which ? spread[1][1] : spread[0][1]};
         if (s.h.bits == 3)
-          encode_tokens<T, 3>(s, p.map[which], tab_lane, spread, stage_s[warp], rows_s[warp], norms_s[warp], together, src, n, lane);
+          encode_tokens<T, 3>(s, p.map[which], tab_lane, sg, stage_s[warp], rows_s[warp], norms_s[warp], together, src, n, lane);
         else
-          encode_tokens<T, 4>(s, p.map[which], tab_lane, spread, stage_s[warp], rows_s[warp], norms_s[warp], together, src, n, lane);
+          encode_tokens<T, 4>(s, p.map[which], tab_lane, sg, stage_s[warp], rows_s[warp], norms_s[warp], together, src, n, lane);
       } else {
         // some token has no place (reported): the others one by one
         for (int r = 0; r < n; ++r) {
@@ -727,7 +730,8 @@ extern "C" int tq_paged_append(const tq_paged_params* p) {
   cudaStream_t st = (cudaStream_t)p->stream;
   // From 16 tokens on a warp's worth of neighbouring rows exists: two threads per vector (six prompts of up to 5000
   // tokens, 8 heads, 3-bit: 60 us against 184 with a warp per row).
-  if (p->dim == 128 && a.tokens >= kSplitTokens && a.half[0].x_dtype == a.half[1].x_dtype) {
+  const int64_t units = (int64_t)a.batch * a.heads * ((a.tokens + kSplitTokens - 1) / kSplitTokens);
+  if (p->dim == 128 && a.tokens >= kSplitTokens && a.half[0].x_dtype == a.half[1].x_dtype && units < (1ll << 28)) {
     SplitArgs sp;
     memset(&sp, 0, sizeof(sp));
     if (split_supported(a.half[0], &sp.map[0]) && split_supported(a.half[1], &sp.map[1])) {
