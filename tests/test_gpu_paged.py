@@ -174,6 +174,140 @@ def test_decode_graph_replay_and_streams(tq, dev):
     pr.check(out, ref, tol)
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_decode_output_types(tq, dev, out_dtype):
+    _decode(tq, dev, lens=[300, 40], n_q=8, n_kv=2, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("kbits", [0, 3])
+def test_decode_one_bad_head_stays_alone(tq, dev, kbits):
+    """A query head of NaN or infinity spoils its own row and no other."""
+    got, (q, k, v, table, seq, scale) = _decode(tq, dev, lens=[200, 77], n_q=8, n_kv=2, kbits=kbits)
+    for bad in (float("nan"), float("inf")):
+        q2 = q.clone()
+        q2[0, 3, 5] = bad
+        out = tq.paged_decode(q2, k=k.desc, v=v.desc, page_table=table, seq_lens=seq, attn_scale=scale)
+        keep = torch.ones((2, 8), dtype=torch.bool, device=dev)
+        keep[0, 3] = False
+        assert torch.equal(out[keep], got[keep]) and not bool(out[0, 3].isfinite().all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 3.0])
+def test_decode_scales(tq, dev, scale):
+    _decode(tq, dev, lens=[300], n_q=8, n_kv=2, scale=scale, q_gain=0.3)
+
+
+@pytest.mark.parametrize("what", ["norms", "words", "strides"])
+def test_decode_unaligned_pools(tq, dev, what):
+    """Pools whose rows are not 16-byte aligned take the general kernel: same values."""
+    got, (q, k, v, table, seq, scale) = _decode(tq, dev, lens=[300, 77], n_q=8, n_kv=2)
+    desc = dict(v.desc)
+    P, H, page, words = v.packed.shape
+
+    def shifted(t, pad):
+        if what == "strides":
+            wide = torch.zeros((P, H * t[0, 0].numel() + 1), dtype=torch.int32, device=dev)
+            out = wide[:, :-1].view(P, H, *t.shape[2:]) if wide[:, :-1].is_contiguous() else wide.as_strided(
+                t.shape, (wide.stride(0), *t.stride()[1:]))
+        else:
+            out = torch.zeros((t.numel() + 1,), dtype=torch.int32, device=dev)[1:].view(t.shape)
+        out.copy_(t.view(torch.int32))
+        return out.view(t.dtype)
+    if what in ("words", "strides"):
+        desc["packed"] = shifted(v.packed, 1)
+    if what in ("norms", "strides"):
+        desc["norms"] = shifted(v.norms, 1)
+    out = tq.paged_decode(q, k=k.desc, v=desc, page_table=table, seq_lens=seq, attn_scale=scale)
+    ref, tol = pr.decode_ref(tq, q, k, v, table, [300, 77], scale, weight_eps=HALF_F16, out_dtype=out.dtype)
+    pr.check(out, ref, tol)
+
+
+@pytest.mark.parametrize("kind", ["uneven", "huge", "tiny"])
+def test_decode_other_codebooks(tq, dev, kind):
+    """Codebooks that have no good 16-bit scale take the 32-bit kernel."""
+    lens = [200]
+    table, pages = pr.make_table(lens, 64, 0, dev=dev)
+    k, v = pr.Pool(tq, 1, pages, 2, 64, 128, 3, dev), pr.Pool(tq, 2, pages, 2, 64, 128, 4, dev)
+    for p in (k, v):
+        n = 1 << p.bits
+        base = torch.linspace(-2.1, 2.3, n) + 0.013 * torch.arange(n) ** 2
+        p.quant.centroids = (base * {"uneven": 1.0, "huge": 1e6, "tiny": 1e-7}[kind]).float().to(dev)
+        p.desc["centroids"] = p.quant.centroids
+    q = torch.randn((1, 4, 128), generator=torch.Generator().manual_seed(0)).half().to(dev)
+    scale = {"uneven": 0.05, "huge": 5e-8, "tiny": 5e5}[kind]
+    out = tq.paged_decode(q, k=k.desc, v=v.desc, page_table=table, seq_lens=torch.tensor(lens, dtype=torch.int32, device=dev),
+                          attn_scale=scale, out_dtype=torch.float32)
+    # "uneven" may take either kernel: a 16-bit codebook is off by at most 2^-13 there
+    ref, tol = pr.decode_ref(tq, q, k, v, table, lens, scale, weight_eps=HALF_F16 + 4 * 2.0 ** -13, out_dtype=torch.float32)
+    pr.check(out, ref, tol)
+
+
+@pytest.mark.parametrize("stride", [(1 << 30) - 4096, 1 << 30])
+def test_decode_offsets_beyond_32_bits(tq, dev, stride):
+    """Pages whose byte offsets pass 2^32 (and element offsets 2^31): tensor-core and general kernel, insert, read-back and
+    page copies."""
+    H, page, words, P = 2, 64, 13, 3
+    lens = [150]
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=dev)
+    small = [pr.Pool(tq, s, P, H, page, 128, 3, dev) for s in (1, 2)]
+    q = torch.randn((1, 8, 128), generator=torch.Generator().manual_seed(0)).half().to(dev)
+    seq = torch.tensor(lens, dtype=torch.int32, device=dev)
+    want = tq.paged_decode(q, k=small[0].desc, v=small[1].desc, page_table=table, seq_lens=seq, attn_scale=0.1)
+    buf = torch.empty((2 * stride + H * page * words,), dtype=torch.int32, device=dev)
+    far = buf.as_strided((P, H, page, words), (stride, page * words, words, 1))
+    far.copy_(small[1].packed.view(torch.int32))
+    v = dict(small[1].desc, packed=far.view(torch.uint32))
+    got = tq.paged_decode(q, k=small[0].desc, v=v, page_table=table, seq_lens=seq, attn_scale=0.1)
+    ref, tol = pr.decode_ref(tq, q, small[0], small[1], table, lens, 0.1, weight_eps=HALF_F16, out_dtype=got.dtype)
+    pr.check(got, ref, tol)
+    assert stride >= 1 << 30 or torch.equal(got, want)
+    assert torch.equal(tq.paged_dequantize(v, page_table=table, seq_lens=seq, length=150),
+                       tq.paged_dequantize(small[1].desc, page_table=table, seq_lens=seq, length=150))
+    x = torch.randn((1, H, 30, 128), device=dev, dtype=torch.float16)
+    for desc in (v, small[1].desc):
+        tq.paged_append(x, x, k=small[0].desc, v=desc, page_table=table, starts=torch.tensor([120], dtype=torch.int32, device=dev))
+    assert torch.equal(far, small[1].packed.view(torch.int32))
+    del buf, far, v
+    big = torch.zeros((5, 1 << 28), dtype=torch.int32, device=dev)      # 1 GiB pages
+    big[4, -7:] = 5
+    tq.copy_pages([big], [4], [2])
+    assert torch.equal(big[2], big[4]) and not bool(big[:2].any())
+
+
+def test_first_call_inside_a_capture(tq, dev):
+    """A process whose first paged call is captured: works or raises, and the next eager call is right (child process)."""
+    code = """
+import torch, sys
+sys.path.insert(0, %r); sys.path.insert(0, %r)
+import __graft_entry__ as e, paged_ref as pr
+tq = e.load_package(); dev = torch.device("cuda", 0)
+table, pages = pr.make_table([100], 64, 0, dev=dev)
+k, v = pr.Pool(tq, 1, pages, 2, 64, 128, 3, dev), pr.Pool(tq, 2, pages, 2, 64, 128, 3, dev)
+q = torch.randn((1, 8, 128), device=dev, dtype=torch.float16)
+seq = torch.tensor([100], dtype=torch.int32, device=dev)
+call = lambda: tq.paged_decode(q, k=k.desc, v=v.desc, page_table=table, seq_lens=seq, attn_scale=0.1)
+torch.cuda.synchronize()
+g, out = torch.cuda.CUDAGraph(), None
+try:
+    with torch.cuda.graph(g):
+        out = call()
+except Exception as ex:
+    print("raised", type(ex).__name__)
+    out = None
+want = call()
+if out is not None:
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+ref, tol = pr.decode_ref(tq, q, k, v, table, [100], 0.1, weight_eps=2.0 ** -11, out_dtype=want.dtype)
+pr.check(want, ref, tol)
+print("fine")
+""" % (os.path.dirname(os.path.dirname(os.path.abspath(__file__))), os.path.dirname(os.path.abspath(__file__)))
+    import subprocess
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
 def test_decode_repeats_exactly(tq, dev):
     got, (q, k, v, table, seq, scale) = _decode(tq, dev, lens=[5000, 3], n_q=28, n_kv=4)
     for _ in range(3):

@@ -282,6 +282,9 @@ int check_paged_params(const tq_paged_params* p) {
   TQ_REQUIRE(p->n_pages > 0 && p->n_pages < (1ll << 31), TQ_ERR_BAD_ARG, "n_pages must be in [1, 2^31), got %lld",
              (long long)p->n_pages);
   TQ_REQUIRE(p->page_table && p->seq_lens && p->table_width > 0, TQ_ERR_BAD_ARG, "page_table and seq_lens are required");
+  // plans number the tiles of a batch in 32 bits
+  TQ_REQUIRE((int64_t)p->batch * ((int64_t)p->table_width * p->page_size / kMinPage + 64) < (1ll << 31), TQ_ERR_BAD_ARG,
+             "batch * table_width * page_size is too large");
   return TQ_OK;
 }
 
@@ -386,7 +389,11 @@ extern "C" int tq_paged_decode(const tq_paged_params* p) {
   a.part = (float*)(a.counters + kMaxCtas);
   a.ctas = num_sms() < kMaxCtas ? num_sms() : kMaxCtas;
   cudaStream_t st = (cudaStream_t)p->stream;
-  if (paged_mma_supported(a, p->dim)) return launch_paged_mma(a, st);
+  if (paged_mma_supported(a, p->dim)) {
+    bool taken = false;
+    rc = launch_paged_mma(a, st, &taken);
+    if (taken) return rc;
+  }
   a.tile_shift = 5;
   a.min_tiles = kWarps;
   a.group_cost = 2;

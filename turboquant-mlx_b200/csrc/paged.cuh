@@ -47,7 +47,7 @@ struct PageView {
 
   __device__ __forceinline__ int capacity() const {
     const int64_t c = (int64_t)table_width << page_shift;
-    return c > 0x7fffffe0 ? 0x7fffffe0 : (int)c;
+    return c > 0x7fff0000 ? 0x7fff0000 : (int)c;         // room for a tile behind the last position
   }
   __device__ __forceinline__ int entry(int b, int pos) const { return __ldg(table + b * table_stride + (pos >> page_shift)); }
   // Pool page of position `pos` of sequence b, -1 when the table names none in the pool.
@@ -388,6 +388,6 @@ __device__ __forceinline__ void join_row(const PagedDecodeArgs& a, int c0, int c
 #endif  // __CUDACC__
 
 bool paged_mma_supported(const PagedDecodeArgs& a, int dim);
-int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st);
+int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st, bool* taken);
 
 }  // namespace tq

@@ -780,10 +780,12 @@ struct ScaledBook {
   float key[16];
   uint16_t c16[16];
   float beta;
+  bool good;             // every centroid within 2^-13 of its value (a codebook with wild levels may have no such factor)
 };
 void scale_book(const float* c, int n, ScaledBook* out) {
   static std::mutex mu;
-  static ScaledBook kept[8];
+  constexpr int kKept = 16;
+  static ScaledBook kept[kKept];
   static int n_kept = 0;
   std::lock_guard<std::mutex> lock(mu);
   for (int i = 0; i < n_kept; ++i)
@@ -804,7 +806,7 @@ void scale_book(const float* c, int n, ScaledBook* out) {
       if (c[i] == 0.f) continue;
       const double exact = (double)beta * (double)c[i];
       const double rel = fabs((double)__half2float(__float2half_rn((float)exact)) - exact) / fabs(exact);
-      if (rel > worst) worst = rel;
+      if (!(rel <= worst)) worst = rel == rel ? rel : 1e30;
     }
     if (worst < best) {
       best = worst;
@@ -812,7 +814,8 @@ void scale_book(const float* c, int n, ScaledBook* out) {
     }
   }
   for (int i = 0; i < n; ++i) sb.c16[i] = __half_as_ushort(__float2half_rn(sb.beta * c[i]));
-  if (n_kept < 8) kept[n_kept++] = sb;
+  sb.good = best <= 1.0 / 8192;
+  if (n_kept < kKept) kept[n_kept++] = sb;
   *out = sb;
 }
 
@@ -866,11 +869,14 @@ bool paged_mma_supported(const PagedDecodeArgs& a, int dim) {
          a.k.norm_page_stride % 4 == 0 && a.k.norm_head_stride % 4 == 0;
 }
 
-int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st) {
+// *taken: whether the kernel takes the call (its codebooks may not fit 16 bits).
+int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st, bool* taken) {
   MmaTables tb;
   memset(&tb, 0, sizeof(tb));
   ScaledBook vb;
   scale_book(a.v.cent.v, 1 << a.v.bits, &vb);
+  *taken = vb.good;
+  if (!*taken) return TQ_OK;
   memcpy(tb.v_c16, vb.c16, sizeof(tb.v_c16));
   tb.v_post = 1.0f / vb.beta;
   tb.k_post = a.scale_log2;
@@ -881,6 +887,8 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st) {
   if (a.k.format == TQ_KV_POLAR) {
     ScaledBook kb;
     scale_book(a.k.cent.v, 1 << a.k.bits, &kb);
+    *taken = kb.good;
+    if (!*taken) return TQ_OK;
     memcpy(tb.k_c16, kb.c16, sizeof(tb.k_c16));
     tb.k_post = a.scale_log2 / ((float)kDim * kb.beta);
   }
