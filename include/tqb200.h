@@ -473,7 +473,8 @@ int tq_copy_pages(void* const* pools, const int64_t* page_bytes, int n_pools, in
                   const int32_t* dst, int64_t n_pairs, void* stream);
 /* What the paged kernels of the current device found wrong since the last call (synchronises the
  * stream; resets the word): 0 nothing, 1 a page id outside the pool, 2 a position behind the
- * page table, 3 a bounded wait that gave up. */
+ * page table, 3 a bounded wait that gave up, 4 a decode kernel whose shared memory does not begin
+ * where it counts on (3 and 4 are faults of the library; outputs are then invalid). */
 int tq_paged_status(int* status, void* stream);
 
 /* Peer-to-peer exchange of a block between the GPUs of one node (sequence-sharded

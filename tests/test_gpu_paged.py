@@ -274,6 +274,49 @@ def test_decode_offsets_beyond_32_bits(tq, dev, stride):
     assert torch.equal(big[2], big[4]) and not bool(big[:2].any())
 
 
+def test_decode_sliced_table(tq, dev):
+    """Rows of a wider table, and one row seen by every sequence."""
+    got, (q, k, v, table, seq, scale) = _decode(tq, dev, lens=[300, 77, 150], n_q=8, n_kv=2)
+    wide = torch.full((3, table.shape[1] + 5), 1 << 30, dtype=torch.int32, device=dev)
+    wide[:, 3:3 + table.shape[1]] = table
+    part = wide[:, 3:3 + table.shape[1]]
+    assert torch.equal(tq.paged_decode(q, k=k.desc, v=v.desc, page_table=part, seq_lens=seq, attn_scale=scale), got)
+    same = table[:1].expand(3, -1)
+    n = torch.tensor([300, 300, 300], dtype=torch.int32, device=dev)
+    out = tq.paged_decode(q, k=k.desc, v=v.desc, page_table=same, seq_lens=n, attn_scale=scale)
+    assert torch.equal(out, tq.paged_decode(q, k=k.desc, v=v.desc, page_table=same.contiguous(), seq_lens=n, attn_scale=scale))
+    assert tq.paged_status(dev) == 0
+
+
+def test_decode_two_streams_at_once(tq, dev):
+    """Split groups of two eager streams in flight together: each stream has its own scratch."""
+    a = _decode(tq, dev, lens=[9000], n_q=8, n_kv=1)
+    b = _decode(tq, dev, lens=[7000, 40], n_q=28, n_kv=4, kbits=0, seed=5)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, (s, (_, (q, k, v, table, seq, scale))) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                outs[i].append(tq.paged_decode(q, k=k.desc, v=v.desc, page_table=table, seq_lens=seq, attn_scale=scale))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, a[0]) for o in outs[0]) and all(torch.equal(o, b[0]) for o in outs[1])
+
+
+def test_copy_pages_in_a_capture(tq, dev):
+    pool = torch.zeros((4, 64), dtype=torch.int32, device=dev)
+    src, dst = (torch.tensor([i], dtype=torch.int32, device=dev) for i in (1, 3))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            tq.copy_pages([pool], [1], [3])
+        tq.copy_pages([pool], src, dst)
+    pool[1] = 7
+    graph.replay()
+    assert torch.equal(pool[3], pool[1]) and not bool(pool[2].any())
+
+
 def test_first_call_inside_a_capture(tq, dev):
     """A process whose first paged call is captured: works or raises, and the next eager call is right (child process)."""
     code = """

@@ -269,3 +269,36 @@ def test_decode_loop_with_window_in_a_graph(tq, dev, hook):
         held = sum(p >= 0 for p in dec.seqs._pages[s])
         assert held <= 6 and dec.seqs.length(s) == 290
     assert torch.equal(got[0], got[1]) and tq.paged_status(dev) == 0
+
+
+def test_step_scratch(tq, dev, hook):
+    """A capture without an eager call in front brings its own scratch; steps do not share theirs; resize ends a step."""
+    scale = 1 / math.sqrt(D)
+    cache, = tq.make_paged_caches(1, 12, 1, page_size=32)
+    seqs = cache.sequences
+    ids = [seqs.add()]
+    seqs.begin(ids, 300)
+    cache.update_and_fetch(*_tokens(1, 1, 300, torch.float16, dev, 0))
+    seqs.begin(ids, 1)
+    keys, values = _tokens(1, 1, 1, torch.float16, dev, 1)
+    q = torch.randn((1, 8, 1, D), generator=torch.Generator().manual_seed(2)).half().to(dev)
+    cache.update_and_fetch(keys, values)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hook.scaled_dot_product_attention(q, keys, values, cache, scale, None)
+    for _ in range(3):
+        graph.replay()
+        eager = hook.scaled_dot_product_attention(q, keys, values, cache, scale, None)
+        assert torch.equal(out, eager)
+    ref, tol = _reference(tq, cache, q[:, :, 0], scale)
+    pr.check(out[:, :, 0], ref, tol)
+    first = seqs._workspace(D)
+    del graph
+    seqs.begin(ids, 1)
+    assert seqs._workspace(D) is not first
+    with pytest.raises(ValueError, match="sink"):
+        hook.scaled_dot_product_attention(q, keys, values, cache, scale, None, sinks=torch.zeros(8, device=dev))
+    seqs.resize(16)
+    with pytest.raises(RuntimeError, match="begin"):
+        cache.update_and_fetch(keys, values)

@@ -9,7 +9,8 @@
 namespace tq {
 
 // One word per device: what a kernel of this file's family found wrong with its inputs since the last
-// tq_paged_status (1: a page id outside the pool, 2: a position behind the page table, 3: a bounded wait gave up).
+// tq_paged_status (1: a page id outside the pool, 2: a position behind the page table, 3: a bounded wait gave up,
+// 4: shared memory does not begin where the tensor-core decode kernel counts on it).
 __device__ int g_paged_status = 0;
 
 int paged_status_ptr(int** out) {

@@ -69,7 +69,8 @@ struct Layout {
   static constexpr uint32_t q_post = up16(info + rings * S * 4);            // 8 floats
   static constexpr uint32_t ml = q_post + 32;                           // m, l of the warps that hand over rows: [2][W][8]
   static constexpr uint32_t flag = ml + 2 * W * 32;
-  static constexpr uint32_t prefix = flag + 16;
+  static constexpr uint32_t ends = flag + 16;                               // both ends of the CTA's run: [2] Cursor
+  static constexpr uint32_t prefix = ends + 2 * sizeof(Cursor);
   static constexpr uint32_t norms = up16(prefix + kPlanInts * 4);   // per warp: key norms, log2 value norms, value norms
   static constexpr uint32_t q = norms + W * 3 * 32 * H * 4;                 // query fragments [k-step][lane][4]
   static constexpr uint32_t small_end = q + 8 * 32 * 16;
@@ -273,8 +274,8 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
   const int cta = blockIdx.x;
   if (plan.total == 0 || cta >= plan.ctas) return;
   const int rg_per_head = a.groups / a.n_kv_heads;
-  // both ends of the run, found by a warp each (the exchange area is free until the first group ends)
-  Cursor* ends = reinterpret_cast<Cursor*>(smem + L::xch - kBase);
+  // both ends of the run, found by a warp each
+  Cursor* ends = reinterpret_cast<Cursor*>(smem + L::ends - kBase);
   if (warp < 2) {
     Cursor c;
     c.seek_run(a, prefix, plan, cta, warp == 1, lane);

@@ -266,6 +266,8 @@ def _page_ids(ids, n_pages: int, what: str, index: int):
         if ids.dtype is not torch.int32 or ids.ndim != 1 or not ids.is_contiguous() or ids.get_device() != index:
             raise ValueError(f"{what} must be a contiguous one-dimensional int32 tensor on cuda:{index}")
         return ids, None
+    if _capturing():
+        raise RuntimeError(f"copy_pages in a captured graph needs {what} as a CUDA tensor")
     host = [int(i) for i in ids]
     bad = [i for i in host if not 0 <= i < n_pages]
     if bad:
@@ -312,7 +314,8 @@ def copy_pages(pools, src, dst) -> None:
 
 def paged_status(device) -> int:
     """What the paged kernels found wrong on this device since the last call (synchronises the current stream): 0
-    nothing, 1 a page id outside the pool, 2 a position behind the page table, 3 a bounded wait that gave up."""
+    nothing, 1 a page id outside the pool, 2 a position behind the page table, 3 a bounded wait that gave up, 4 a
+    decode kernel that found its shared memory elsewhere than it counts on (3 and 4 are faults of the library)."""
     device = torch.device(device)
     word = ctypes.c_int(0)
     with torch.cuda.device(device):

@@ -18,7 +18,7 @@ import torch
 
 from .cache import _Quantizer, _zero
 from .packing import packed_dim
-from .paged import copy_pages, paged_append, paged_decode, paged_dequantize
+from .paged import copy_pages, paged_append, paged_decode, paged_dequantize, paged_workspace_bytes
 
 
 class PagedSequences:
@@ -51,6 +51,7 @@ class PagedSequences:
         self._host_starts: list = []
         self._host_lens: list = []
         self._most = 0
+        self._scratch: dict = {}                            # head_dim -> decode workspace, shared by the layers of the step
 
     # ---- sequences --------------------------------------------------------------------------------------
     def add(self) -> int:
@@ -178,6 +179,7 @@ class PagedSequences:
         self._host_starts = [t[1] for t in todo]
         self._host_lens = [t[1] + t[2] for t in todo]
         self._most = max(counts)
+        self._scratch = {}
         width = max(1, max(len(self._pages[s]) for s in ids))
         rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in ids]
         # one upload: [starts | lens | counts | table]
@@ -187,9 +189,17 @@ class PagedSequences:
         self.starts, self.lens, self.counts = flat[:n], flat[n:2 * n], flat[2 * n:3 * n]
         self.table = flat[3 * n:].view(n, width)
 
+    def _workspace(self, dim: int):
+        """Decode scratch of the step.  A graph captured in one step never shares it with a graph of another; None in a
+        capture without an eager call in front (the call then gets its own)."""
+        if dim not in self._scratch and not torch.cuda.is_current_stream_capturing():
+            self._scratch[dim] = torch.zeros((paged_workspace_bytes(self.device, dim),), dtype=torch.uint8, device=self.device)
+        return self._scratch.get(dim)
+
     def advance_device(self) -> None:
         """One more token per active sequence, on the device only: the body of a captured decode step ends with it.  The
-        pages must have been reserved (`begin(..., reserve=n)`); `advance` tells the host afterwards."""
+        pages must have been reserved (`begin(..., reserve=n)`); `advance` tells the host afterwards.  A captured step
+        belongs to the `begin` in front of it: it reads that step's tables, and the next `begin` ends its use."""
         self.starts += 1
         self.lens += 1
 
@@ -222,9 +232,11 @@ class PagedSequences:
         return len(moved)
 
     def resize(self, n_pages: int) -> None:
-        """Grow or shrink every layer's pools to n_pages; pages that would be cut off must be free."""
+        """Grow or shrink every layer's pools to n_pages; pages that would be cut off must be free.  The pools are new
+        tensors, so the active step ends here (a graph captured in it would go on with the old ones)."""
         if n_pages < 1 or any(self._refs[p] for p in range(n_pages, self.n_pages)):
             raise ValueError(f"pages behind {n_pages} are in use")
+        self._drop_step()
         for layer in self.layers:
             layer._resize(n_pages)
         self._refs = (self._refs + [0] * n_pages)[:n_pages]
@@ -250,7 +262,6 @@ class PagedTurboQuantCache:
         self._v_q = _Quantizer(dim, self.v_bits, seed + 1, dev)
         self._k_q = _Quantizer(dim, self.k_bits, seed, dev) if self.k_bits else None
         self.k, self.v = self._pool(self._k_q), self._pool(self._v_q)
-        self._workspace = None
         sequences.layers.append(self)
 
     def _pool(self, q):
@@ -323,11 +334,8 @@ class PagedTurboQuantCache:
         if B != len(s.active):
             raise ValueError(f"{B} queries, {len(s.active)} active sequences")
         if T == 1:
-            if self._workspace is None:
-                from .paged import paged_workspace_bytes
-                self._workspace = torch.zeros((paged_workspace_bytes(s.device, D),), dtype=torch.uint8, device=s.device)
             out = paged_decode(queries[:, :, 0], k=self.k, v=self.v, page_table=s.table, seq_lens=s.lens, attn_scale=scale,
-                               window=s.window, sinks=s.sinks, workspace=self._workspace)
+                               window=s.window, sinks=s.sinks, workspace=s._workspace(D))
             return out.unsqueeze(2)
         k, v = self.dequantized(queries.dtype)
         out = torch.zeros_like(queries)

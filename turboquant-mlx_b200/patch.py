@@ -30,6 +30,8 @@ def _patched_sdpa(queries, keys, values, cache, scale, mask, sinks=None):
     from .v_only_cache import VOnlyTurboQuantCache
 
     if isinstance(cache, PagedTurboQuantCache):
+        if sinks is not None:
+            raise ValueError("paged attention takes no sink logits (sink tokens are set on the sequences)")
         return cache.attention(queries, scale, mask)
     is_decode = queries.shape[2] == 1
     if isinstance(cache, TurboQuantKVCache) and cache.offset > 0 and cache.fused and not cache.v_only:
