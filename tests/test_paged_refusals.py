@@ -139,3 +139,16 @@ def test_wrappers_refuse_cpu_tensors(tq):
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         tq.copy_pages([x], [0], [0])
     assert tq.copy_pages([], [0], [1]) is None
+
+
+def test_native_calls_report_their_errors(tq):
+    """Errors raised in the extension module arrive as Python exceptions, numbers in their texts included."""
+    calls = tq.paged._load()
+    for name, n in (("decode", 11), ("append", 7), ("dequantize", 6), ("copy_pages", 3)):
+        with pytest.raises(TypeError, match=f"{n} arguments expected, got 1"):
+            getattr(calls, name)(None)
+    with pytest.raises(TypeError, match="must be a tensor"):
+        tq.copy_pages([3], [0], [1])
+    with pytest.raises(TypeError, match="sequence of tensors"):
+        tq.copy_pages(3, [0], [1])
+    assert not tq.copy_pages([], [0], [1])

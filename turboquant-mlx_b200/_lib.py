@@ -129,7 +129,6 @@ class PrefillParams(ctypes.Structure):
     ]
 
 
-PAGED_PARAMS = struct.Struct("=" + _layout(PagedParams))
 PREFILL_PARAMS = struct.Struct("=" + _layout(PrefillParams))
 
 _lib = None
