@@ -4,9 +4,10 @@
 // turboquant_mlx/patch.py:37, on keys / values that update_and_fetch returned
 // in the input dtype, cache.py:100-150).
 //
-// Blackwell-native formulation, one CTA per (128-query tile, query head, batch):
+// Blackwell-native formulation, one persistent CTA per SM over the items (128-query tile, query head, batch):
 //   * Q, K and V tiles arrive by TMA (cp.async.bulk.tensor, 128-byte swizzle)
-//     into shared memory; K / V tiles of 128 keys run through a 2-stage ring.
+//     into shared memory; K tiles of 128 keys run through a ring of three, V tiles through one of two, Q
+//     through one of two, from item to item without a break.
 //   * S = Q K^T and O += P V are tcgen05.mma (cta_group::1, kind::f16, M = N =
 //     128, K = 16 per instruction) issued by one thread.  Three score buffers
 //     and O live in tensor memory (128 lanes x 128 fp32 columns each); P goes
@@ -58,20 +59,22 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 384, kColPinS = 64;
 
 struct Smem {                    // offsets from the 1024-byte aligned base
-  static constexpr uint32_t q = 0;
-  static constexpr uint32_t k0 = q + kTileBytes;                   // K stage s: k0 + s * kTileBytes
+  static constexpr uint32_t q = 0;                                 // Q of work item i: q + (i & 1) * kTileBytes
+  static constexpr uint32_t k0 = q + 2 * kTileBytes;               // K stage s: k0 + s * kTileBytes
   static constexpr uint32_t v0 = k0 + kKStages * kTileBytes;       // V stage s: v0 + s * kTileBytes
-  static constexpr uint32_t mbox = v0 + kVStages * kTileBytes;     // running row maxima [2][128], then final (m, l) [2][2][128]
-  static constexpr uint32_t bars = mbox + 6 * kBM * 4;
-  static constexpr uint32_t tmem_slot = bars + 32 * 8;
+  static constexpr uint32_t mbox = v0 + kVStages * kTileBytes;     // running row maxima [2][128], row sums handed over [2][128]
+  static constexpr uint32_t bars = mbox + 4 * kBM * 4;
+  static constexpr uint32_t tmem_slot = bars + 42 * 8;
   static constexpr uint32_t total = tmem_slot + 16;
 };
-constexpr uint32_t kSmemBytes = Smem::total + 1024;   // slack for the alignment
+constexpr uint32_t kSmemBytes = Smem::total;          // dynamic memory begins at a multiple of 1024 (checked)
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
 
 struct PrefillArgs {
   void* out;
   int64_t o_batch_stride, o_head_stride, o_row_stride;   // elements
   int seq_q, seq_k, n_rep, causal, bf16;
+  int n_heads, heads_batches, items;     // query heads; heads * batch; work items = query tiles * heads * batch
   int window, sinks;             // windowed kernel: row i sees keys > i + off - window and keys < sinks
   float scale_log2;
   int* status;
@@ -117,12 +120,15 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading_by
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((leading_bytes >> 4) & 0x3FFFu) << 16) |
          ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+// The whole warp executes these with the same operands and one elected lane issues: operands that the compiler knows to
+// be uniform go straight to the uniform registers the instruction reads.
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                          uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -130,14 +136,19 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                             uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
@@ -184,6 +195,25 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// two 32-bit floats at once, each rounded like the scalar operation
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
   if (bf16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -194,34 +224,58 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
 }
 
 // Barrier slots (8 bytes each) inside Smem::bars.
-enum : int { B_Q = 0, B_K_FULL = 1, B_K_EMPTY = 4, B_V_FULL = 7, B_V_EMPTY = 9, B_S_FULL = 11, B_P_FULL = 14,
-             B_PV_DONE = 17 /* 2: by tile parity */, B_ALL_DONE = 19, B_MBOX = 20 /* 8: [row group][tile parity] */ };
+enum : int { B_Q_FULL = 0 /* 2 */, B_Q_EMPTY = 2 /* 2 */, B_K_FULL = 4, B_K_EMPTY = 7, B_V_FULL = 10, B_V_EMPTY = 12,
+             B_S_FULL = 14, B_P_FULL = 17, B_PV_DONE = 20 /* 2: by tile parity */, B_ALL_DONE = 22, B_O_FREE = 23,
+             B_MBOX = 24 /* 8: [row group][tile parity] */, B_SUM = 32 /* 8: [row group][exchange parity] */,
+             B_ITEM_DONE = 40 /* 2: by item parity */, B_COUNT = 42 };
 
+// One work item: the 128-query tile of one head, and the key tiles it sees.
+struct Item {
+  int q0, head, batch;
+  int first, sink_tiles, n;      // windowed: tiles 0 .. sink_tiles - 1, then from tile `first` on; n in all
+  __device__ __forceinline__ int key0(int j) const { return (j < sink_tiles ? j : j - sink_tiles + first) * kBN; }
+};
+// The i-th item of this CTA; false behind the last.  Items are numbered by falling cost (latest queries first, then head by
+// head) and dealt out round by round, every other round backwards, so that no CTA gets the longest of every round.
+template <bool WINDOW>
+__device__ __forceinline__ bool item_at(const PrefillArgs& a, int i, Item& it) {
+  const int64_t at = (int64_t)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  if (at >= a.items) return false;
+  const int rank = (int)at / a.heads_batches, rest = (int)at - rank * a.heads_batches;
+  const int off = a.seq_k - a.seq_q;                     // key index of query row 0's diagonal
+  it.q0 = ((a.seq_q + kBM - 1) / kBM - 1 - rank) * kBM;
+  it.batch = rest / a.n_heads;
+  it.head = rest - it.batch * a.n_heads;
+  // keys the item can see: [0, k_end), windowed without those between the sinks and the window of its first row
+  const int k_end = a.causal ? min(a.seq_k, it.q0 + kBM + off) : a.seq_k;
+  it.first = WINDOW ? (int)(max((int64_t)0, (int64_t)it.q0 + off - a.window + 1) / kBN) : 0;
+  it.sink_tiles = WINDOW ? min((min(a.sinks, a.seq_k) + kBN - 1) / kBN, it.first) : 0;
+  it.n = (k_end + kBN - 1) / kBN - it.first + it.sink_tiles;
+  return true;
+}
+
+// Persistent: a CTA takes item after item, and the tiles of all its items form one sequence t = 0, 1, ... through the
+// rings of K, V and score buffers.  The loads and score products of the next item run while this one ends.
 template <bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v, const PrefillArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int q_tile = (int)gridDim.x - 1 - (int)blockIdx.x;     // longest (latest) tiles first
-  const int head = blockIdx.y, batch = blockIdx.z;
-  const int kv_head = head / a.n_rep;
-  const int q0 = q_tile * kBM;
-  const int off = a.seq_k - a.seq_q;                           // key index of query row 0's diagonal
-  // keys this tile can see: [0, k_end)
-  const int k_end = a.causal ? min(a.seq_k, q0 + kBM + off) : a.seq_k;
-  // windowed: tiles of the sinks, then those from the window of the tile's first row on (tile 0 .. first - 1 hidden)
-  const int first = WINDOW ? (int)(max((int64_t)0, (int64_t)q0 + off - a.window + 1) / kBN) : 0;
-  const int sink_tiles = WINDOW ? min((min(a.sinks, a.seq_k) + kBN - 1) / kBN, first) : 0;
-  const int n_tiles = (k_end + kBN - 1) / kBN - first + sink_tiles;
-  auto key0 = [&](int j) { return (!WINDOW || j < sink_tiles ? j : j - sink_tiles + first) * kBN; };   // first key of the j-th tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = smem_u32(smem);
+  if (sbase & 1023u) {           // the launcher has checked that this cannot be
+    if (threadIdx.x == 0) atomicExch(a.status, 20);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);          // uniform, and known to be
   auto bar = [&](int i) { return sbase + Smem::bars + 8u * i; };
   auto wait = [&](uint32_t b, uint32_t parity) { return mbar_wait(b, parity, a.status); };
 
   if (tid == 0) {
-    mbar_init(bar(B_Q), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(B_Q_FULL + i), 1);
+      mbar_init(bar(B_Q_EMPTY + i), 1);
+    }
     for (int s = 0; s < kKStages; ++s) {
       mbar_init(bar(B_K_FULL + s), 1);
       mbar_init(bar(B_K_EMPTY + s), 1);
@@ -237,7 +291,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     mbar_init(bar(B_PV_DONE), 1);
     mbar_init(bar(B_PV_DONE + 1), 1);
     mbar_init(bar(B_ALL_DONE), 1);
+    mbar_init(bar(B_ITEM_DONE), 1);
+    mbar_init(bar(B_ITEM_DONE + 1), 1);
+    mbar_init(bar(B_O_FREE), kGroupThreads);
     for (int i = 0; i < 8; ++i) mbar_init(bar(B_MBOX + i), 32);
+    for (int i = 0; i < 8; ++i) mbar_init(bar(B_SUM + i), 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {   // this warp owns the tensor-memory allocation
@@ -255,282 +313,328 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   if (warp == kProducerWarp) {
     // ------------------------------ TMA producer ------------------------------
     if (lane == 0) {
-      mbar_expect_tx(bar(B_Q), kTileBytes);
-      tma_load_4d(sbase + Smem::q, &map_q, 0, q0, head, batch, bar(B_Q));
-      tma_load_4d(sbase + Smem::q + kHalfBytes, &map_q, 64, q0, head, batch, bar(B_Q));
-      auto load_k = [&](int j) {
-        const int s = j % kKStages;
-        if (j >= kKStages && !wait(bar(B_K_EMPTY + s), ((j / kKStages) - 1) & 1)) return false;
+      int q_loads = 0;
+      // two walks over the sequence of tiles: K (with the items' Q in front), and V
+      Item ki, vi;
+      int k_item = 0, v_item = 0, kj = 0, vj = 0, jk = 0, jv = 0;       // item, tile in the item, tile in the sequence
+      bool k_more = item_at<WINDOW>(a, 0, ki), v_more = item_at<WINDOW>(a, 0, vi);
+      auto load_k = [&]() {
+        if (kj == 0) {
+          const int slot = k_item & 1;
+          if (k_item >= 2 && !wait(bar(B_Q_EMPTY + slot), ((k_item >> 1) - 1) & 1)) return false;
+          const uint32_t dst = sbase + Smem::q + slot * kTileBytes;
+          mbar_expect_tx(bar(B_Q_FULL + slot), kTileBytes);
+          tma_load_4d(dst, &map_q, 0, ki.q0, ki.head, ki.batch, bar(B_Q_FULL + slot));
+          tma_load_4d(dst + kHalfBytes, &map_q, 64, ki.q0, ki.head, ki.batch, bar(B_Q_FULL + slot));
+          ++q_loads;
+        }
+        const int s = jk % kKStages, kv_head = ki.head / a.n_rep;
+        if (jk >= kKStages && !wait(bar(B_K_EMPTY + s), ((jk / kKStages) - 1) & 1)) return false;
         const uint32_t dst = sbase + Smem::k0 + s * kTileBytes;
         mbar_expect_tx(bar(B_K_FULL + s), kTileBytes);
-        tma_load_4d(dst, &map_k, 0, key0(j), kv_head, batch, bar(B_K_FULL + s));
-        tma_load_4d(dst + kHalfBytes, &map_k, 64, key0(j), kv_head, batch, bar(B_K_FULL + s));
+        tma_load_4d(dst, &map_k, 0, ki.key0(kj), kv_head, ki.batch, bar(B_K_FULL + s));
+        tma_load_4d(dst + kHalfBytes, &map_k, 64, ki.key0(kj), kv_head, ki.batch, bar(B_K_FULL + s));
+        ++jk;
+        if (++kj == ki.n) {
+          kj = 0;
+          k_more = item_at<WINDOW>(a, ++k_item, ki);
+        }
         return true;
       };
-      auto load_v = [&](int j) {
-        const int s = j % kVStages;
-        if (j >= kVStages && !wait(bar(B_V_EMPTY + s), ((j / kVStages) - 1) & 1)) return false;
+      auto load_v = [&]() {
+        const int s = jv % kVStages, kv_head = vi.head / a.n_rep;
+        if (jv >= kVStages && !wait(bar(B_V_EMPTY + s), ((jv / kVStages) - 1) & 1)) return false;
         const uint32_t dst = sbase + Smem::v0 + s * kTileBytes;
         mbar_expect_tx(bar(B_V_FULL + s), kTileBytes);
-        tma_load_4d(dst, &map_v, 0, key0(j), kv_head, batch, bar(B_V_FULL + s));
-        tma_load_4d(dst + kHalfBytes, &map_v, 64, key0(j), kv_head, batch, bar(B_V_FULL + s));
+        tma_load_4d(dst, &map_v, 0, vi.key0(vj), kv_head, vi.batch, bar(B_V_FULL + s));
+        tma_load_4d(dst + kHalfBytes, &map_v, 64, vi.key0(vj), kv_head, vi.batch, bar(B_V_FULL + s));
+        ++jv;
+        if (++vj == vi.n) {
+          vj = 0;
+          v_more = item_at<WINDOW>(a, ++v_item, vi);
+        }
         return true;
       };
       // K runs ahead of V: the scores are computed up to three tiles ahead of the softmax
-      int jk = 0, jv = 0;
       bool ok = true;
-      while (ok && (jk < n_tiles || jv < n_tiles)) {
-        if (jk < n_tiles && jk <= jv + 2) {
-          ok = load_k(jk);
-          if (ok) ++jk;
-        } else {
-          ok = load_v(jv);
-          if (ok) ++jv;
-        }
-      }
+      while (ok && (k_more || v_more)) ok = k_more && jk <= jv + 2 ? load_k() : load_v();
       if (!ok) atomicExch(a.status, 11);
       // drain: every copy this thread issued has landed before the CTA may exit
-      mbar_wait(bar(B_Q), 0, nullptr);
+      for (int i = max(0, q_loads - 2); i < q_loads; ++i) mbar_wait(bar(B_Q_FULL + (i & 1)), (i >> 1) & 1, nullptr);
       for (int j = max(0, jk - kKStages); j < jk; ++j) mbar_wait(bar(B_K_FULL + j % kKStages), (j / kKStages) & 1, nullptr);
       for (int j = max(0, jv - kVStages); j < jv; ++j) mbar_wait(bar(B_V_FULL + j % kVStages), (j / kVStages) & 1, nullptr);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------ MMA issuer ------------------------------
-    if (lane == 0) {
+    {
+      auto all_wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, a.status)) != 0; };
       const uint32_t fmt = a.bf16 ? 1u : 0u;
       // D f32, A / B f16 or bf16, M = 128, N = 128; B of the second product is MN-major
       const uint32_t idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kBN >> 3) << 17) |
                                 ((uint32_t)(kBM >> 4) << 24);
       const uint32_t idesc_pv = idesc_qk | (1u << 16);
-      bool ok = wait(bar(B_Q), 0);
-      int fail = ok ? 0 : 12;
+      bool ok = true;
+      int fail = 0;
       // descriptors are built once; inside the loops only the 16-byte-unit address field moves
       uint64_t q_desc[kD / 16];
 #pragma unroll
       for (int kk = 0; kk < kD / 16; ++kk)
         q_desc[kk] = smem_desc(sbase + Smem::q + (kk >> 2) * kHalfBytes + (kk & 3) * 32, 16);
       const uint64_t k_desc0 = smem_desc(sbase + Smem::k0, 16), v_desc0 = smem_desc(sbase + Smem::v0, kHalfBytes);
-      auto issue_qk = [&](int j) {     // S[j % 3] = Q K_j^T
-        const int s = j % kKStages;
-        if (!wait(bar(B_K_FULL + s), (j / kKStages) & 1)) return false;
+      Item qi, pi;                     // of the next score product and of the next value product
+      int q_item = 0, qj = 0, qt = 0;
+      bool q_more = item_at<WINDOW>(a, 0, qi);
+      auto issue_qk = [&]() {          // S[t % 3] = Q K_t^T for the next tile t of the sequence
+        const int s = qt % kKStages;
+        if (qj == 0 && !all_wait(bar(B_Q_FULL + (q_item & 1)), (q_item >> 1) & 1)) {
+          fail = 12;
+          return false;
+        }
+        if (!all_wait(bar(B_K_FULL + s), (qt / kKStages) & 1)) {
+          fail = 13;
+          return false;
+        }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t kd = k_desc0 + (uint64_t)(s * (kTileBytes >> 4));
-        const uint32_t d_tmem = tmem + kColS + (j % kSBufs) * kBN;
+        const uint64_t kd = k_desc0 + (uint64_t)(s * (kTileBytes >> 4)), qo = (uint64_t)((q_item & 1) * (kTileBytes >> 4));
+        const uint32_t d_tmem = tmem + kColS + (qt % kSBufs) * kBN;
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk)
-          umma_f16(d_tmem, q_desc[kk], kd + (uint64_t)(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
+          umma_f16(d_tmem, q_desc[kk] + qo, kd + (uint64_t)(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
         umma_commit(bar(B_K_EMPTY + s));
-        umma_commit(bar(B_S_FULL + j % kSBufs));
+        umma_commit(bar(B_S_FULL + qt % kSBufs));
+        ++qt;
+        if (++qj == qi.n) {
+          umma_commit(bar(B_Q_EMPTY + (q_item & 1)));
+          qj = 0;
+          q_more = item_at<WINDOW>(a, ++q_item, qi);
+        }
         return true;
       };
-      for (int j = 0; j < kSBufs && j < n_tiles && ok; ++j)
-        if (!issue_qk(j)) {
-          ok = false;
-          fail = 13;
-        }
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int s = j % kVStages;
-        if (!wait(bar(B_V_FULL + s), (j / kVStages) & 1) || !wait(bar(B_P_FULL + j % kSBufs), (j / kSBufs) & 1)) {
-          ok = false;
-          fail = 14;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t vd = v_desc0 + (uint64_t)(s * (kTileBytes >> 4));
-        const uint32_t p_tmem = tmem + kColS + (j % kSBufs) * kBN + kColPinS;
+      for (int k = 0; k < kSBufs && q_more && ok; ++k) ok = issue_qk();
+      int t = 0;
+      for (int i = 0; ok && item_at<WINDOW>(a, i, pi); ++i)
+        for (int j = 0; j < pi.n && ok; ++j, ++t) {
+          const int s = t % kVStages;
+          // O is free for the next item once the last one's has been read
+          if (!all_wait(bar(B_V_FULL + s), (t / kVStages) & 1) || !all_wait(bar(B_P_FULL + t % kSBufs), (t / kSBufs) & 1) ||
+              (j == 0 && i > 0 && !all_wait(bar(B_O_FREE), (i - 1) & 1))) {
+            ok = false;
+            fail = 14;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t vd = v_desc0 + (uint64_t)(s * (kTileBytes >> 4));
+          const uint32_t p_tmem = tmem + kColS + (t % kSBufs) * kBN + kColPinS;
 #pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)    // 16 keys = 8 packed columns of P, 2 x 1024 bytes of V
-          umma_f16_ts(tmem_o, p_tmem + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
-                      (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(bar(B_V_EMPTY + s));
-        umma_commit(bar(B_PV_DONE + (j & 1)));
-        // the scores three tiles on go over this tile's buffer: the tensor core runs its work in
-        // issue order, so they follow the product that has just read P from it
-        if (j + kSBufs < n_tiles && !issue_qk(j + kSBufs)) {
-          ok = false;
-          fail = 13;
-          break;
+          for (int kk = 0; kk < kBN / 16; ++kk)    // 16 keys = 8 packed columns of P, 2 x 1024 bytes of V
+            umma_f16_ts(tmem_o, p_tmem + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(bar(B_V_EMPTY + s));
+          umma_commit(bar(B_PV_DONE + (t & 1)));
+          if (j == pi.n - 1) umma_commit(bar(B_ITEM_DONE + (i & 1)));
+          // the scores three tiles on go over this tile's buffer: the tensor core runs its work in
+          // issue order, so they follow the product that has just read P from it
+          if (q_more) ok = issue_qk();
         }
-      }
       umma_commit(bar(B_ALL_DONE));
-      if (fail) atomicExch(a.status, fail);
+      if (fail && lane == 0) atomicExch(a.status, fail);
     }
   } else {
-    // ---------------- softmax: group `who` takes the tiles j = who, who + 2, ...; one row per thread ----------------
+    // ---------------- softmax: group `who` takes the tiles t = who, who + 2, ...; one row per thread ----------------
+    // An item's output is written by the group that has its last tile; the other has handed over its row sums and is at
+    // the next item by then.  At an item's first tile a group still waits for the maximum of the tile in front (and
+    // ignores it), so neither gets more than one tile ahead of what the other has still to read.  Whoever waits for a
+    // phase of a barrier knows the phase in front of it to be over: a parity says no more than that.
     const int who = warp >> 2, rg = warp & 3;
     const int row = rg * 32 + lane;                        // = tensor-memory lane
     const uint32_t lane_base = (uint32_t)(rg * 32) << 16;
     float* mbox = reinterpret_cast<float*>(smem + Smem::mbox);    // [tile parity][row]
-    float* fin = mbox + 2 * kBM;                                  // [m | l][who][row]
-    const int kmax = a.causal ? q0 + row + off : a.seq_k - 1;     // last key this row may see
+    float* sums = mbox + 2 * kBM;                                 // [exchange parity][row]
+    const int off = a.seq_k - a.seq_q;
+    Item it = {};
+    int kmax = 0;                                                 // last key this row may see
     float m_mine = -INFINITY, l_mine = 0.f;                       // l_mine is relative to m_mine
     bool ok = true;
-    // the 64 scores of one half row: load, mask what the row may not see
-    auto load_half = [&](int j, int h, uint32_t (&v)[2][32]) {
-      const uint32_t src = tmem + kColS + (j % kSBufs) * kBN + lane_base + h * 64;
-      tmem_ld32(src, v[0]);
-      tmem_ld32(src + 32, v[1]);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      const int k0 = key0(j);
-      const bool need_mask = (k0 + kBN - 1 > (a.causal ? q0 + off : a.seq_k - 1)) || (k0 + kBN > a.seq_k);
-      if (WINDOW && k0 <= q0 + off + kBM - 1 - a.window && k0 + kBN > a.sinks) {
-        // the window of the tile's last row starts inside or behind this key tile, and not all of it are sinks:
-        // columns in [slim, wlo) are hidden
-        const int slim = a.sinks - (k0 + h * 64), wlo = kmax - a.window + 1 - (k0 + h * 64);
+    // the 128 scores of a row: load, mask what the row may not see
+    auto load_row = [&](int t, int k0, uint32_t (&v)[4][32]) {
+      const uint32_t src = tmem + kColS + (t % kSBufs) * kBN + lane_base;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 4; ++c) tmem_ld32(src + 32 * c, v[c]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      const bool need_mask = (k0 + kBN - 1 > (a.causal ? it.q0 + off : a.seq_k - 1)) || (k0 + kBN > a.seq_k);
+      if (WINDOW && k0 <= it.q0 + off + kBM - 1 - a.window && k0 + kBN > a.sinks) {
+        // the window of the item's last row starts inside or behind this key tile, and not all of it are sinks:
+        // columns in [slim, wlo) are hidden
+        const int slim = a.sinks - k0, wlo = kmax - a.window + 1 - k0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (c * 32 + i >= slim && c * 32 + i < wlo) v[c][i] = 0xff800000u;
       }
       if (need_mask) {
-        const int klim = min(kmax, a.seq_k - 1) - (k0 + h * 64);     // columns <= klim are visible
+        const int klim = min(kmax, a.seq_k - 1) - k0;     // columns <= klim are visible
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (c * 32 + i > klim) v[c][i] = 0xff800000u;   // -inf
       }
     };
-    auto half_max = [&](const uint32_t (&v)[2][32]) {
+    auto row_max = [&](const uint32_t (&v)[4][32]) {
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // four independent chains
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[c][i]));
+        for (int i = 0; i < 32; i += 2)
+          mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
       return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
     };
     // exponentials of a half row -> 32 packed columns of P at `dst`; returns their sum
-    auto half_exp = [&](const uint32_t (&v)[2][32], float neg_m, uint32_t dst) {
+    auto half_exp = [&](const uint32_t (&v0)[32], const uint32_t (&v1)[32], float neg_m, uint32_t dst) {
       uint32_t pk[32];
-      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 scale = make_float2(a.scale_log2, a.scale_log2), shift = make_float2(neg_m, neg_m);
+      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = ex2(fmaf(__uint_as_float(v[c][2 * i]), a.scale_log2, neg_m));
-          const float p1 = ex2(fmaf(__uint_as_float(v[c][2 * i + 1]), a.scale_log2, neg_m));
-          ls[i & 3] += p0 + p1;
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t (&v)[32] = c ? v1 : v0;
+          const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, shift);
+          const float2 y = fma2(make_float2(__uint_as_float(v[2 * i + 2]), __uint_as_float(v[2 * i + 3])), scale, shift);
+          const float p0 = ex2(x.x), p1 = ex2(x.y), p2 = ex2(y.x), p3 = ex2(y.y);
+          ls[(i >> 1) & 1] = add2(ls[(i >> 1) & 1], add2(make_float2(p0, p2), make_float2(p1, p3)));
           pk[c * 16 + i] = pack16(p0, p1, a.bf16);
+          pk[c * 16 + i + 1] = pack16(p2, p3, a.bf16);
         }
       tmem_st32(dst, pk);
-      return (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      return (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
     };
-    for (int j = who; j < n_tiles && ok; j += 2) {
-      if (!__all_sync(0xffffffffu, wait(bar(B_S_FULL + j % kSBufs), (j / kSBufs) & 1))) {   // warp-uniform: aligned tcgen05 ops follow
-        if (lane == 0) atomicExch(a.status, 15);
-        ok = false;
-        break;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      // pass 1: the row maximum (the lower half is read again for its exponentials; the upper half stays)
-      uint32_t sv[2][32];
-      load_half(j, 0, sv);
-      float mraw = half_max(sv);
-      load_half(j, 1, sv);
-      mraw = fmaxf(mraw, half_max(sv));
-      const float mt = mraw * a.scale_log2;              // scale > 0: order preserved
-      // the running maximum after the previous tile comes from the other group
-      if (j > 0) {
-        if (!__all_sync(0xffffffffu, wait(bar(B_MBOX + rg * 2 + ((j - 1) & 1)), ((j - 1) >> 1) & 1))) {
-          if (lane == 0) atomicExch(a.status, 18);
-          ok = false;
-          break;
-        }
-        const float m_prev = mbox[((j - 1) & 1) * kBM + row];
-        if (m_prev != m_mine) {
-          l_mine *= m_mine == -INFINITY ? 0.f : ex2(m_mine - m_prev);
-          m_mine = m_prev;
-        }
-      }
-      // lazy rescale: the reference maximum only moves when a row maximum outgrows it by 2^8
-      const bool grow = mt > m_mine + kRescale;
-      float alpha = 1.f;
-      if (grow) {
-        alpha = m_mine == -INFINITY ? 0.f : ex2(m_mine - mt);
-        m_mine = mt;
-        l_mine *= alpha;
-      }
-      // publish before touching O: the other group only scales its P with it, and its product is
-      // issued after this tile's, which waits for the arrival at the end of this iteration
-      mbox[(j & 1) * kBM + row] = m_mine;
-      mbar_arrive(bar(B_MBOX + rg * 2 + (j & 1)));
-      if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        // O must be complete up to the previous tile before it is rescaled
-        if (!__all_sync(0xffffffffu, wait(bar(B_PV_DONE + ((j - 1) & 1)), ((j - 1) >> 1) & 1))) {
-          if (lane == 0) atomicExch(a.status, 16);
+    int t0 = 0, xi = 0;              // first tile of the item in the sequence; items with an exchange so far
+    for (int i = 0; ok && item_at<WINDOW>(a, i, it); ++i) {
+      kmax = a.causal ? it.q0 + row + off : a.seq_k - 1;
+      m_mine = -INFINITY;
+      l_mine = 0.f;
+      float m_oth = -INFINITY;       // reference of the other group's sum, at the item's last tile
+      for (int j = (who ^ t0) & 1; j < it.n; j += 2) {
+        const int t = t0 + j, k0 = it.key0(j);
+        if (!__all_sync(0xffffffffu, wait(bar(B_S_FULL + t % kSBufs), (t / kSBufs) & 1))) {   // warp-uniform: aligned tcgen05 ops follow
+          if (lane == 0) atomicExch(a.status, 15);
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {      // rare path: kept small in registers
-          uint32_t ov[16];
-          tmem_ld16(tmem_o + lane_base + c * 16, ov);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-          for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-          tmem_st16(tmem_o + lane_base + c * 16, ov);
-        }
-      }
-      if (j == 1) {
-        // start half a period behind group 0, so that one group's exponentials run while the other
-        // loads and reduces scores
-        if (!__all_sync(0xffffffffu, wait(bar(B_P_FULL), 0))) {
-          if (lane == 0) atomicExch(a.status, 19);
-          ok = false;
-          break;
-        }
-      }
-      // pass 2: P over columns 64..127 of the scores (both halves of which are in registers or consumed by now)
-      const float neg_m = m_mine == -INFINITY ? 0.f : -m_mine;
-      const uint32_t p_dst = tmem + kColS + (j % kSBufs) * kBN + lane_base + kColPinS;
-      l_mine += half_exp(sv, neg_m, p_dst + 32);          // keys 64..127 -> packed columns 32..63
-      load_half(j, 0, sv);
-      l_mine += half_exp(sv, neg_m, p_dst);               // keys 0..63 -> packed columns 0..31
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      mbar_arrive(bar(B_P_FULL + j % kSBufs));
-    }
-    if (ok && n_tiles > 0) {
-      if (!__all_sync(0xffffffffu, wait(bar(B_ALL_DONE), 0))) {
-        if (lane == 0) atomicExch(a.status, 17);
-        ok = false;
-      }
-    }
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    // the two groups combine their row sums (each relative to its own last maximum); group 0 writes
-    // output columns 0..63, group 1 columns 64..127
-    fin[who * kBM + row] = m_mine;
-    fin[(2 + who) * kBM + row] = l_mine;
-    asm volatile("bar.sync %0, 64;" ::"r"(1 + rg) : "memory");
-    const float m_oth = fin[(who ^ 1) * kBM + row], l_oth = fin[(2 + (who ^ 1)) * kBM + row];
-    const float m_fin = fmaxf(m_mine, m_oth);
-    const float l_row = (m_mine == -INFINITY ? 0.f : l_mine * ex2(m_mine - m_fin)) +
-                        (m_oth == -INFINITY ? 0.f : l_oth * ex2(m_oth - m_fin));
-    if (ok && n_tiles > 0) {
-      const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
-      const bool live = q0 + row < a.seq_q;
-      uint8_t* orow = reinterpret_cast<uint8_t*>(a.out) + who * 128 +
-                      2 * (batch * a.o_batch_stride + head * a.o_head_stride + (int64_t)(q0 + row) * a.o_row_stride);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t ov[32];
-        tmem_ld32(tmem_o + lane_base + who * 64 + c * 32, ov);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (live) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 w;
-            w.x = pack16(__uint_as_float(ov[8 * i]) * inv, __uint_as_float(ov[8 * i + 1]) * inv, a.bf16);
-            w.y = pack16(__uint_as_float(ov[8 * i + 2]) * inv, __uint_as_float(ov[8 * i + 3]) * inv, a.bf16);
-            w.z = pack16(__uint_as_float(ov[8 * i + 4]) * inv, __uint_as_float(ov[8 * i + 5]) * inv, a.bf16);
-            w.w = pack16(__uint_as_float(ov[8 * i + 6]) * inv, __uint_as_float(ov[8 * i + 7]) * inv, a.bf16);
-            *reinterpret_cast<uint4*>(orow + c * 64 + i * 16) = w;
+        uint32_t sv[4][32];
+        load_row(t, k0, sv);
+        const float mraw = row_max(sv);
+        const float mt = mraw * a.scale_log2;              // scale > 0: order preserved
+        // the running maximum after the previous tile comes from the other group
+        if (t > 0) {
+          if (!__all_sync(0xffffffffu, wait(bar(B_MBOX + rg * 2 + ((t - 1) & 1)), ((t - 1) >> 1) & 1))) {
+            if (lane == 0) atomicExch(a.status, 18);
+            ok = false;
+            break;
+          }
+          if (j > 0) {
+            m_oth = mbox[((t - 1) & 1) * kBM + row];
+            if (m_oth != m_mine) {
+              l_mine *= m_mine == -INFINITY ? 0.f : ex2(m_mine - m_oth);
+              m_mine = m_oth;
+            }
           }
         }
+        // lazy rescale: the reference maximum only moves when a row maximum outgrows it by 2^8
+        const bool grow = mt > m_mine + kRescale;
+        float alpha = 1.f;
+        if (grow) {
+          alpha = m_mine == -INFINITY ? 0.f : ex2(m_mine - mt);
+          m_mine = mt;
+          l_mine *= alpha;
+        }
+        // publish before touching O: the other group only scales its P with it, and its product is
+        // issued after this tile's, which waits for the arrival at the end of this iteration
+        mbox[(t & 1) * kBM + row] = m_mine;
+        mbar_arrive(bar(B_MBOX + rg * 2 + (t & 1)));
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+          // O must be complete up to the previous tile before it is rescaled
+          if (!__all_sync(0xffffffffu, wait(bar(B_PV_DONE + ((t - 1) & 1)), ((t - 1) >> 1) & 1))) {
+            if (lane == 0) atomicExch(a.status, 16);
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {      // rare path: kept small in registers
+            uint32_t ov[16];
+            tmem_ld16(tmem_o + lane_base + c * 16, ov);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < 16; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * alpha);
+            tmem_st16(tmem_o + lane_base + c * 16, ov);
+          }
+        }
+        if (j == 1) {
+          // start half a period behind the other group, so that one group's exponentials run while the other
+          // loads and reduces scores
+          if (!__all_sync(0xffffffffu, wait(bar(B_P_FULL + (t - 1) % kSBufs), ((t - 1) / kSBufs) & 1))) {
+            if (lane == 0) atomicExch(a.status, 19);
+            ok = false;
+            break;
+          }
+        }
+        // P over columns 64..127 of the scores, which are in registers by now
+        const float neg_m = m_mine == -INFINITY ? 0.f : -m_mine;
+        const uint32_t p_dst = tmem + kColS + (t % kSBufs) * kBN + lane_base + kColPinS;
+        l_mine += half_exp(sv[2], sv[3], neg_m, p_dst + 32);          // keys 64..127 -> packed columns 32..63
+        l_mine += half_exp(sv[0], sv[1], neg_m, p_dst);               // keys 0..63 -> packed columns 0..31
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        mbar_arrive(bar(B_P_FULL + t % kSBufs));
+      }
+      const int tl = t0 + it.n - 1, slot = xi & 1, turn = (xi >> 1) & 1;      // the item's last tile
+      t0 += it.n;
+      xi += it.n > 1;
+      if (!ok) break;
+      if ((tl & 1) != who) {
+        if (it.n > 1) {
+          sums[slot * kBM + row] = l_mine;
+          mbar_arrive(bar(B_SUM + rg * 2 + slot));
+        }
+        continue;
+      }
+      if (!__all_sync(0xffffffffu, wait(bar(B_ITEM_DONE + (i & 1)), (i >> 1) & 1) &&
+                                       (it.n == 1 || wait(bar(B_SUM + rg * 2 + slot), turn)))) {
+        if (lane == 0) atomicExch(a.status, 17);
+        ok = false;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const float l_oth = m_oth == -INFINITY ? 0.f : sums[slot * kBM + row] * ex2(m_oth - m_mine);
+      const float l_row = (m_mine == -INFINITY ? 0.f : l_mine) + l_oth;
+      const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
+      uint32_t pk[kD / 2];
+#pragma unroll
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t ov[32];
+        tmem_ld32(tmem_o + lane_base + c * 32, ov);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          pk[c * 16 + k] = pack16(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv, a.bf16);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      mbar_arrive(bar(B_O_FREE));
+      if (it.q0 + row < a.seq_q) {
+        uint8_t* orow = reinterpret_cast<uint8_t*>(a.out) +
+                        2 * (it.batch * a.o_batch_stride + it.head * a.o_head_stride + (int64_t)(it.q0 + row) * a.o_row_stride);
+#pragma unroll
+        for (int k = 0; k < kD / 8; ++k)
+          *reinterpret_cast<uint4*>(orow + k * 16) = make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
       }
     }
+    // nothing of the tensor core's is left when the CTA ends
+    if (!__all_sync(0xffffffffu, wait(bar(B_ALL_DONE), 0)) && lane == 0) atomicExch(a.status, 17);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -637,11 +741,19 @@ static int prefill_sdpa(const void* q, const void* k, const void* v, void* out, 
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err == cudaSuccess && (dev < 0 || dev >= 64 || !ready[windowed][dev])) {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    int reserved = 0;
+    err = cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev);
+    TQ_REQUIRE(err != cudaSuccess || reserved % 1024 == 0, TQ_ERR_LAUNCH, "tq_prefill_sdpa: shared memory begins at %d", reserved);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (err == cudaSuccess && dev >= 0 && dev < 64) ready[windowed][dev] = true;
   }
   if (err != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "tq_prefill_sdpa: %s", cudaGetErrorString(err));
-  const dim3 grid((unsigned)((seq_q + kBM - 1) / kBM), (unsigned)n_q_heads, (unsigned)batch);
+  const int64_t items = (seq_q + kBM - 1) / kBM * n_q_heads * batch;
+  TQ_REQUIRE(items < (1ll << 31), TQ_ERR_BAD_ARG, "tq_prefill_sdpa: too many query tiles");
+  a.n_heads = n_q_heads;
+  a.heads_batches = n_q_heads * batch;
+  a.items = (int)items;
+  const unsigned grid = (unsigned)(items < num_sms() ? items : num_sms());
   kernel<<<grid, kThreads, kSmemBytes, static_cast<cudaStream_t>(stream)>>>(mq, mk, mv, a);
   return check_launch("tq_prefill_sdpa");
 }
