@@ -6,8 +6,8 @@
 //
 // Blackwell-native formulation, one persistent CTA per SM over the items (128-query tile, query head, batch):
 //   * Q, K and V tiles arrive by TMA (cp.async.bulk.tensor, 128-byte swizzle)
-//     into shared memory; K tiles of 128 keys run through a ring of three, V tiles through one of two, Q
-//     through one of two, from item to item without a break.
+//     into shared memory; K tiles of 128 keys run through a ring of three, V tiles through another,
+//     from item to item without a break.
 //   * S = Q K^T and O += P V are tcgen05.mma (cta_group::1, kind::f16, M = N =
 //     128, K = 16 per instruction) issued by one thread.  Three score buffers
 //     and O live in tensor memory (128 lanes x 128 fp32 columns each); P goes
@@ -42,12 +42,12 @@ constexpr int kD = 128;          // head_dim
 constexpr int kBM = 128;         // queries per CTA
 constexpr int kBN = 128;         // keys per tile
 constexpr int kKStages = 3;      // K tiles run three ahead of the softmax
-constexpr int kVStages = 2;
+constexpr int kVStages = 3;
 constexpr int kSBufs = 3;        // score buffers in tensor memory: tile j uses buffer j % 3
 constexpr int kGroupThreads = 128;               // one softmax group: one thread per query row
 constexpr int kSoftmaxThreads = 2 * kGroupThreads;
-constexpr int kThreads = kSoftmaxThreads + 64;   // + TMA warp + MMA warp
-constexpr int kProducerWarp = kSoftmaxThreads / 32, kMmaWarp = kProducerWarp + 1;
+constexpr int kThreads = kSoftmaxThreads + 96;   // + TMA warps (Q and K; V) + MMA warp
+constexpr int kKWarp = kSoftmaxThreads / 32, kVWarp = kKWarp + 1, kMmaWarp = kKWarp + 2;
 constexpr uint32_t kTileBytes = kBM * kD * 2;    // 32 KiB: one 128 x 128 16-bit tile
 constexpr uint32_t kHalfBytes = kTileBytes / 2;  // one 128-row x 64-element swizzle block
 constexpr uint32_t kSpin = 1u << 20;
@@ -59,12 +59,12 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 384, kColPinS = 64;
 
 struct Smem {                    // offsets from the 1024-byte aligned base
-  static constexpr uint32_t q = 0;                                 // Q of work item i: q + (i & 1) * kTileBytes
-  static constexpr uint32_t k0 = q + 2 * kTileBytes;               // K stage s: k0 + s * kTileBytes
+  static constexpr uint32_t q = 0;
+  static constexpr uint32_t k0 = q + kTileBytes;                   // K stage s: k0 + s * kTileBytes
   static constexpr uint32_t v0 = k0 + kKStages * kTileBytes;       // V stage s: v0 + s * kTileBytes
   static constexpr uint32_t mbox = v0 + kVStages * kTileBytes;     // running row maxima [2][128], row sums handed over [2][128]
   static constexpr uint32_t bars = mbox + 4 * kBM * 4;
-  static constexpr uint32_t tmem_slot = bars + 42 * 8;
+  static constexpr uint32_t tmem_slot = bars + 42 * 8;           // B_COUNT barriers
   static constexpr uint32_t total = tmem_slot + 16;
 };
 constexpr uint32_t kSmemBytes = Smem::total;          // dynamic memory begins at a multiple of 1024 (checked)
@@ -73,7 +73,7 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
 struct PrefillArgs {
   void* out;
   int64_t o_batch_stride, o_head_stride, o_row_stride;   // elements
-  int seq_q, seq_k, n_rep, causal, bf16;
+  int seq_q, seq_k, n_rep, causal;
   int n_heads, heads_batches, items;     // query heads; heads * batch; work items = query tiles * heads * batch
   int window, sinks;             // windowed kernel: row i sees keys > i + off - window and keys < sinks
   float scale_log2;
@@ -214,8 +214,9 @@ __device__ __forceinline__ float2 add2(float2 x, float2 y) {
       : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return r;
 }
-__device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
-  if (bf16) {
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if (BF) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
@@ -224,8 +225,8 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
 }
 
 // Barrier slots (8 bytes each) inside Smem::bars.
-enum : int { B_Q_FULL = 0 /* 2 */, B_Q_EMPTY = 2 /* 2 */, B_K_FULL = 4, B_K_EMPTY = 7, B_V_FULL = 10, B_V_EMPTY = 12,
-             B_S_FULL = 14, B_P_FULL = 17, B_PV_DONE = 20 /* 2: by tile parity */, B_ALL_DONE = 22, B_O_FREE = 23,
+enum : int { B_Q_FULL = 0, B_Q_EMPTY = 1, B_K_FULL = 2, B_K_EMPTY = 5, B_V_FULL = 8, B_V_EMPTY = 11, B_S_FULL = 14,
+             B_P_FULL = 17, B_PV_DONE = 20 /* 2: by tile parity */, B_ALL_DONE = 22, B_O_FREE = 23,
              B_MBOX = 24 /* 8: [row group][tile parity] */, B_SUM = 32 /* 8: [row group][exchange parity] */,
              B_ITEM_DONE = 40 /* 2: by item parity */, B_COUNT = 42 };
 
@@ -256,7 +257,7 @@ __device__ __forceinline__ bool item_at(const PrefillArgs& a, int i, Item& it) {
 
 // Persistent: a CTA takes item after item, and the tiles of all its items form one sequence t = 0, 1, ... through the
 // rings of K, V and score buffers.  The loads and score products of the next item run while this one ends.
-template <bool WINDOW>
+template <bool WINDOW, bool BF>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v, const PrefillArgs a) {
@@ -272,10 +273,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   auto wait = [&](uint32_t b, uint32_t parity) { return mbar_wait(b, parity, a.status); };
 
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(B_Q_FULL + i), 1);
-      mbar_init(bar(B_Q_EMPTY + i), 1);
-    }
+    mbar_init(bar(B_Q_FULL), 1);
+    mbar_init(bar(B_Q_EMPTY), 1);
     for (int s = 0; s < kKStages; ++s) {
       mbar_init(bar(B_K_FULL + s), 1);
       mbar_init(bar(B_K_EMPTY + s), 1);
@@ -310,65 +309,64 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Smem::tmem_slot);
   const uint32_t tmem_o = tmem + kColO;
 
-  if (warp == kProducerWarp) {
-    // ------------------------------ TMA producer ------------------------------
+  if (warp == kKWarp) {
+    // ------------------------------ TMA producer of Q and K ------------------------------
     if (lane == 0) {
-      int q_loads = 0;
-      // two walks over the sequence of tiles: K (with the items' Q in front), and V
-      Item ki, vi;
-      int k_item = 0, v_item = 0, kj = 0, vj = 0, jk = 0, jv = 0;       // item, tile in the item, tile in the sequence
-      bool k_more = item_at<WINDOW>(a, 0, ki), v_more = item_at<WINDOW>(a, 0, vi);
-      auto load_k = [&]() {
-        if (kj == 0) {
-          const int slot = k_item & 1;
-          if (k_item >= 2 && !wait(bar(B_Q_EMPTY + slot), ((k_item >> 1) - 1) & 1)) return false;
-          const uint32_t dst = sbase + Smem::q + slot * kTileBytes;
-          mbar_expect_tx(bar(B_Q_FULL + slot), kTileBytes);
-          tma_load_4d(dst, &map_q, 0, ki.q0, ki.head, ki.batch, bar(B_Q_FULL + slot));
-          tma_load_4d(dst + kHalfBytes, &map_q, 64, ki.q0, ki.head, ki.batch, bar(B_Q_FULL + slot));
-          ++q_loads;
-        }
-        const int s = jk % kKStages, kv_head = ki.head / a.n_rep;
-        if (jk >= kKStages && !wait(bar(B_K_EMPTY + s), ((jk / kKStages) - 1) & 1)) return false;
-        const uint32_t dst = sbase + Smem::k0 + s * kTileBytes;
-        mbar_expect_tx(bar(B_K_FULL + s), kTileBytes);
-        tma_load_4d(dst, &map_k, 0, ki.key0(kj), kv_head, ki.batch, bar(B_K_FULL + s));
-        tma_load_4d(dst + kHalfBytes, &map_k, 64, ki.key0(kj), kv_head, ki.batch, bar(B_K_FULL + s));
-        ++jk;
-        if (++kj == ki.n) {
-          kj = 0;
-          k_more = item_at<WINDOW>(a, ++k_item, ki);
-        }
-        return true;
-      };
-      auto load_v = [&]() {
-        const int s = jv % kVStages, kv_head = vi.head / a.n_rep;
-        if (jv >= kVStages && !wait(bar(B_V_EMPTY + s), ((jv / kVStages) - 1) & 1)) return false;
-        const uint32_t dst = sbase + Smem::v0 + s * kTileBytes;
-        mbar_expect_tx(bar(B_V_FULL + s), kTileBytes);
-        tma_load_4d(dst, &map_v, 0, vi.key0(vj), kv_head, vi.batch, bar(B_V_FULL + s));
-        tma_load_4d(dst + kHalfBytes, &map_v, 64, vi.key0(vj), kv_head, vi.batch, bar(B_V_FULL + s));
-        ++jv;
-        if (++vj == vi.n) {
-          vj = 0;
-          v_more = item_at<WINDOW>(a, ++v_item, vi);
-        }
-        return true;
-      };
-      // K runs ahead of V: the scores are computed up to three tiles ahead of the softmax
+      int items = 0, t = 0;            // loads issued: items' Q, tiles
       bool ok = true;
-      while (ok && (k_more || v_more)) ok = k_more && jk <= jv + 2 ? load_k() : load_v();
-      if (!ok) atomicExch(a.status, 11);
+      Item it;
+      for (; ok && item_at<WINDOW>(a, items, it); ) {
+        if (items > 0 && !wait(bar(B_Q_EMPTY), (items - 1) & 1)) break;
+        mbar_expect_tx(bar(B_Q_FULL), kTileBytes);
+        tma_load_4d(sbase + Smem::q, &map_q, 0, it.q0, it.head, it.batch, bar(B_Q_FULL));
+        tma_load_4d(sbase + Smem::q + kHalfBytes, &map_q, 64, it.q0, it.head, it.batch, bar(B_Q_FULL));
+        ++items;
+        const int kv_head = it.head / a.n_rep;
+        for (int j = 0; j < it.n; ++j, ++t) {
+          const int s = t % kKStages;
+          if (t >= kKStages && !wait(bar(B_K_EMPTY + s), ((t / kKStages) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = sbase + Smem::k0 + s * kTileBytes;
+          mbar_expect_tx(bar(B_K_FULL + s), kTileBytes);
+          tma_load_4d(dst, &map_k, 0, it.key0(j), kv_head, it.batch, bar(B_K_FULL + s));
+          tma_load_4d(dst + kHalfBytes, &map_k, 64, it.key0(j), kv_head, it.batch, bar(B_K_FULL + s));
+        }
+      }
+      if (!ok || item_at<WINDOW>(a, items, it)) atomicExch(a.status, 11);
       // drain: every copy this thread issued has landed before the CTA may exit
-      for (int i = max(0, q_loads - 2); i < q_loads; ++i) mbar_wait(bar(B_Q_FULL + (i & 1)), (i >> 1) & 1, nullptr);
-      for (int j = max(0, jk - kKStages); j < jk; ++j) mbar_wait(bar(B_K_FULL + j % kKStages), (j / kKStages) & 1, nullptr);
-      for (int j = max(0, jv - kVStages); j < jv; ++j) mbar_wait(bar(B_V_FULL + j % kVStages), (j / kVStages) & 1, nullptr);
+      if (items > 0) mbar_wait(bar(B_Q_FULL), (items - 1) & 1, nullptr);
+      for (int j = max(0, t - kKStages); j < t; ++j) mbar_wait(bar(B_K_FULL + j % kKStages), (j / kKStages) & 1, nullptr);
+    }
+  } else if (warp == kVWarp) {
+    // ------------------------------ TMA producer of V ------------------------------
+    if (lane == 0) {
+      int t = 0;
+      bool ok = true;
+      Item it;
+      for (int i = 0; ok && item_at<WINDOW>(a, i, it); ++i) {
+        const int kv_head = it.head / a.n_rep;
+        for (int j = 0; j < it.n; ++j, ++t) {
+          const int s = t % kVStages;
+          if (t >= kVStages && !wait(bar(B_V_EMPTY + s), ((t / kVStages) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = sbase + Smem::v0 + s * kTileBytes;
+          mbar_expect_tx(bar(B_V_FULL + s), kTileBytes);
+          tma_load_4d(dst, &map_v, 0, it.key0(j), kv_head, it.batch, bar(B_V_FULL + s));
+          tma_load_4d(dst + kHalfBytes, &map_v, 64, it.key0(j), kv_head, it.batch, bar(B_V_FULL + s));
+        }
+      }
+      if (!ok) atomicExch(a.status, 11);
+      for (int j = max(0, t - kVStages); j < t; ++j) mbar_wait(bar(B_V_FULL + j % kVStages), (j / kVStages) & 1, nullptr);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------ MMA issuer ------------------------------
     {
       auto all_wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, a.status)) != 0; };
-      const uint32_t fmt = a.bf16 ? 1u : 0u;
+      const uint32_t fmt = BF ? 1u : 0u;
       // D f32, A / B f16 or bf16, M = 128, N = 128; B of the second product is MN-major
       const uint32_t idesc_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kBN >> 3) << 17) |
                                 ((uint32_t)(kBM >> 4) << 24);
@@ -386,7 +384,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       bool q_more = item_at<WINDOW>(a, 0, qi);
       auto issue_qk = [&]() {          // S[t % 3] = Q K_t^T for the next tile t of the sequence
         const int s = qt % kKStages;
-        if (qj == 0 && !all_wait(bar(B_Q_FULL + (q_item & 1)), (q_item >> 1) & 1)) {
+        if (qj == 0 && !all_wait(bar(B_Q_FULL), q_item & 1)) {
           fail = 12;
           return false;
         }
@@ -395,16 +393,16 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           return false;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t kd = k_desc0 + (uint64_t)(s * (kTileBytes >> 4)), qo = (uint64_t)((q_item & 1) * (kTileBytes >> 4));
+        const uint64_t kd = k_desc0 + (uint64_t)(s * (kTileBytes >> 4));
         const uint32_t d_tmem = tmem + kColS + (qt % kSBufs) * kBN;
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk)
-          umma_f16(d_tmem, q_desc[kk] + qo, kd + (uint64_t)(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
+          umma_f16(d_tmem, q_desc[kk], kd + (uint64_t)(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
         umma_commit(bar(B_K_EMPTY + s));
         umma_commit(bar(B_S_FULL + qt % kSBufs));
         ++qt;
         if (++qj == qi.n) {
-          umma_commit(bar(B_Q_EMPTY + (q_item & 1)));
+          umma_commit(bar(B_Q_EMPTY));
           qj = 0;
           q_more = item_at<WINDOW>(a, ++q_item, qi);
         }
@@ -504,8 +502,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           const float2 y = fma2(make_float2(__uint_as_float(v[2 * i + 2]), __uint_as_float(v[2 * i + 3])), scale, shift);
           const float p0 = ex2(x.x), p1 = ex2(x.y), p2 = ex2(y.x), p3 = ex2(y.y);
           ls[(i >> 1) & 1] = add2(ls[(i >> 1) & 1], add2(make_float2(p0, p2), make_float2(p1, p3)));
-          pk[c * 16 + i] = pack16(p0, p1, a.bf16);
-          pk[c * 16 + i + 1] = pack16(p2, p3, a.bf16);
+          pk[c * 16 + i] = pack16<BF>(p0, p1);
+          pk[c * 16 + i + 1] = pack16<BF>(p2, p3);
         }
       tmem_st32(dst, pk);
       return (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
@@ -573,15 +571,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             tmem_st16(tmem_o + lane_base + c * 16, ov);
           }
         }
-        if (j == 1) {
-          // start half a period behind the other group, so that one group's exponentials run while the other
-          // loads and reduces scores
-          if (!__all_sync(0xffffffffu, wait(bar(B_P_FULL + (t - 1) % kSBufs), ((t - 1) / kSBufs) & 1))) {
-            if (lane == 0) atomicExch(a.status, 19);
-            ok = false;
-            break;
-          }
-        }
         // P over columns 64..127 of the scores, which are in registers by now
         const float neg_m = m_mine == -INFINITY ? 0.f : -m_mine;
         const uint32_t p_dst = tmem + kColS + (t % kSBufs) * kBN + lane_base + kColPinS;
@@ -620,7 +609,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          pk[c * 16 + k] = pack16(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv, a.bf16);
+          pk[c * 16 + k] = pack16<BF>(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       mbar_arrive(bar(B_O_FREE));
@@ -729,23 +718,24 @@ static int prefill_sdpa(const void* q, const void* k, const void* v, void* out, 
   a.seq_k = (int)seq_k;
   a.n_rep = n_q_heads / n_kv_heads;
   a.causal = causal ? 1 : 0;
-  a.bf16 = bf16;
   a.scale_log2 = attn_scale * kLog2e;
   a.status = status;
   // a window that reaches the first key from every row hides nothing: the full form
   const bool windowed = window > 0 && window < seq_k;
   a.window = windowed ? (int)window : 0;
   a.sinks = windowed ? (int)(sinks < seq_k ? sinks : seq_k) : 0;
-  auto kernel = windowed ? prefill_kernel<true> : prefill_kernel<false>;
-  static bool ready[2][64] = {{false}};        // per device: the attribute belongs to the device's context
+  auto kernel = windowed ? (bf16 ? prefill_kernel<true, true> : prefill_kernel<true, false>)
+                         : (bf16 ? prefill_kernel<false, true> : prefill_kernel<false, false>);
+  static bool ready_of[2][2][64] = {};         // per device: the attribute belongs to the device's context
+  bool (&ready)[64] = ready_of[windowed][bf16];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess && (dev < 0 || dev >= 64 || !ready[windowed][dev])) {
+  if (err == cudaSuccess && (dev < 0 || dev >= 64 || !ready[dev])) {
     int reserved = 0;
     err = cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev);
     TQ_REQUIRE(err != cudaSuccess || reserved % 1024 == 0, TQ_ERR_LAUNCH, "tq_prefill_sdpa: shared memory begins at %d", reserved);
     if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
-    if (err == cudaSuccess && dev >= 0 && dev < 64) ready[windowed][dev] = true;
+    if (err == cudaSuccess && dev >= 0 && dev < 64) ready[dev] = true;
   }
   if (err != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "tq_prefill_sdpa: %s", cudaGetErrorString(err));
   const int64_t items = (seq_q + kBM - 1) / kBM * n_q_heads * batch;
