@@ -609,3 +609,51 @@ def test_prompt_window_equals_full_form_when_wide(tq, dev):
     q, k, v = [torch.randn((1, h, 300, 128), device=dev, dtype=torch.float16) for h in (4, 2, 2)]
     full = tq.prefill_attention(q, k, v, 0.1)
     assert torch.equal(tq.prefill_attention(q, k, v, 0.1, window=300, sinks=2), full)
+
+
+@pytest.mark.parametrize("L,S,causal,window,sinks", [
+    (64, 64, True, 0, 0), (64, 64, True, 20, 3), (130, 130, True, 0, 0), (130, 300, True, 100, 5), (200, 700, True, 300, 1),
+    (513, 513, True, 0, 0), (513, 513, True, 140, 200), (90, 100, False, 0, 0), (150, 260, False, 0, 0)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_many_items(tq, dev, L, S, causal, window, sinks, dtype):
+    """Several work items per SM, of one key tile and more, with scores large enough for the accumulators to be rescaled."""
+    B, n_q, n_kv, D, gain = 11, 32, 8, 128, 4.0
+    g = torch.Generator(device="cuda").manual_seed(L + S)
+    q, k, v = [torch.randn((B, h, n, D), generator=g, device=dev).to(dtype) for h, n in ((n_q, L), (n_kv, S), (n_kv, S))]
+    q = q * gain
+    scale = 1 / math.sqrt(D)
+    got = tq.prefill_attention(q, k, v, scale, causal=causal, window=window, sinks=sinks)
+    again = tq.prefill_attention(q, k, v, scale, causal=causal, window=window, sinks=sinks)
+    assert tq.kernels.prefill_status(dev) == 0 and torch.equal(got, again)
+    half = torch.finfo(dtype).eps / 2
+    i, j = torch.arange(L, device=dev)[:, None] + S - L, torch.arange(S, device=dev)
+    seen = torch.ones((L, S), dtype=torch.bool, device=dev) if not causal else j <= i
+    if window:
+        seen &= (j > i - window) | (j < sinks)
+    for b in range(B):                 # the tolerance of test_prompt_window
+        qd, kd, vd = [t[b].double() for t in (q, k.repeat_interleave(n_q // n_kv, 1), v.repeat_interleave(n_q // n_kv, 1))]
+        s = qd @ kd.transpose(-1, -2) * scale
+        mag = qd.abs() @ kd.abs().transpose(-1, -2) * scale
+        p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        ref = p @ vd
+        d = ((D + 8) * 2.0 ** -24 * mag).masked_fill(~seen, 0).amax(-1, keepdim=True) + \
+            4 * 2.0 ** -24 * s.abs().masked_fill(~seen, 0).amax(-1, keepdim=True) + 2.0 ** -22
+        reach = p @ vd.abs()
+        rel = 2 * d + half + S * 2.0 ** -24
+        pr.check(got[b], ref.cpu(), (rel * reach + half * (ref.abs() + rel * reach) + 1e-12).cpu(), f"batch {b}")
+
+
+def test_prompt_out_is_checked(tq, dev):
+    q, k, v = [torch.randn((1, h, 40, 128), device=dev, dtype=torch.float16) for h in (4, 2, 2)]
+    want = tq.prefill_attention(q, k, v, 0.1, window=16)
+    out = torch.empty((1, 40, 4, 128), device=dev, dtype=torch.float16).transpose(1, 2)
+    assert tq.prefill_attention(q, k, v, 0.1, window=16, out=out) is not None and torch.equal(out, want)
+    for bad in (out.float(), out[:, :3], out.cpu(), torch.empty((1, 4, 40, 129), device=dev, dtype=torch.float16)[..., :128]):
+        with pytest.raises(ValueError):
+            tq.prefill_attention(q, k, v, 0.1, window=16, out=bad)
+    with pytest.raises(ValueError):
+        tq.prefill_attention(q, k, v[:, :, :39], 0.1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tq.prefill_attention(q, k.cpu(), v, 0.1)
+    odd = torch.randn((1 * 2 * 40 * 128 + 1,), device=dev).half()[1:].view(1, 2, 40, 128)        # not 16-byte aligned
+    assert torch.equal(tq.prefill_attention(q, odd, v, 0.1, window=16), tq.prefill_attention(q, odd.clone(), v, 0.1, window=16))

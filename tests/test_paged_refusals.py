@@ -143,8 +143,8 @@ def test_wrappers_refuse_cpu_tensors(tq):
 
 def test_native_calls_report_their_errors(tq):
     """Errors raised in the extension module arrive as Python exceptions, numbers in their texts included."""
-    calls = tq.paged._load()
-    for name, n in (("decode", 11), ("append", 7), ("dequantize", 6), ("copy_pages", 3)):
+    calls = tq._lib.load_native()
+    for name, n in (("decode", 11), ("append", 7), ("dequantize", 6), ("copy_pages", 3), ("prefill", 9)):
         with pytest.raises(TypeError, match=f"{n} arguments expected, got 1"):
             getattr(calls, name)(None)
     with pytest.raises(TypeError, match="must be a tensor"):

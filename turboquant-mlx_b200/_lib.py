@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 import weakref
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
@@ -72,19 +71,6 @@ class FlashParams(ctypes.Structure):
     ]
 
 
-def _layout(cls, prefix=""):
-    """struct-module format of a ctypes structure (native sizes, no implicit padding: the fields are checked to be
-    packed), so that a whole argument block is filled by one call."""
-    codes = {c_int32: "i", c_int64: "q", c_void_p: "Q", c_float: "f", POINTER(c_float): "Q", c_int64 * 3: "3q"}
-    out, at = "", 0
-    for name, kind in cls._fields_:
-        assert getattr(cls, name).offset == at, f"{cls.__name__}.{name} is not packed"
-        at += ctypes.sizeof(kind)
-        out += _layout(kind) if issubclass(kind, ctypes.Structure) else codes[kind]
-    assert at == ctypes.sizeof(cls)
-    return out
-
-
 class PagedHalf(ctypes.Structure):
     """Mirror of `tq_paged_half` (include/tqb200.h)."""
 
@@ -128,8 +114,6 @@ class PrefillParams(ctypes.Structure):
         ("status", c_void_p), ("stream", c_void_p),
     ]
 
-
-PREFILL_PARAMS = struct.Struct("=" + _layout(PrefillParams))
 
 _lib = None
 
@@ -210,6 +194,23 @@ def lib() -> ctypes.CDLL:
 
 def exported_symbols():
     return sorted(_SIGNATURES)
+
+
+native = None            # the extension module that makes the calls whose host time counts (csrc/calls.cpp)
+
+
+def load_native():
+    """Load it (once), bound to the loaded libtqb200.so."""
+    global native
+    try:
+        from . import _calls
+    except ImportError as e:
+        raise RuntimeError("_calls.so is missing or does not fit this torch: run make in the package folder") from e
+    import sys
+    _calls.bind(sys.modules[__name__], *[ctypes.cast(getattr(lib(), "tq_" + name), c_void_p).value for name in (
+        "paged_decode", "paged_append", "paged_dequantize", "paged_decode_workspace_bytes", "copy_pages", "prefill_sdpa_window")])
+    native = _calls
+    return native
 
 
 def check(status: int) -> None:

@@ -1,8 +1,8 @@
-// The paged caches' calls from Python: argument checks and argument blocks (include/tqb200.h) without the interpreter.
+// The calls of the paged caches and of prompt attention from Python: argument checks and argument blocks (include/tqb200.h) without the interpreter.
 // A decode step's kernels take 2 to 20 us, so the host's share of a call counts when it is not replayed from a CUDA
 // graph: the same checks written in Python took 11 us of the 17 us of a single-token decode call, here about 1.
 //
-// Module _calls; `paged.py` holds the signatures and their documentation.  The entry points come in by address
+// Module _calls; `paged.py` and `kernels.py` hold the signatures and their documentation.  The entry points come in by address
 // (bind), so that whichever libtqb200.so the package has loaded is the one that is called.
 #include <Python.h>
 
@@ -28,6 +28,7 @@ struct Entry {
   int (*dequantize)(const tq_paged_params*);
   int64_t (*workspace_bytes)(int);
   int (*copy)(void* const*, const int64_t*, int, int64_t, const int32_t*, const int32_t*, int64_t, void*);
+  int (*prefill)(const tq_prefill_params*);
 } entry;
 PyObject *host_floats, *host_cache, *check_status;      // of the package's _lib (borrowed for good)
 
@@ -474,12 +475,85 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(lib, decode, append, dequantize, workspace_bytes, copy): the package's _lib module and the entry points' addresses
+// (queries, keys, values, scale, causal, out, window, sinks, status) -> out
+PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  arguments(nargs, 9);
+  at::Tensor x[3] = {tensor(args[0], "queries"), tensor(args[1], "keys"), tensor(args[2], "values")};
+  for (const at::Tensor& t : x) require_cuda(t);
+  const int index = (int)x[0].get_device();
+  TORCH_CHECK_VALUE(x[0].scalar_type() == at::kHalf || x[0].scalar_type() == at::kBFloat16,
+                    "prefill_attention takes float16 or bfloat16 tensors");
+  TORCH_CHECK_VALUE(x[1].scalar_type() == x[0].scalar_type() && x[2].scalar_type() == x[0].scalar_type(),
+                    "queries, keys and values must share one dtype");
+  TORCH_CHECK_VALUE(x[0].dim() == 4 && x[1].dim() == 4 && x[2].dim() == 4, "queries, keys and values must be (batch, heads, length, 128)");
+  const int64_t B = x[0].size(0), n_q = x[0].size(1), L = x[0].size(2), D = x[0].size(3), n_kv = x[1].size(1), S = x[1].size(2);
+  TORCH_CHECK_VALUE(D == 128 && x[1].size(3) == 128 && x[2].size(3) == 128, "prefill_attention supports head_dim 128, got ", D);
+  TORCH_CHECK_VALUE(n_kv > 0 && n_q % n_kv == 0, "n_q_heads (", n_q, ") must equal n_kv_heads (", n_kv, ") * n_rep (",
+                    n_q / std::max<int64_t>(n_kv, 1), ")");
+  TORCH_CHECK_VALUE(x[1].size(0) == B && x[2].sizes() == x[1].sizes(), "keys and values must have the same (batch, heads, length)");
+  TORCH_CHECK_VALUE(index_of(x[1]) == index && index_of(x[2]) == index, "queries, keys and values must be on one device");
+  TORCH_CHECK_VALUE(std::max(B, n_q) <= INT32_MAX, "too many heads");
+  const int causal = PyObject_IsTrue(args[4]);
+  if (causal < 0) raise_python();
+  const double scale = PyFloat_AsDouble(args[3]);
+  if (scale == -1.0 && PyErr_Occurred()) raise_python();
+  const int64_t window = integer(args[6]), sinks = integer(args[7]);
+  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0) && (window == 0 || causal), "window (", window,
+                    ") and sinks (", sinks, ") must not be negative, sinks need a window, and a window needs causal attention");
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)index);
+  auto usable = [](const at::Tensor& t) {
+    return t.stride(3) == 1 && ((t.stride(0) | t.stride(1) | t.stride(2)) & 7) == 0 && ((uintptr_t)t.data_ptr() & 15) == 0;
+  };
+  for (at::Tensor& t : x)
+    if (!usable(t)) t = t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
+  at::Tensor out;
+  if (args[5] == Py_None) {
+    out = at::empty({B, n_q, L, D}, x[0].options());
+  } else {
+    out = tensor(args[5], "out");
+    TORCH_CHECK_VALUE(out.sizes() == x[0].sizes() && out.scalar_type() == x[0].scalar_type() && index_of(out) == index && usable(out),
+                      "out must be ", x[0].sizes(), " of the inputs' dtype on cuda:", index,
+                      ", 16-byte aligned, with a contiguous last dimension");
+  }
+  const at::Tensor& status = tensor(args[8], "status");
+  tq_prefill_params p;
+  memset(&p, 0, sizeof(p));
+  p.struct_bytes = (int32_t)sizeof(p);
+  p.dtype = dtype_code(x[0].scalar_type());
+  p.batch = (int32_t)B;
+  p.n_q_heads = (int32_t)n_q;
+  p.n_kv_heads = (int32_t)n_kv;
+  p.dim = (int32_t)D;
+  p.seq_q = L;
+  p.seq_k = S;
+  p.q = x[0].data_ptr();
+  p.k = x[1].data_ptr();
+  p.v = x[2].data_ptr();
+  p.out = out.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    p.q_strides[i] = x[0].stride(i);
+    p.k_strides[i] = x[1].stride(i);
+    p.v_strides[i] = x[2].stride(i);
+    p.o_strides[i] = out.stride(i);
+  }
+  p.window = window;
+  p.sinks = sinks;
+  p.attn_scale = (float)scale;
+  p.causal = causal;
+  p.status = (int*)status.data_ptr();
+  p.stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream();
+  checked(entry.prefill(&p));
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(lib, decode, append, dequantize, workspace_bytes, copy, prefill): the package's _lib module and the entry points' addresses
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  arguments(nargs, 6);
-  void* at[5];
-  for (int i = 0; i < 5; ++i) {
+  arguments(nargs, 7);
+  void* at[6];
+  for (int i = 0; i < 6; ++i) {
     at[i] = PyLong_AsVoidPtr(args[1 + i]);
     if (!at[i]) raise_python();
   }
@@ -493,6 +567,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   entry.dequantize = reinterpret_cast<decltype(entry.dequantize)>(at[2]);
   entry.workspace_bytes = reinterpret_cast<decltype(entry.workspace_bytes)>(at[3]);
   entry.copy = reinterpret_cast<decltype(entry.copy)>(at[4]);
+  entry.prefill = reinterpret_cast<decltype(entry.prefill)>(at[5]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -503,6 +578,7 @@ PyMethodDef methods[] = {
     {"append", (PyCFunction)(void*)append, METH_FASTCALL, nullptr},
     {"dequantize", (PyCFunction)(void*)dequantize, METH_FASTCALL, nullptr},
     {"copy_pages", (PyCFunction)(void*)copy_pages, METH_FASTCALL, nullptr},
+    {"prefill", (PyCFunction)(void*)prefill, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -699,47 +699,8 @@ def prefill_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.T
     window > 0 (causal only): the query at position i = row + S - L sees the keys in (i - window, i]
     and the first `sinks` ones; key tiles that nothing sees are skipped.  As in any masked matrix
     product, a hidden value row that is Inf or NaN still reaches rows that share a 128-key tile with it."""
-    _lib.require_cuda(queries, keys, values)
-    if queries.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError("prefill_attention takes float16 or bfloat16 tensors")
-    if keys.dtype != queries.dtype or values.dtype != queries.dtype:
-        raise ValueError("queries, keys and values must share one dtype")
-    B, n_q, L, D = queries.shape
-    Bk, n_kv, S, Dk = keys.shape
-    if D != 128 or Dk != 128 or values.shape[-1] != 128:
-        raise ValueError(f"prefill_attention supports head_dim 128, got {D}")
-    if n_q % n_kv:
-        raise ValueError(f"n_q_heads ({n_q}) must equal n_kv_heads ({n_kv}) * n_rep ({n_q // max(n_kv, 1)})")
-    if values.shape[:3] != keys.shape[:3] or Bk != B:
-        raise ValueError("keys and values must have the same (batch, heads, length)")
-
-    def usable(t):
-        st = t.stride()
-        return t if st[3] == 1 and not (st[0] | st[1] | st[2]) & 7 and not t.data_ptr() & 15 else t.contiguous()
-
-    q, k, v = usable(queries), usable(keys), usable(values)
-    if window < 0 or sinks < 0 or (sinks and not window) or (window and not causal):
-        raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, sinks need a window, "
-                         "and a window needs causal attention")
-    if out is None:
-        out = torch.empty((B, n_q, L, D), dtype=q.dtype, device=q.device)
-    status = _lib.workspace(16, q.device, tag="prefill").data_ptr()
-    stream = _lib.stream_handle(q.device)
-    qs, ks, vs, os = q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3]
-    if not window:
-        _lib.check(_lib.lib().tq_prefill_sdpa(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.dtype_code(q.dtype), B, n_q, n_kv, L, S, D,
-            *qs, *ks, *vs, *os, float(scale), 1 if causal else 0, status, stream))
-        return out
-    args = _lib.PREFILL_PARAMS.pack(
-        _lib.PREFILL_PARAMS.size, _lib.dtype_code(q.dtype), B, n_q, n_kv, D, L, S, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        out.data_ptr(), *qs, *ks, *vs, *os, min(int(window), 1 << 40), min(int(sinks), 1 << 40), scale, 1, status, stream)
-    if q.get_device() == torch.cuda.current_device():
-        _lib.check(_lib.lib().tq_prefill_sdpa_window(args))
-    else:
-        with torch.cuda.device(q.device):
-            _lib.check(_lib.lib().tq_prefill_sdpa_window(args))
-    return out
+    status = _lib.workspace(16, queries.device, tag="prefill") if queries.is_cuda else queries
+    return (_lib.native or _lib.load_native()).prefill(queries, keys, values, scale, causal, out, window, sinks, status)
 
 
 def prefill_status(device) -> int:

@@ -24,22 +24,6 @@ from . import _lib
 
 __all__ = ["paged_append", "paged_decode", "paged_dequantize", "copy_pages", "paged_status"]
 
-_native = None
-
-
-def _load():
-    """The extension module that makes the calls (csrc/calls.cpp), bound to the loaded libtqb200.so."""
-    global _native
-    try:
-        from . import _calls
-    except ImportError as e:
-        raise RuntimeError("_calls.so is missing or does not fit this torch: run make in the package folder") from e
-    lib = _lib.lib()
-    _calls.bind(_lib, *[ctypes.cast(getattr(lib, "tq_" + name), ctypes.c_void_p).value for name in (
-        "paged_decode", "paged_append", "paged_dequantize", "paged_decode_workspace_bytes", "copy_pages")])
-    _native = _calls
-    return _calls
-
 
 def paged_append(keys: torch.Tensor, values: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
                  starts: torch.Tensor, counts: torch.Tensor | None = None) -> None:
@@ -50,7 +34,7 @@ def paged_append(keys: torch.Tensor, values: torch.Tensor, *, k: dict, v: dict, 
     tokens behind counts[b] are not read.  Packed halves get the words and norms `fused_quantize` gives; dense halves
     are copied and need the pages' own type.  Two tokens of one call must not share a place (sequences that share a
     page must not both write it)."""
-    (_native or _load()).append(keys, values, k, v, page_table, starts, counts)
+    (_lib.native or _lib.load_native()).append(keys, values, k, v, page_table, starts, counts)
 
 
 def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor, seq_lens: torch.Tensor, attn_scale: float,
@@ -68,7 +52,7 @@ def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
 
     The weights are 16-bit in the tensor-core kernel (head_dim 128, 3 / 4-bit values, 16-bit or 3 / 4-bit keys, 16-bit
     queries); float32 queries and every other shape take the 32-bit kernel."""
-    return (_native or _load()).decode(q, k, v, page_table, seq_lens, attn_scale, window, sinks, out, out_dtype, workspace)
+    return (_lib.native or _lib.load_native()).decode(q, k, v, page_table, seq_lens, attn_scale, window, sinks, out, out_dtype, workspace)
 
 
 def paged_workspace_bytes(device, dim: int) -> int:
@@ -85,7 +69,7 @@ def paged_dequantize(pool: dict, *, page_table: torch.Tensor, seq_lens: torch.Te
     and `packed_dequantize` give; rows at and behind seq_lens[b], and of pages that the sequence no longer holds
     (table entry -1), are zero.  Dense pools are gathered as they are.
     `out` optionally names the contiguous tensor to write."""
-    return (_native or _load()).dequantize(pool, page_table, seq_lens, length, dtype, out)
+    return (_lib.native or _lib.load_native()).dequantize(pool, page_table, seq_lens, length, dtype, out)
 
 
 def copy_pages(pools, src, dst) -> None:
@@ -94,7 +78,7 @@ def copy_pages(pools, src, dst) -> None:
 
     src / dst: lists or CPU tensors, which are checked here, or int32 CUDA tensors, of which the kernel only checks
     that they lie inside the pools.  No page may be written twice, or both read and written, by one call."""
-    (_native or _load()).copy_pages(pools, src, dst)
+    (_lib.native or _lib.load_native()).copy_pages(pools, src, dst)
 
 
 def paged_status(device) -> int:
