@@ -29,7 +29,7 @@ int paged_status_ptr(int** out) {
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kTile = 32;            // positions per tile of the general kernel: one per lane
 
 // ---- general decode -----------------------------------------------------------------------------------
@@ -75,7 +75,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
     const int cnt = cur.count_to(end);
     const int b = cur.b, kvh = cur.group / rg_per_head, r0 = (cur.group % rg_per_head) * kPagedRows;
     const int nr = min(kPagedRows, a.n_rep - r0), h0 = kvh * a.n_rep + r0;
-    {   // query rows of the group: warp r prepares row r (rotated for packed keys), stored [element][row]
+    if (warp < kPagedRows) {   // query rows of the group: warp r prepares row r (rotated for packed keys), stored [element][row]
       float x[EPL];
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
