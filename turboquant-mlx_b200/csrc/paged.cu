@@ -32,6 +32,15 @@ namespace {
 constexpr int kWarps = 16;
 constexpr int kTile = 32;            // positions per tile of the general kernel: one per lane
 
+// two 32-bit floats at once, each rounded like the scalar operation
+__device__ __forceinline__ float2 fma2(float2 x, float y, float2 z) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %6};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y), "f"(z.x), "f"(z.y));
+  return r;
+}
+
 // ---- general decode -----------------------------------------------------------------------------------
 // out = sum_p softmax(scale * q . k_p) v_p in 32 bits on the CUDA cores, for every head dimension, code width
 // and key format; calls that qualify take the tensor-core kernel instead.  One pass over the rows with a
@@ -68,6 +77,8 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
   const int kvpw = vals_per_word(a.k.bits), kpd = packed_words(DIM, a.k.bits);
   const int vvpw = vals_per_word(a.v.bits), vpd = packed_words(DIM, a.v.bits);
   const uint32_t kmask = (1u << a.k.bits) - 1u, vmask = (1u << a.v.bits) - 1u;
+  // a lane's elements lie in one word or two neighbours
+  const int v_word0 = lane * EPL / vvpw, v_word1 = (lane * EPL + EPL - 1) / vvpw;
   const bool polar = a.k.format == TQ_KV_POLAR;
   const int rg_per_head = a.groups / a.n_kv_heads;
 
@@ -89,13 +100,14 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
       for (int j = 0; j < EPL; ++j) q_s[(lane * EPL + j) * kPagedRows + warp] = x[j];
     }
     __syncthreads();
-    float m[kPagedRows], l[kPagedRows], o[kPagedRows][EPL];
+    float m[kPagedRows], l[kPagedRows];
+    float2 o[kPagedRows / 2][EPL];                     // two heads side by side
 #pragma unroll
     for (int r = 0; r < kPagedRows; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.f;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) o[r][j] = 0.f;
+      for (int j = 0; j < EPL; ++j) o[r / 2][j] = make_float2(0.f, 0.f);
     }
     for (int i = warp; i < cnt; i += kWarps) {
       const int p0 = cur.span.tile_at(cur.j + i) * kTile, pos = p0 + lane;
@@ -103,22 +115,26 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
       const int row = p0 & ((1 << a.view.page_shift) - 1);
       if (page < 0 && lane == 0) atomicExch(a.view.status, 1);
       const bool seen = cur.span.sees(pos, a.sinks);
-      float s[kPagedRows];
+      float2 s2[kPagedRows / 2];
 #pragma unroll
-      for (int r = 0; r < kPagedRows; ++r) s[r] = 0.f;
+      for (int r = 0; r < kPagedRows / 2; ++r) s2[r] = make_float2(0.f, 0.f);
       if (page >= 0 && seen) {
         auto add = [&](int e, float c) {
           const float4 qa = *reinterpret_cast<const float4*>(q_s + e * kPagedRows);
           const float4 qb = *reinterpret_cast<const float4*>(q_s + e * kPagedRows + 4);
-          s[0] += c * qa.x; s[1] += c * qa.y; s[2] += c * qa.z; s[3] += c * qa.w;
-          s[4] += c * qb.x; s[5] += c * qb.y; s[6] += c * qb.z; s[7] += c * qb.w;
+          s2[0] = fma2(make_float2(qa.x, qa.y), c, s2[0]);
+          s2[1] = fma2(make_float2(qa.z, qa.w), c, s2[1]);
+          s2[2] = fma2(make_float2(qb.x, qb.y), c, s2[2]);
+          s2[3] = fma2(make_float2(qb.z, qb.w), c, s2[3]);
         };
         float post = a.scale_log2;
         if (polar) {
           const uint32_t* kr = reinterpret_cast<const uint32_t*>(a.k.data) + page * a.k.page_stride + kvh * a.k.head_stride +
                                (int64_t)(row + lane) * kpd;
+          uint32_t next = __ldg(kr);
           for (int w = 0; w < kpd; ++w) {
-            const uint32_t word = __ldg(kr + w);
+            const uint32_t word = next;
+            if (w + 1 < kpd) next = __ldg(kr + w + 1);
             for (int k = 0; k < kvpw && w * kvpw + k < DIM; ++k) add(w * kvpw + k, kc_s[(word >> (k * a.k.bits)) & kmask]);
           }
           post *= a.k.norms[page * a.k.norm_page_stride + kvh * a.k.norm_head_stride + row + lane] * (1.0f / DIM);
@@ -127,7 +143,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
           for (int e = 0; e < DIM; ++e) add(e, load_elem(a.k.data, a.k.dtype, off + e));
         }
 #pragma unroll
-        for (int r = 0; r < kPagedRows; ++r) s[r] *= post;
+        for (int r = 0; r < kPagedRows / 2; ++r) s2[r] = make_float2(s2[r].x * post, s2[r].y * post);
       }
       const float vn = page >= 0 && seen
                            ? a.v.norms[page * a.v.norm_page_stride + kvh * a.v.norm_head_stride + row + lane] : 0.f;
@@ -136,7 +152,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
 #pragma unroll
       for (int r = 0; r < kPagedRows; ++r) {
         // a page outside the pool: the sequence's output becomes NaN instead of a plausible number
-        const float sr = page < 0 ? __int_as_float(0x7fc00000) : seen ? s[r] : -INFINITY;
+        const float sr = page < 0 ? __int_as_float(0x7fc00000) : seen ? (r & 1 ? s2[r / 2].y : s2[r / 2].x) : -INFINITY;
         const float mn = fmaxf(m[r], warp_max(sr));       // fmaxf passes over NaN: the sum below carries it
         const float alpha = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn);
         const float p = mn == -INFINITY ? (page < 0 ? sr : 0.f) : paged_ex2(sr - mn);
@@ -144,22 +160,34 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
         l[r] = l[r] * alpha + warp_sum(p);
         pw[lane * kPagedRows + r] = p * vn;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) o[r][j] *= alpha;
+        for (int j = 0; j < EPL; ++j) (r & 1 ? o[r / 2][j].y : o[r / 2][j].x) *= alpha;
       }
       __syncwarp();
       if (page >= 0) {
         const uint32_t* vr = reinterpret_cast<const uint32_t*>(a.v.data) + page * a.v.page_stride + kvh * a.v.head_stride +
                              (int64_t)row * vpd;
-        for (int k = 0; k < kTile; ++k) {
-          if (!cur.span.sees(p0 + k, a.sinks)) continue;
-          const float4 wa = *reinterpret_cast<const float4*>(pw + k * kPagedRows);
-          const float4 wb = *reinterpret_cast<const float4*>(pw + k * kPagedRows + 4);
+        // hidden positions have weight 0; four rows' words are on their way at a time
+#pragma unroll 1
+        for (int k0 = 0; k0 < kTile; k0 += 4) {
+          uint32_t w0[4], w1[4];
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            const int e = lane * EPL + j;
-            const float c = vc_s[(__ldg(vr + (int64_t)k * vpd + e / vvpw) >> ((e % vvpw) * a.v.bits)) & vmask];
-            o[0][j] += wa.x * c; o[1][j] += wa.y * c; o[2][j] += wa.z * c; o[3][j] += wa.w * c;
-            o[4][j] += wb.x * c; o[5][j] += wb.y * c; o[6][j] += wb.z * c; o[7][j] += wb.w * c;
+          for (int k = 0; k < 4; ++k) {
+            w0[k] = __ldg(vr + (k0 + k) * vpd + v_word0);
+            w1[k] = __ldg(vr + (k0 + k) * vpd + v_word1);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 wa = *reinterpret_cast<const float4*>(pw + (k0 + k) * kPagedRows);
+            const float4 wb = *reinterpret_cast<const float4*>(pw + (k0 + k) * kPagedRows + 4);
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) {
+              const int e = lane * EPL + j, at = e / vvpw;
+              const float c = vc_s[((at == v_word0 ? w0[k] : w1[k]) >> ((e - at * vvpw) * a.v.bits)) & vmask];
+              o[0][j] = fma2(make_float2(wa.x, wa.y), c, o[0][j]);
+              o[1][j] = fma2(make_float2(wa.z, wa.w), c, o[1][j]);
+              o[2][j] = fma2(make_float2(wb.x, wb.y), c, o[2][j]);
+              o[3][j] = fma2(make_float2(wb.z, wb.w), c, o[3][j]);
+            }
           }
         }
       }
@@ -168,7 +196,7 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
 #pragma unroll
     for (int r = 0; r < kPagedRows; ++r) {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) o_s[(warp * kPagedRows + r) * DIM + lane * EPL + j] = o[r][j];
+      for (int j = 0; j < EPL; ++j) o_s[(warp * kPagedRows + r) * DIM + lane * EPL + j] = r & 1 ? o[r / 2][j].y : o[r / 2][j].x;
       if (lane == 0) {
         m_s[warp][r] = m[r];
         l_s[warp][r] = l[r];
