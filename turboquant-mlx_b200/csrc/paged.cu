@@ -140,7 +140,22 @@ paged_decode_general_kernel(const PagedDecodeArgs a) {
           post *= a.k.norms[page * a.k.norm_page_stride + kvh * a.k.norm_head_stride + row + lane] * (1.0f / DIM);
         } else {
           const int64_t off = page * a.k.page_stride + kvh * a.k.head_stride + (int64_t)(row + lane) * DIM;
-          for (int e = 0; e < DIM; ++e) add(e, load_elem(a.k.data, a.k.dtype, off + e));
+          const uint16_t* kr = reinterpret_cast<const uint16_t*>(a.k.data) + off;
+          if (a.k.dtype != TQ_F32 && ((uintptr_t)kr & 15) == 0) {
+            for (int e = 0; e < DIM; e += 8) {
+              const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(kr + e));
+              const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = a.k.dtype == TQ_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                                     : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+                add(e + 2 * k, f.x);
+                add(e + 2 * k + 1, f.y);
+              }
+            }
+          } else {
+            for (int e = 0; e < DIM; ++e) add(e, load_elem(a.k.data, a.k.dtype, off + e));
+          }
         }
 #pragma unroll
         for (int r = 0; r < kPagedRows / 2; ++r) s2[r] = make_float2(s2[r].x * post, s2[r].y * post);
