@@ -189,14 +189,6 @@ __device__ __forceinline__ Plan make_paged_plan(const PagedDecodeArgs& a, const 
   }
   return p;
 }
-// Cost of one group in the sequences in front of sequence b.
-__device__ __forceinline__ int cost_before(const PagedDecodeArgs& a, const int* prefix, int b) {
-  const int per = plan_stride(a);
-  int t = prefix[b / per];
-  for (int i = b / per * per; i < b; ++i) t += cost_of(a, span_of(a, i));
-  return t;
-}
-
 // A tile of the numbering: sequence, (kv head, row group), tile inside the group.
 struct Cursor {
   int b, group, j;
