@@ -1,0 +1,61 @@
+"""Steps of a paged batch in which the sequences differ in what they receive, on a GPU, against 64-bit references."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import paged_ref as pr  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+D = 128
+SCALE = 1 / math.sqrt(D)
+
+
+class _Half:
+    """A cache half seen by the 64-bit reference."""
+
+    def __init__(self, cache, desc, q):
+        self.bits, self.dim, self.page = (q.bits if q else 0), cache.dim, cache.sequences.page_size
+        if q is None:
+            self.data = desc["data"]
+        else:
+            self.packed, self.norms, self.quant = desc["packed"], desc["norms"], q
+
+    rotated, rows = pr.Pool.rotated, pr.Pool.rows
+
+
+def _check(tq, cache, q, out, lens):
+    """A single-token step's attention against 64 bits; its weights are 16-bit."""
+    s = cache.sequences
+    ref, tol = pr.decode_ref(tq, q[:, :, 0], _Half(cache, cache.k, cache._k_q), _Half(cache, cache.v, cache._v_q), s.table,
+                             lens, SCALE, s.window, s.sinks, torch.finfo(torch.float16).eps / 2, q.dtype)
+    pr.check(out[:, :, 0], ref, tol)
+
+
+def _rows(B, H, T, dev, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn((B, H, T, D), generator=g).half().to(dev) for _ in range(2)]
+
+
+def _query(B, n_q, dev, seed):
+    return torch.randn((B, n_q, 1, D), generator=torch.Generator().manual_seed(seed)).half().to(dev)
+
+
+@pytest.mark.parametrize("k_bits", [0, 3])
+@pytest.mark.parametrize("n,window,sinks", [(95, 64, 0), (163, 100, 4), (195, 100, 4), (96, 64, 0)])
+def test_a_waiting_sequence_keeps_its_window(tq, dev, k_bits, n, window, sinks):
+    """At these lengths the window of a sequence that receives nothing begins at the end of a page (and, last, behind it)."""
+    cache, = tq.make_paged_caches(1, 20, 2, k_bits=k_bits, page_size=32, window=window, sinks=sinks)
+    seqs = cache.sequences
+    ids = [seqs.add(), seqs.add()]
+    seqs.begin(ids, n)
+    cache.update_and_fetch(*_rows(2, 2, n, dev, n))
+    seqs.begin(ids, [1, 0])
+    cache.update_and_fetch(*_rows(2, 2, 1, dev, n + 1))
+    q = _query(2, 8, dev, n)
+    out = cache.attention(q, SCALE)
+    assert tq.paged_status(dev) == 0
+    _check(tq, cache, q, out, [n + 1, n])

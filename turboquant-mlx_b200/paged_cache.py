@@ -141,8 +141,9 @@ class PagedSequences:
             shared = [i for i in range(first, min(want, len(pages))) if pages[i] >= 0 and self._refs[pages[i]] > 1] if c else []
             hidden = []
             if self.window:
+                # the step attends from position `start`, a sequence that receives nothing from its last one
                 hidden = [i for i in range(min(first, len(pages))) if pages[i] >= 0 and i * size >= self.sinks
-                          and (i + 1) * size <= start + 1 - self.window]
+                          and (i + 1) * size <= start + min(c, 1) - self.window]
                 gone += [pages[i] for i in hidden]
             need += max(0, want - len(pages)) + len(shared)
             todo.append((seq, start, c, want, shared, hidden))
@@ -325,8 +326,9 @@ class PagedTurboQuantCache:
     def attention(self, queries, scale: float, mask=None):
         """queries (B, n_q, T, dim) of the step's new tokens -> (B, n_q, T, dim) in their dtype.
 
-        One token per sequence: `paged_decode`.  Several: the sequences' rows are read back and the prompt kernel
-        attends, causally and within the window; rows of padding tokens are zero."""
+        One token per sequence: `paged_decode`; a sequence that received none in this step is attended from its last
+        position, as if the query were that token's (an empty one gives zeros).  Several: the sequences' rows are read
+        back and the prompt kernel attends, causally and within the window; rows of padding tokens are zero."""
         s = self._step()
         B, n_q, T, D = queries.shape
         if not (mask is None or (isinstance(mask, str) and mask == "causal")):
