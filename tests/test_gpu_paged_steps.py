@@ -59,3 +59,35 @@ def test_a_waiting_sequence_keeps_its_window(tq, dev, k_bits, n, window, sinks):
     out = cache.attention(q, SCALE)
     assert tq.paged_status(dev) == 0
     _check(tq, cache, q, out, [n + 1, n])
+
+
+def test_a_waiting_sequence_in_a_replayed_step(tq, dev):
+    """A captured step with a sequence that receives nothing, replayed over the end of its page: it neither grows nor
+    changes, and the one that receives grows as in eager steps."""
+    cache, = tq.make_paged_caches(1, 12, 2, page_size=32)
+    seqs = cache.sequences
+    ids = [seqs.add(), seqs.add()]
+    seqs.begin(ids, 31)
+    cache.update_and_fetch(*_rows(2, 2, 31, dev, 0))
+    keys, values = _rows(2, 2, 1, dev, 1)
+    q = _query(2, 8, dev, 2)
+    seqs.begin(ids, [1, 0], reserve=4)
+
+    def step():
+        cache.update_and_fetch(keys, values)
+        out = cache.attention(q, SCALE)
+        seqs.advance_device()
+        return out
+
+    first = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for n in range(33, 37):
+        graph.replay()
+        assert seqs.lens.tolist() == [n + 1, 31]                # of the step to come
+        _check(tq, cache, q, out, [n, 31])
+        assert torch.equal(out[1], first[1])
+    seqs.advance(4)
+    assert [seqs.length(s) for s in ids] == [36, 31] and tq.paged_status(dev) == 0

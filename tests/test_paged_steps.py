@@ -30,3 +30,28 @@ def test_a_waiting_sequence_keeps_its_window(tq, window, sinks):
         _assert_visible_held(seqs, b, n - 1)
         seqs.begin([b], 1)
         _assert_visible_held(seqs, b, n)
+
+
+def test_replays_advance_only_what_receives(tq):
+    """A captured one-token step replayed: a sequence that began it with 0 tokens stays where it is, on the device and on
+    the host; steps of several tokens cannot be replayed as one-token steps."""
+    seqs = _seqs(tq)
+    a, b, c = seqs.add(), seqs.add(), seqs.add()
+    seqs.begin([a, b, c], [31, 10, 0], reserve=7)
+    with pytest.raises(ValueError, match="one new token"):
+        seqs.advance_device()
+    with pytest.raises(ValueError, match="one new token"):
+        seqs.advance(1)
+    assert [seqs.length(s) for s in (a, b, c)] == [31, 10, 0] and seqs.starts.tolist() == [0, 0, 0]
+    seqs.begin([a, b, c], [1, 0, 0], reserve=5)
+    for k in range(3):
+        assert seqs.starts.tolist() == [31 + k, 10, 0] and seqs.lens.tolist() == [32 + k, 10, 0]
+        seqs.advance_device()
+    seqs.advance(2)
+    assert [seqs.length(s) for s in (a, b, c)] == [34, 10, 0]
+    assert seqs._host_starts == [33, 10, 0] and seqs._host_lens == [34, 10, 0]
+    with pytest.raises(ValueError, match="no pages"):
+        seqs.advance(100)
+    with pytest.raises(ValueError):
+        seqs.advance(-1)
+    assert [seqs.length(s) for s in (a, b, c)] == [34, 10, 0]

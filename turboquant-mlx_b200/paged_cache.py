@@ -50,6 +50,7 @@ class PagedSequences:
         self.table = self.starts = self.lens = self.counts = None
         self._host_starts: list = []
         self._host_lens: list = []
+        self._host_counts: list = []
         self._most = 0
         self._scratch: dict = {}                            # head_dim -> decode workspace, shared by the layers of the step
 
@@ -179,6 +180,7 @@ class PagedSequences:
         self.active = ids
         self._host_starts = [t[1] for t in todo]
         self._host_lens = [t[1] + t[2] for t in todo]
+        self._host_counts = counts
         self._most = max(counts)
         self._scratch = {}
         width = max(1, max(len(self._pages[s]) for s in ids))
@@ -197,22 +199,33 @@ class PagedSequences:
             self._scratch[dim] = torch.zeros((paged_workspace_bytes(self.device, dim),), dtype=torch.uint8, device=self.device)
         return self._scratch.get(dim)
 
+    def _one_token_step(self):
+        if self._most > 1:
+            raise ValueError(f"the step began with up to {self._most} tokens per sequence: only steps of at most one new token "
+                             "per sequence are replayed")
+
     def advance_device(self) -> None:
-        """One more token per active sequence, on the device only: the body of a captured decode step ends with it.  The
-        pages must have been reserved (`begin(..., reserve=n)`); `advance` tells the host afterwards.  A captured step
-        belongs to the `begin` in front of it: it reads that step's tables, and the next `begin` ends its use."""
-        self.starts += 1
-        self.lens += 1
+        """One more token per active sequence that receives one, on the device only: the body of a captured decode step ends
+        with it.  Sequences that began the step with 0 tokens stay where they are.  The pages must have been reserved
+        (`begin(..., reserve=n)`); `advance` tells the host afterwards.  A captured step belongs to the `begin` in front of
+        it: it reads that step's tables, and the next `begin` ends its use."""
+        self._one_token_step()
+        self.starts += self.counts
+        self.lens += self.counts
 
     def advance(self, n: int) -> None:
         """Host lengths after n replays of a captured one-token step."""
-        for k, seq in enumerate(self.active):
-            if self._lens[seq] + n > len(self._pages[seq]) * self.page_size:
-                raise ValueError(f"sequence {seq} has no pages for {n} more tokens")
-        for k, seq in enumerate(self.active):
-            self._lens[seq] += n
-            self._host_starts[k] += n
-            self._host_lens[k] += n
+        self._one_token_step()
+        if n < 0:
+            raise ValueError(f"{n} replays")
+        grow = [n * c for c in self._host_counts]
+        for seq, g in zip(self.active, grow):
+            if self._lens[seq] + g > len(self._pages[seq]) * self.page_size:
+                raise ValueError(f"sequence {seq} has no pages for {g} more tokens")
+        for k, (seq, g) in enumerate(zip(self.active, grow)):
+            self._lens[seq] += g
+            self._host_starts[k] += g
+            self._host_lens[k] += g
 
     def compact(self) -> int:
         """Move the used pages to the front of the pools, in one launch; returns how many moved.  The pages behind
