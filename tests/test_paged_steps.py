@@ -55,3 +55,109 @@ def test_replays_advance_only_what_receives(tq):
     with pytest.raises(ValueError):
         seqs.advance(-1)
     assert [seqs.length(s) for s in (a, b, c)] == [34, 10, 0]
+
+
+def test_replays_after_a_fork_write_to_pages_of_their_own(tq):
+    """Pages reserved by an earlier step belong to the sequence they were taken for, not to its forks: whatever `advance`
+    accepts ends in pages that nobody else holds."""
+    seqs = _seqs(tq, n_pages=12)
+    a = seqs.add()
+    seqs.begin([a], 1, reserve=90)
+    b = seqs.fork(a)
+    assert seqs.used_pages == 3 and len(seqs._pages[b]) == 1
+    seqs.begin([a, b], 1)
+    for s in (a, b):
+        for p in seqs._pages[s][seqs._host_starts[0] // 32:]:
+            assert seqs._refs[p] == 1
+    with pytest.raises(ValueError, match=f"sequence {b} has no pages"):
+        seqs.advance(60)                                   # nothing is reserved for b
+    seqs.begin([a, b], 1, reserve=60)
+    seqs.advance(60)
+    assert not set(seqs._pages[a]) & set(seqs._pages[b])
+    assert seqs.length(a) == seqs.length(b) == 63
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+def test_places_written_by_replays_are_private(tq, monkeypatch, window, sinks):
+    """Random histories with forks, reserves and replays: every place a replay writes lies in a page of one sequence, what
+    a step sees is held, and contents stay those of the sequence."""
+    import turboquant_mlx_b200.paged_cache as pc
+    for seed in range(30):
+        rng = random.Random(seed)
+        seqs = _seqs(tq, rng.choice([12, 30, 80]), window=window, sinks=sinks)
+        place, text, token = {}, {}, 0
+
+        def copy(_pools, src, dst):
+            assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+            for s, d in zip(src, dst):
+                for r in range(32):
+                    place[d, r] = place.get((s, r))
+        monkeypatch.setattr(pc, "copy_pages", copy)
+        seqs.layers.append(type("L", (), {"pools": lambda self: [], "_resize": lambda self, n: None})())
+
+        def write(s, pos):
+            nonlocal token
+            page = seqs._pages[s][pos // 32]
+            assert page >= 0 and seqs._refs[page] == 1
+            place[page, pos % 32] = token
+            text[s].append(token)
+            token += 1
+
+        for _ in range(200):
+            op = rng.choice(["step", "step", "step", "add", "fork", "free", "trim", "compact"])
+            if op == "add":
+                text[seqs.add()] = []
+            elif op == "fork" and text:
+                s = rng.choice(list(text))
+                text[seqs.fork(s)] = list(text[s])
+            elif op == "free" and text:
+                s = rng.choice(list(text))
+                seqs.free(s)
+                del text[s]
+            elif op == "trim" and text:
+                s = rng.choice(list(text))
+                try:
+                    n = seqs.trim(s, rng.randint(1, 50))
+                except ValueError:
+                    assert window
+                    continue
+                text[s] = text[s][:len(text[s]) - n]
+            elif op == "compact":
+                seqs.compact()
+            elif op == "step" and text:
+                ids = rng.sample(list(text), rng.randint(1, len(text)))
+                counts = [rng.choice([0, 1, 1, 1] if rng.random() < 0.6 else [0, 1, 40]) for _ in ids]
+                if max(counts) == 0:
+                    continue
+                try:
+                    seqs.begin(ids, counts, reserve=rng.choice([0, 0, 70]))
+                except MemoryError:
+                    continue
+                for s, c in zip(ids, counts):
+                    _assert_visible_held(seqs, s, len(text[s]) + min(c, 1) - 1)
+                    for pos in range(len(text[s]), len(text[s]) + c):
+                        write(s, pos)
+                if rng.random() < 0.3:
+                    s = rng.choice(ids)
+                    text[seqs.fork(s)] = list(text[s])
+                if max(counts) == 1:
+                    n = rng.randint(0, 40)
+                    try:
+                        seqs.advance(n)
+                    except ValueError:
+                        n = 0
+                    for _ in range(n):
+                        for s, c in zip(ids, counts):
+                            if c:
+                                page = seqs._pages[s][len(text[s]) // 32]
+                                # a fork made inside the step may share the page in hand, but not what is written now
+                                assert page >= 0 and all(o == s or seqs.length(o) <= len(text[s]) or
+                                                         page not in seqs._pages[o] for o in text)
+                                place[page, len(text[s]) % 32] = token
+                                text[s].append(token)
+                                token += 1
+            for s, want in text.items():
+                assert seqs.length(s) == len(want)
+                for i, t in enumerate(want):
+                    page = seqs._pages[s][i // 32]
+                    assert page < 0 and window or place[page, i % 32] == t

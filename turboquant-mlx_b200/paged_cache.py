@@ -62,8 +62,9 @@ class PagedSequences:
         return seq
 
     def fork(self, seq: int) -> int:
-        """A new sequence with the contents of `seq`, sharing its pages until one of the two writes to them."""
-        pages = list(self._pages[seq])
+        """A new sequence with the contents of `seq`, sharing the pages that hold them until one of the two writes to them.
+        Pages reserved for further tokens stay with `seq` alone: its replays write to them without another `begin`."""
+        pages = self._pages[seq][:-(-self._lens[seq] // self.page_size)]
         new = self.add()
         for p in pages:
             if p >= 0:
