@@ -161,3 +161,47 @@ def test_places_written_by_replays_are_private(tq, monkeypatch, window, sinks):
                 for i, t in enumerate(want):
                     page = seqs._pages[s][i // 32]
                     assert page < 0 and window or place[page, i % 32] == t
+
+
+def test_forks_that_write_together_need_one_page_less(tq, monkeypatch):
+    """The last of the sequences that share a page keeps it: a pool with room for the others' copies is enough, and one
+    page less is refused with nothing changed."""
+    import turboquant_mlx_b200.paged_cache as pc
+    copied = []
+    monkeypatch.setattr(pc, "copy_pages", lambda pools, src, dst: copied.append((src, dst)))
+    for n_forks, idle in ((1, 0), (3, 0), (3, 2)):
+        for spare in (0, -1):
+            copies = n_forks + (idle > 0)                  # an idle fork keeps the page, so every writer copies
+            n_pages = 1 + copies + spare
+            seqs = _seqs(tq, n_pages)
+            seqs.layers.append(type("L", (), {"pools": lambda self: []})())
+            a = seqs.add()
+            seqs.begin([a], 10)
+            ids = [a] + [seqs.fork(a) for _ in range(n_forks)]
+            for _ in range(idle):
+                seqs.fork(a)
+            copied.clear()
+            if spare:
+                with pytest.raises(MemoryError):
+                    seqs.begin(ids, 1)
+                assert [seqs.length(s) for s in ids] == [10] * len(ids) and not copied
+            else:
+                seqs.begin(ids, 1)
+                assert seqs.free_pages == 0 and len({seqs._pages[s][0] for s in ids}) == len(ids)
+                assert sum(len(src) for src, _ in copied) == copies
+
+
+def test_a_page_that_slides_out_of_one_fork_is_kept_by_the_other(tq, monkeypatch):
+    """A page that one active sequence frees behind its window while the other writes to it needs no copy."""
+    import turboquant_mlx_b200.paged_cache as pc
+    monkeypatch.setattr(pc, "copy_pages", lambda pools, src, dst: pytest.fail("copied"))
+    seqs = _seqs(tq, 3, window=32)
+    seqs.layers.append(type("L", (), {"pools": lambda self: []})())
+    a = seqs.add()
+    seqs.begin([a], 64)
+    b = seqs.fork(a)
+    seqs.trim(b, 44)
+    first = seqs._pages[a][0]
+    assert seqs._pages[b] == [first] and seqs.free_pages == 1
+    seqs.begin([a, b], 1)
+    assert seqs._pages[a][0] == -1 and seqs._pages[b] == [first] and seqs.free_pages == 0

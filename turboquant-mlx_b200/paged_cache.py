@@ -135,7 +135,7 @@ class PagedSequences:
         if len(counts) != len(ids) or min(counts) < 0 or max(counts) < 1 or reserve < 0:
             raise ValueError(f"{len(ids)} sequences, new tokens {counts}, reserve {reserve}")
         size = self.page_size
-        todo, need, gone = [], 0, []
+        todo, need, gone, writers = [], 0, [], {}            # writers: shared page -> active sequences that write to it
         for seq, c in zip(ids, counts):
             pages, start = self._pages[seq], self._lens[seq]
             want = -(-(start + c + (reserve if c else 0)) // size)
@@ -147,13 +147,16 @@ class PagedSequences:
                 hidden = [i for i in range(min(first, len(pages))) if pages[i] >= 0 and i * size >= self.sinks
                           and (i + 1) * size <= start + min(c, 1) - self.window]
                 gone += [pages[i] for i in hidden]
-            need += max(0, want - len(pages)) + len(shared)
+            need += max(0, want - len(pages))
+            for i in shared:
+                writers[pages[i]] = writers.get(pages[i], 0) + 1
             todo.append((seq, start, c, want, shared, hidden))
         drops: dict = {}
         for p in gone:
             drops[p] = drops.get(p, 0) + 1
         freed = sum(1 for p, n in drops.items() if self._refs[p] == n)
-        # two active sequences that share a page both want a copy of it although the second could keep it: counted above
+        # each writer of a shared page copies it, except the last when nobody else is left
+        need += sum(min(n, self._refs[p] - drops.get(p, 0) - 1) for p, n in writers.items())
         if need > len(self._free) + freed:
             raise MemoryError(f"the step needs {need} pages, {len(self._free) + freed} of {self.n_pages} are free")
         src, dst = [], []
