@@ -91,3 +91,68 @@ def test_a_waiting_sequence_in_a_replayed_step(tq, dev):
         assert torch.equal(out[1], first[1])
     seqs.advance(4)
     assert [seqs.length(s) for s in ids] == [36, 31] and tq.paged_status(dev) == 0
+
+
+def _three_layers(tq, dev, n=700):
+    """Caches of three layers with different rows, one query each, and what attention gives one after the other."""
+    caches = tq.make_paged_caches(3, 60, 2, page_size=32)
+    seqs = caches[0].sequences
+    ids = [seqs.add(), seqs.add()]
+    seqs.begin(ids, [n, 3])
+    for i, c in enumerate(caches):
+        c.update_and_fetch(*_rows(2, 2, n, dev, i))
+    seqs.begin(ids, 1)
+    for i, c in enumerate(caches):
+        c.update_and_fetch(*_rows(2, 2, 1, dev, 10 + i))
+    qs = [_query(2, 8, dev, 20 + i) for i in range(3)]
+    want = [c.attention(q, SCALE) for c, q in zip(caches, qs)]
+    for c, q, w in zip(caches, qs, want):
+        _check(tq, c, q, w, [n + 1, 4])
+    return caches, qs, want
+
+
+def test_layers_of_a_step_on_two_streams(tq, dev):
+    """Two layers of a step attended at the same time on two streams, many times over: each stream has its own scratch."""
+    caches, qs, want = _three_layers(tq, dev)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    outs = [[], []]
+    for _ in range(40):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(caches[i].attention(qs[i], SCALE))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_layers_of_a_captured_step(tq, dev):
+    """One graph with all layers, one with its layers on two branches: right in every replay, also side by side with each
+    other and with eager calls."""
+    caches, qs, want = _three_layers(tq, dev)
+    torch.cuda.synchronize()
+    main, side = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+    chain, fork = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(chain, stream=main):
+        a = [c.attention(q, SCALE) for c, q in zip(caches, qs)]
+    with torch.cuda.graph(fork, stream=main):
+        b = [caches[0].attention(qs[0], SCALE)]
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b.append(caches[1].attention(qs[1], SCALE))
+        b.append(caches[2].attention(qs[2], SCALE))
+        main.wait_stream(side)
+    for t in a + b:
+        t.zero_()
+    torch.cuda.synchronize()
+    eager = []
+    for _ in range(20):
+        with torch.cuda.stream(main):
+            chain.replay()
+        with torch.cuda.stream(side):
+            fork.replay()
+        eager.append(caches[0].attention(qs[0], SCALE))
+    torch.cuda.synchronize()
+    for got in (a, b):
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+    assert all(torch.equal(e, want[0]) for e in eager) and tq.paged_status(dev) == 0

@@ -205,3 +205,30 @@ def test_a_page_that_slides_out_of_one_fork_is_kept_by_the_other(tq, monkeypatch
     assert seqs._pages[b] == [first] and seqs.free_pages == 1
     seqs.begin([a, b], 1)
     assert seqs._pages[a][0] == -1 and seqs._pages[b] == [first] and seqs.free_pages == 0
+
+
+def test_step_scratch_belongs_to_a_stream(tq, monkeypatch):
+    """Attention calls of a step on two streams may run at the same time, so they do not share decode scratch; within a
+    capture the call brings its own."""
+    import types
+    import torch
+    import turboquant_mlx_b200.paged_cache as pc
+    now = types.SimpleNamespace(stream=11, capturing=False)
+    monkeypatch.setattr(pc, "paged_workspace_bytes", lambda device, dim: 64)
+    monkeypatch.setattr(pc, "stream_handle", lambda device: now.stream, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now.capturing)
+    seqs = _seqs(tq)
+    a = seqs.add()
+    seqs.begin([a], 1)
+    first = seqs._workspace(128)
+    assert first is seqs._workspace(128) and first is not seqs._workspace(64)
+    now.stream = 12
+    second = seqs._workspace(128)
+    assert second is not first and second.data_ptr() != first.data_ptr() and not second.any()
+    now.stream = 11
+    assert seqs._workspace(128) is first
+    now.capturing = True
+    assert seqs._workspace(128) is None                    # a graph's scratch is the graph's
+    now.capturing = False
+    seqs.begin([a], 1)
+    assert seqs._workspace(128) is not first

@@ -224,13 +224,15 @@ void checked(int rc) {
   if (!r.p) raise_python();
 }
 void arguments(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK_TYPE(n == want, want, " arguments expected, got ", n); }
-bool capturing(void* stream) {
+// The id of the capture the stream is in (never used twice in a process), 0: none.
+unsigned long long capture_of(void* stream) {
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing((cudaStream_t)stream, &st) != cudaSuccess) {
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &st, &id) != cudaSuccess) {
     cudaGetLastError();
-    return false;
+    return 0;
   }
-  return st != cudaStreamCaptureStatusNone;
+  return st == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
 // (q, k, v, page_table, seq_lens, attn_scale, window, sinks, out, out_dtype, workspace) -> out
@@ -284,8 +286,12 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   p.out = out.data_ptr();
   p.out_batch_stride = out.stride(0);
   p.out_head_stride = out.stride(1);
-  // scratch of the calls made on a stream outside of captures; never freed (the map outlives the interpreter)
-  static auto* kept = new std::map<std::tuple<int, void*, int64_t>, at::Tensor>;
+  // Scratch of the calls made on a stream outside of captures, and of those captured last on it; never freed (the maps
+  // outlive the interpreter).
+  using Place = std::tuple<int, void*, int64_t>;
+  static auto* kept = new std::map<Place, at::Tensor>;
+  static auto* captured = new std::map<Place, std::pair<unsigned long long, at::Tensor>>;
+  const Place place(index, p.stream, dim);
   at::Tensor own;
   const at::Tensor* ws = &own;
   if (args[10] != Py_None) {
@@ -293,10 +299,16 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int64_t need = entry.workspace_bytes(p.dim);
     TORCH_CHECK_VALUE(own.scalar_type() == at::kByte && own.is_contiguous() && index_of(own) == index && own.numel() >= need,
                       "workspace must be a contiguous uint8 tensor of at least ", need, " bytes on cuda:", index);
-  } else if (capturing(p.stream)) {                      // the graph's own, zeroed by every replay
-    own = at::zeros({entry.workspace_bytes(p.dim)}, q.options().dtype(at::kByte));
+  } else if (const unsigned long long id = capture_of(p.stream)) {
+    // the graph's own, from its pool, zeroed by every replay: the calls of one capture on one stream follow each other
+    auto& mine = (*captured)[place];
+    if (mine.first != id) {
+      mine.second = at::zeros({entry.workspace_bytes(p.dim)}, q.options().dtype(at::kByte));
+      mine.first = id;
+    }
+    ws = &mine.second;
   } else {
-    at::Tensor& mine = (*kept)[std::make_tuple(index, p.stream, dim)];
+    at::Tensor& mine = (*kept)[place];
     if (!mine.defined()) mine = at::zeros({entry.workspace_bytes(p.dim)}, q.options().dtype(at::kByte));
     ws = &mine;
   }
@@ -443,7 +455,7 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)index);
   void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream();
-  const bool in_capture = capturing(stream);
+  const bool in_capture = capture_of(stream) != 0;
   Ids src = ids(args[1], n_pages, "src", index, in_capture), dst = ids(args[2], n_pages, "dst", index, in_capture);
   const int64_t pairs = src.count();
   TORCH_CHECK_VALUE(pairs == dst.count(), pairs, " source and ", dst.count(), " target pages");

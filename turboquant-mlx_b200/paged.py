@@ -47,8 +47,8 @@ def paged_decode(q: torch.Tensor, *, k: dict, v: dict, page_table: torch.Tensor,
     `create_causal_mask` does); pages outside both may have been freed.  A sequence of length 0 gives zeros.
     Lengths beyond the table are cut to it.  `out` optionally names the tensor to write (rows contiguous).
     `workspace`: a zero-filled uint8 tensor of `paged_workspace_bytes` used by no other call that may be in flight
-    together with this one; every call leaves it ready for the next.  Without it the calls of a stream share one, and a
-    call captured in a CUDA graph gets one of its own from the graph's pool.
+    together with this one; every call leaves it ready for the next.  Without it the calls of a stream share one, and the
+    calls captured in a CUDA graph one per stream of the capture, from the graph's pool, zeroed by every replay.
 
     The weights are 16-bit in the tensor-core kernel (head_dim 128, 3 / 4-bit values, 16-bit or 3 / 4-bit keys, 16-bit
     queries); float32 queries and every other shape take the 32-bit kernel."""

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 
+from ._lib import stream_handle
 from .cache import _Quantizer, _zero
 from .packing import packed_dim
 from .paged import copy_pages, paged_append, paged_decode, paged_dequantize, paged_workspace_bytes
@@ -52,7 +53,7 @@ class PagedSequences:
         self._host_lens: list = []
         self._host_counts: list = []
         self._most = 0
-        self._scratch: dict = {}                            # head_dim -> decode workspace, shared by the layers of the step
+        self._scratch: dict = {}                            # (head_dim, stream) -> decode workspace, shared by the step's layers
 
     # ---- sequences --------------------------------------------------------------------------------------
     def add(self) -> int:
@@ -127,7 +128,8 @@ class PagedSequences:
         """Start a step: `ids` are the active sequences, in batch order, each about to receive new_tokens positions (one
         number, or one per sequence).  Pages for them, and for `reserve` further tokens, are taken; pages behind the
         window are freed; shared pages that will be written are copied.  Raises MemoryError, with nothing changed, when
-        the pool has too few free pages."""
+        the pool has too few free pages.  Work of the step before on other streams must have been joined to the current
+        stream (its tables go back to the allocator, and its freed pages to other sequences)."""
         ids = list(ids)
         if len(set(ids)) != len(ids) or not ids:
             raise ValueError("a step needs at least one sequence, each named once")
@@ -197,11 +199,14 @@ class PagedSequences:
         self.table = flat[3 * n:].view(n, width)
 
     def _workspace(self, dim: int):
-        """Decode scratch of the step.  A graph captured in one step never shares it with a graph of another; None in a
-        capture without an eager call in front (the call then gets its own)."""
-        if dim not in self._scratch and not torch.cuda.is_current_stream_capturing():
-            self._scratch[dim] = torch.zeros((paged_workspace_bytes(self.device, dim),), dtype=torch.uint8, device=self.device)
-        return self._scratch.get(dim)
+        """Decode scratch of the step on the current stream: calls on different streams may run at the same time.  None in
+        a capture, where the call takes scratch of the graph's own."""
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        key = dim, stream_handle(self.device)
+        if key not in self._scratch:
+            self._scratch[key] = torch.zeros((paged_workspace_bytes(self.device, dim),), dtype=torch.uint8, device=self.device)
+        return self._scratch[key]
 
     def _one_token_step(self):
         if self._most > 1:
