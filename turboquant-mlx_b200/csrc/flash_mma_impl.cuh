@@ -41,10 +41,9 @@
 // thread reads contiguous bytes of a row (see kslot_element()).
 #include <cuda_fp16.h>
 
-#include <mutex>
-
 #include "flash.cuh"
 #include "quantize_row.cuh"
+#include "scaled_book.cuh"
 
 namespace tq {
 namespace {
@@ -1234,59 +1233,6 @@ flash_mma_kernel(const FlashArgs a, const MmaTables tb) {
   if (independent && tid == 0) grid_dependency_wait();
 }
 
-// ---- host side: scaled f16 codebooks --------------------------------------------------
-struct ScaledBook {
-  float key[16];
-  int n;
-  uint16_t c16[16];
-  float beta;
-};
-
-// f16 has an 11-bit significand; rounding the centroids directly would leave a
-// fixed relative error of up to 2^-12 on each.  A common factor beta in [1, 2)
-// is searched so that every beta * c_i lands (almost) on an f16 value; 1/beta is
-// applied in float32 after the MMA.
-static void scale_codebook(const float* c, int n, ScaledBook* out) {
-  static std::mutex mu;
-  static ScaledBook cache[8];
-  static int n_cached = 0;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < n_cached; ++i) {
-    if (cache[i].n == n && memcmp(cache[i].key, c, n * sizeof(float)) == 0) {
-      *out = cache[i];
-      return;
-    }
-  }
-  float best_beta = 1.f;
-  double best_err = 1e30;
-  for (int step = 0; step < (1 << 16); ++step) {
-    const float beta = 1.0f + step * (1.0f / 65536.0f);
-    double worst = 0.0;
-    for (int i = 0; i < n && worst < best_err; ++i) {
-      if (c[i] == 0.f) continue;
-      const double exact = (double)beta * (double)c[i];
-      const double got = (double)__half2float(__float2half_rn((float)exact));
-      const double rel = fabs(got - exact) / fabs(exact);
-      if (rel > worst) worst = rel;
-    }
-    if (worst < best_err) {
-      best_err = worst;
-      best_beta = beta;
-    }
-  }
-  ScaledBook sb;
-  memset(&sb, 0, sizeof(sb));
-  sb.n = n;
-  memcpy(sb.key, c, n * sizeof(float));
-  sb.beta = best_beta;
-  for (int i = 0; i < n; ++i) {
-    const __half h = __float2half_rn(best_beta * c[i]);
-    sb.c16[i] = *reinterpret_cast<const uint16_t*>(&h);
-  }
-  if (n_cached < 8) cache[n_cached++] = sb;
-  *out = sb;
-}
-
 static int g_ctas_per_sm_seen = -1;   // occupancy the runtime reports for the variant set up last
 
 
@@ -1381,16 +1327,14 @@ int TQ_CAT(launch_flash_mma_, TQ_GEOM)(const FlashArgs& a, int splits, const Mma
     for (int i = 0; i < 16; ++i) tb.v_c16[i] = (uint16_t)(i == 0 ? 0 : __half_as_ushort(__float2half_rn((float)i)));
     tb.v_post = 1.0f;
   } else {
-    ScaledBook vb;
-    scale_codebook(a.v_cent.v, 1 << a.v_bits, &vb);
+    const ScaledBook vb = scaled_book(a.v_cent.v, 1 << a.v_bits);
     memcpy(tb.v_c16, vb.c16, sizeof(tb.v_c16));
     tb.v_post = 1.0f / vb.beta;
   }
   tb.k_post = a.attn_scale * kLog2e;
   int kf = KF_DENSE;
   if (a.k_format == TQ_KV_POLAR) {
-    ScaledBook kb;
-    scale_codebook(a.k_cent.v, 1 << a.k_bits, &kb);
+    const ScaledBook kb = scaled_book(a.k_cent.v, 1 << a.k_bits);
     memcpy(tb.k_c16, kb.c16, sizeof(tb.k_c16));
     tb.k_post = a.attn_scale * kLog2e / ((float)kDim * kb.beta);
     kf = a.k_bits == 3 ? KF_POLAR3 : KF_POLAR4;

@@ -27,10 +27,9 @@
 #include <cuda_fp16.h>
 #include <string.h>
 
-#include <mutex>
-
 #include "paged.cuh"
 #include "paged_host.cuh"
+#include "scaled_book.cuh"
 
 namespace tq {
 namespace {
@@ -776,53 +775,6 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------
-// 16-bit floats hold 11 bits; rounding the centroids directly would leave a fixed relative error of up to 2^-12 on each.
-// A common factor beta in [1, 2) is searched so that every beta * c lands (almost) on a 16-bit value; 1 / beta is
-// applied in 32 bits.  Kept by value (the codebook), not by address.
-struct ScaledBook {
-  int n;
-  float key[16];
-  uint16_t c16[16];
-  float beta;
-  bool good;             // every centroid within 2^-13 of its value (a codebook with wild levels may have no such factor)
-};
-void scale_book(const float* c, int n, ScaledBook* out) {
-  static std::mutex mu;
-  constexpr int kKept = 16;
-  static ScaledBook kept[kKept];
-  static int n_kept = 0;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < n_kept; ++i)
-    if (kept[i].n == n && memcmp(kept[i].key, c, n * sizeof(float)) == 0) {
-      *out = kept[i];
-      return;
-    }
-  ScaledBook sb;
-  memset(&sb, 0, sizeof(sb));
-  sb.n = n;
-  memcpy(sb.key, c, n * sizeof(float));
-  double best = 1e30;
-  sb.beta = 1.f;
-  for (int step = 0; step < (1 << 16); ++step) {
-    const float beta = 1.0f + step * (1.0f / 65536.0f);
-    double worst = 0.0;
-    for (int i = 0; i < n && worst < best; ++i) {
-      if (c[i] == 0.f) continue;
-      const double exact = (double)beta * (double)c[i];
-      const double rel = fabs((double)__half2float(__float2half_rn((float)exact)) - exact) / fabs(exact);
-      if (!(rel <= worst)) worst = rel == rel ? rel : 1e30;
-    }
-    if (worst < best) {
-      best = worst;
-      sb.beta = beta;
-    }
-  }
-  for (int i = 0; i < n; ++i) sb.c16[i] = __half_as_ushort(__float2half_rn(sb.beta * c[i]));
-  sb.good = best <= 1.0 / 8192;
-  if (n_kept < kKept) kept[n_kept++] = sb;
-  *out = sb;
-}
-
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <int KF, int VB, int W, int S, int H>
@@ -877,8 +829,7 @@ bool paged_mma_supported(const PagedDecodeArgs& a, int dim) {
 int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st, bool* taken) {
   MmaTables tb;
   memset(&tb, 0, sizeof(tb));
-  ScaledBook vb;
-  scale_book(a.v.cent.v, 1 << a.v.bits, &vb);
+  const ScaledBook vb = scaled_book(a.v.cent.v, 1 << a.v.bits);
   *taken = vb.good;
   if (!*taken) return TQ_OK;
   memcpy(tb.v_c16, vb.c16, sizeof(tb.v_c16));
@@ -889,8 +840,7 @@ int launch_paged_mma(PagedDecodeArgs a, cudaStream_t st, bool* taken) {
   a.kn_page_bytes = (uint32_t)(a.k.norm_page_stride * 4);
   a.vn_page_bytes = (uint32_t)(a.v.norm_page_stride * 4);
   if (a.k.format == TQ_KV_POLAR) {
-    ScaledBook kb;
-    scale_book(a.k.cent.v, 1 << a.k.bits, &kb);
+    const ScaledBook kb = scaled_book(a.k.cent.v, 1 << a.k.bits);
     *taken = kb.good;
     if (!*taken) return TQ_OK;
     memcpy(tb.k_c16, kb.c16, sizeof(tb.k_c16));
