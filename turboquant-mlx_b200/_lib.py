@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import warnings
 import weakref
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
@@ -197,14 +198,22 @@ def exported_symbols():
 
 
 native = None            # the extension module that makes the calls whose host time counts (csrc/calls.cpp)
+_native_absent = False   # it was looked for, not required, and not found
 
 
-def load_native():
-    """Load it (once), bound to the loaded libtqb200.so."""
-    global native
+def load_native(required: bool = True):
+    """Load it (once), bound to the loaded libtqb200.so.  Where it cannot be imported: RuntimeError, or None if it is not
+    required (after a warning)."""
+    global native, _native_absent
+    if _native_absent and not required:
+        return None
     try:
         from . import _calls
     except ImportError as e:
+        if not required:
+            _native_absent = True
+            warnings.warn(f"_calls.so cannot be loaded ({e}): calls take more host time, and the paged caches need it")
+            return None
         raise RuntimeError("_calls.so is missing or does not fit this torch: run make in the package folder") from e
     import sys
     _calls.bind(sys.modules[__name__], *[ctypes.cast(getattr(lib(), "tq_" + name), c_void_p).value for name in (

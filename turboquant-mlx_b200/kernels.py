@@ -699,8 +699,57 @@ def prefill_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.T
     window > 0 (causal only): the query at position i = row + S - L sees the keys in (i - window, i]
     and the first `sinks` ones; key tiles that nothing sees are skipped.  As in any masked matrix
     product, a hidden value row that is Inf or NaN still reaches rows that share a 128-key tile with it."""
+    native = _lib.native or _lib.load_native(required=False)
+    if native is None:
+        return _prefill_by_ctypes(queries, keys, values, scale, causal, out, window, sinks)
     status = _lib.workspace(16, queries.device, tag="prefill") if queries.is_cuda else queries
-    return (_lib.native or _lib.load_native()).prefill(queries, keys, values, scale, causal, out, window, sinks, status)
+    return native.prefill(queries, keys, values, scale, causal, out, window, sinks, status)
+
+
+def _prefill_by_ctypes(queries, keys, values, scale, causal, out, window, sinks):
+    """`prefill_attention` without the extension module: the same checks and the same kernel, 7 us more host time."""
+    _lib.require_cuda(queries, keys, values)
+    if queries.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("prefill_attention takes float16 or bfloat16 tensors")
+    if keys.dtype != queries.dtype or values.dtype != queries.dtype:
+        raise ValueError("queries, keys and values must share one dtype")
+    if queries.ndim != 4 or keys.ndim != 4 or values.ndim != 4:
+        raise ValueError("queries, keys and values must be (batch, heads, length, 128)")
+    B, n_q, L, D = queries.shape
+    n_kv, S = keys.shape[1:3]
+    if D != 128 or keys.shape[3] != 128 or values.shape[3] != 128:
+        raise ValueError(f"prefill_attention supports head_dim 128, got {D}")
+    if n_kv == 0 or n_q % n_kv:
+        raise ValueError(f"n_q_heads ({n_q}) must equal n_kv_heads ({n_kv}) * n_rep ({n_q // max(n_kv, 1)})")
+    if keys.shape[0] != B or values.shape != keys.shape:
+        raise ValueError("keys and values must have the same (batch, heads, length)")
+    if keys.device != queries.device or values.device != queries.device:
+        raise ValueError("queries, keys and values must be on one device")
+    if window < 0 or sinks < 0 or (sinks and not window) or (window and not causal):
+        raise ValueError(f"window ({window}) and sinks ({sinks}) must not be negative, sinks need a window, and a window "
+                         "needs causal attention")
+
+    def usable(t):
+        return t.stride(3) == 1 and not any(st % 8 for st in t.stride()[:3]) and t.data_ptr() % 16 == 0
+
+    q, k, v = (t if usable(t) else t.clone(memory_format=torch.contiguous_format) for t in (queries, keys, values))
+    if out is None:
+        out = torch.empty((B, n_q, L, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not usable(out):
+        raise ValueError(f"out must be {tuple(q.shape)} of the inputs' dtype on {q.device}, 16-byte aligned, with a "
+                         "contiguous last dimension")
+    with torch.cuda.device(q.device):
+        P = _lib.PrefillParams()
+        P.struct_bytes = ctypes.sizeof(P)
+        P.dtype, P.batch, P.n_q_heads, P.n_kv_heads, P.dim, P.seq_q, P.seq_k = _lib.dtype_code(q.dtype), B, n_q, n_kv, D, L, S
+        P.q, P.k, P.v, P.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        for name, t in (("q", q), ("k", k), ("v", v), ("o", out)):
+            setattr(P, name + "_strides", (ctypes.c_int64 * 3)(*t.stride()[:3]))
+        P.window, P.sinks, P.attn_scale, P.causal = min(window, 2 ** 62), min(sinks, 2 ** 62), float(scale), int(bool(causal))
+        P.status = _lib.workspace(16, q.device, tag="prefill").data_ptr()
+        P.stream = _lib.stream_handle(q.device)
+        _lib.check(_lib.lib().tq_prefill_sdpa_window(ctypes.byref(P)))
+    return out
 
 
 def prefill_status(device) -> int:
