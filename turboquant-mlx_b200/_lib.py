@@ -269,12 +269,23 @@ _host_cache: dict = {}     # id(tensor) -> (weak reference, tensor version, ctyp
 
 
 def _remember(t: torch.Tensor, arr) -> None:
+    if t.is_inference():       # no version: a change in place would go unseen
+        return
     key = id(t)
 
     def _evict(_ref, key=key):
         _host_cache.pop(key, None)
 
     _host_cache[key] = (weakref.ref(t, _evict), t._version, arr)
+
+
+def host_param(values, device) -> torch.Tensor:
+    """A small float32 device tensor (signs, centroids, boundaries) whose host copy is remembered: an ordinary tensor in
+    inference mode too."""
+    with torch.inference_mode(False):
+        t = torch.tensor(values, dtype=torch.float32, device=device)
+    register_host_values(t, values)
+    return t
 
 
 def register_host_values(t: torch.Tensor, values) -> None:
@@ -289,11 +300,12 @@ def host_floats(x):
     back once (this synchronises) and the copy is kept for as long as that tensor
     object lives and is not modified in place: the entry is keyed on the object
     itself (not its address, which the allocator hands to the next tensor of the
-    same size) and dropped when the tensor is freed."""
+    same size) and dropped when the tensor is freed.  Tensors made in
+    torch.inference_mode have no version and are read back by every call."""
     if x is None:
         return None
     if isinstance(x, torch.Tensor):
-        hit = _host_cache.get(id(x))
+        hit = _host_cache.get(id(x))                      # (no inference tensor is ever kept)
         if hit is not None and hit[0]() is x and hit[1] == x._version:
             return hit[2]
         vals = x.detach().to(torch.float32).reshape(-1).cpu().tolist()

@@ -38,20 +38,14 @@ def boundary_values(centroids: list) -> list:
     return [_f32((_f32(a) + _f32(b)) / 2.0) for a, b in zip(centroids[:-1], centroids[1:])]
 
 
-def _device_param(vals, device) -> torch.Tensor:
-    t = torch.tensor(vals, dtype=torch.float32, device=device)
-    _lib.register_host_values(t, vals)
-    return t
-
-
 def _compute_gaussian_codebook(bits: int, device=None) -> torch.Tensor:
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-    return _device_param(codebook_values(bits), device)
+    return _lib.host_param(codebook_values(bits), device)
 
 
 def _compute_gaussian_boundaries(centroids: torch.Tensor) -> torch.Tensor:
     vals = boundary_values(list(_lib.host_floats(centroids)))
-    return _device_param(vals, centroids.device)
+    return _lib.host_param(vals, centroids.device)
 
 
 class PolarQuantizer:

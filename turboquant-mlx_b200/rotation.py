@@ -33,9 +33,7 @@ def random_diagonal_sign(d: int, seed: int = 42, device=None) -> torch.Tensor:
     """(d,) float32 tensor of +/-1 on the current CUDA device."""
     vals = sign_values(d, seed)
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-    t = torch.tensor(vals, dtype=torch.float32, device=device)
-    _lib.register_host_values(t, vals)
-    return t
+    return _lib.host_param(vals, device)
 
 
 def _hadamard(x: torch.Tensor, pre, post, normalize: bool) -> torch.Tensor:
