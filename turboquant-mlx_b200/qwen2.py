@@ -114,16 +114,16 @@ class Qwen2Model:
 
     def decode_step(self, tok: torch.Tensor, caches, position: torch.Tensor) -> torch.Tensor:
         """One token per sequence, tok (B, 1), at the position held in the int32 device tensor
-        `position` (1,), or at one position per sequence (B,): logits (B, vocab).  Nothing here depends on a host-side length, so with caches
-        in static decode mode (`enable_static_decode`) the whole step can be captured in a CUDA graph
-        and replayed while the position advances on the device.  Same layer structure as `forward`,
+        `position` (one element), or at one position per sequence (B,): logits (B, vocab).  Nothing here
+        depends on a host-side length, so with caches in static decode mode (`enable_static_decode`) the
+        whole step can be captured in a CUDA graph and replayed while the position advances on the device.  Same layer structure as `forward`,
         with the projections that share an input fused (17 launches per layer instead of ~35)."""
         cfg = self.cfg
         B = tok.shape[0]
         D, nq, nkv = cfg.head_dim, cfg.n_q_heads, cfg.n_kv_heads
         half = D // 2
         x = self.emb[tok[:, 0]]
-        ang = position.to(torch.float32)[:, None, None] * self.inv_freq
+        ang = position.to(torch.float32).reshape(-1, 1, 1) * self.inv_freq
         cos, sin = ang.cos().to(x.dtype), ang.sin().to(x.dtype)
         scale = 1.0 / math.sqrt(D)
         for lw, cache in zip(self.layers, caches):
