@@ -53,11 +53,15 @@ ScaledBook scaled_book(const float* c, int n) {
   memset(&key, 0, sizeof(key));
   key.n = n;
   memcpy(key.c, c, n * sizeof(float));
-  std::lock_guard<std::mutex> lock(mu);
-  const auto hit = kept.find(key);
-  if (hit != kept.end()) return hit->second;
-  if (kept.size() >= kMost) kept.clear();
-  return kept[key] = search(c, n);
+  try {
+    std::lock_guard<std::mutex> lock(mu);
+    const auto hit = kept.find(key);
+    if (hit != kept.end()) return hit->second;
+    if (kept.size() >= kMost) kept.clear();
+    return kept[key] = search(c, n);
+  } catch (...) {                        // no memory to keep it; C callers are above, so nothing may be thrown
+    return search(c, n);
+  }
 }
 
 }  // namespace tq
