@@ -413,9 +413,10 @@ int tq_prefill_sdpa_window(const tq_prefill_params* p);
  * have the layout of the contiguous caches.  Pages may be shared between sequences;
  * entries behind a sequence, or wholly outside its window, are never read.  Lengths
  * and tables live on the device and are read when a kernel runs, so a captured step can
- * be replayed while they advance.  A page id outside the pool (or a position behind the
- * table) is never followed: an insert skips the row, a decode output row or a row read
- * back becomes NaN, and tq_paged_status reports it. */
+ * be replayed while they advance.  A page id outside the pool is never followed:
+ * an insert skips the row, a decode output row or a row read back becomes NaN, and
+ * tq_paged_status reports it.  A position behind the table: an insert skips the row and reports
+ * it; decode cuts a length to the table's capacity, read-back gives zeros, neither reports. */
 typedef struct tq_paged_half {   /* the keys or the values of a pool */
   int32_t format;                /* TQ_KV_POLAR or TQ_KV_DENSE */
   int32_t bits, dtype;           /* code width (polar); element type (dense) */

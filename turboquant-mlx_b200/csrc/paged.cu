@@ -49,6 +49,7 @@ __device__ __forceinline__ float2 fma2(float2 x, float y, float2 z) {
 //            rows, which lie in shared memory element by element, eight heads side by side
 //   values : lane = EPL consecutive elements; the 32 weights come back from shared memory
 // The warps of a CTA take the tiles of its run in turn and meet in shared memory at the end of a group.
+// (128 registers; at head_dim 256 it spills 296 bytes per thread.)
 // Bound by its shared-memory reads (two vectors of queries or weights and a centroid per element), hidden by 16 warps:
 // 32 sequences of 8192 tokens, 32 / 8 heads: 4-bit keys + 3-bit values 490 us (with 8 warps 1.7 times that), 16-bit keys
 // 475 us.
@@ -276,8 +277,8 @@ int launch_general(const PagedDecodeArgs& a, cudaStream_t st) {
 }
 
 // ---- page copies -------------------------------------------------------------------------------------------
-// HBM-bound, four 16-byte words per thread in flight: 1500 pages of 8 tensors, 395 MB read and written, 63 us = 6.3 TB/s
-// (0.96 of the copy peak).
+// HBM-bound, four 16-byte words per thread in flight: 1500 pages of 8 tensors, 381 MB read and written, 63 us = 6.05 TB/s
+// (0.93 of the copy peak).
 constexpr int kCopyPools = 128;          // pools per launch: their pointers travel as kernel parameters
 constexpr int kCopyUnit = 1024;          // 16-byte words a block moves per step: 4 per thread, all in flight
 struct CopyArgs {

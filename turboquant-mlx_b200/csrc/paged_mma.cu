@@ -1,10 +1,11 @@
 // Decode attention over pages on tensor cores: head_dim 128, 3 / 4-bit values, 16-bit dense or 3 / 4-bit keys.
 //
-// A CTA owns an equal run of the launch's tiles (paged.cuh) and W warps that share nothing but tables while they
-// stream it: warp w takes the tiles w, w + W, ... of a group, fetches each with four bulk copies (key rows, key norms,
-// value rows, value norms of 32 positions of one page) into a ring of its own, S tiles deep, and runs ahead into the
-// next group while it finishes this one.  The page id of the tile after next is already on its way when a copy is
-// issued, so the indirection costs no waiting.  Per tile, in one pass:
+// A CTA owns an equal run of the launch's tiles (paged.cuh), W consumer warps that share nothing but tables while they
+// stream it, and a producer warp.  Consumer w takes the tiles w, w + W, ... of a group from a ring of its own, S tiles
+// deep; lane w of the producer fills it with bulk copies (key rows, key norms, value rows, value norms of a tile: 32
+// positions with 16-bit keys, 64 with packed ones, of one page or of two pages of 32) and runs ahead into the next group
+// while this one is finished.  The page id of a ring's next tile is already on its way when a copy is issued, so the
+// indirection costs no waiting.  Per tile, in one pass:
 //   scores : mma m16n8k16, A = query (rows 0-7 the 16-bit high parts of 8 heads, rows 8-15 their residuals), B = K^T.
 //            Codes become 16-bit centroids two at a time through a table in shared memory, one copy per lane
 //            (entry * 256 + lane * 4): conflict free, and for 4-bit codes one byte permute makes the address.
@@ -17,8 +18,9 @@
 //
 // Measured at 32 sequences of 8192 tokens, 32 / 8 heads, pages of 64: 16-bit keys + 3-bit values 109 us = 5.9 TB/s (0.91 of
 // the copy peak: HBM-bound), 4 + 3 bits 93 us = 2.8 TB/s, 4 + 4 bits 82 us = 3.4 TB/s, 3 + 3 bits 90 us = 2.6 TB/s.  Packed
-// halves are bound inside the SM: instruction issue, the integer pipe, shared-memory loads and the tensor pipe are each
-// a little over half busy, and no reordering of one against the other has made the sum smaller.  One sequence of 433
+// halves are bound by latency inside the SM: two warps per scheduler (253 registers a thread) issue in 43 % of the cycles
+// (integer pipe 38 %, shared-memory loads 44 to 51 %, tensor pipe 24 %), and what lies between is a lookup behind its
+// address, a product behind its lookup, an exponential behind its product.  One sequence of 433
 // tokens: 10 us, of 32768 with 16-bit keys: 18 us, where starting (2.6 us), the warps' meeting (1.5 us) and the join of
 // the parts (5 us) are what is left beside the stream.
 //
@@ -724,7 +726,9 @@ paged_mma_kernel(const __grid_constant__ PagedDecodeArgs a, const __grid_constan
       }
     }
     consumer_barrier<W>();
-    gave_up = lds32(L::flag) != 0;   // read behind a barrier that every writer has passed: all warps agree
+    // Behind a barrier that every consumer has passed.  The producer, which also sets the flag, does not join it, so the
+    // warps may see its failure in this group or in the next: until then a warp waits (bounded) for tiles that do not come.
+    gave_up = lds32(L::flag) != 0;
     for (int r = warp; r < nr; r += W) {
       float mx = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
       uint32_t at[4];

@@ -157,8 +157,10 @@ __device__ __forceinline__ void butterfly_pairs(f2 (&v)[32], int q) {
 }
 
 // ---- insert of many tokens: head_dim 128, 3 / 4-bit codes (or 16-bit dense keys), 16-bit rows -----------------------
-// Instruction-bound in its exact 32-bit arithmetic (six prompts of up to 5000 tokens, 8 heads, 3-bit: 55 us = 1.8 TB/s),
-// so the work is cut to what the format asks for: two threads per vector, packed pairs (elements i and i + 32 of a
+// Six prompts of up to 5000 tokens, 8 heads, 3-bit: 59 us = 1.7 TB/s.  The exact 32-bit arithmetic (23 instructions per
+// element) is 26 us of that at full issue; the rest is latency, which 16 warps per SM at 128 registers (and 16 spilled
+// bytes per thread) do not cover, and half-rate instructions.  The work is cut to what the format asks for: two threads
+// per vector, packed pairs (elements i and i + 32 of a
 // thread's 64) for squares, division and butterfly, and one table lookup per code instead of a search: a monotone map
 // puts the rotated value into one of kBuckets buckets that hold at most one threshold each (the host makes sure), and the
 // bucket's entry says how many thresholds lie below and which one to compare with.  A copy of the table per lane: no
@@ -228,7 +230,7 @@ __device__ __forceinline__ void encode_tokens(const AppendHalf& s, const BucketM
   const float nrm = __fsqrt_rn(sum), safe = fmaxf(nrm, 1e-8f);
   if (safe < 1e30f) {
     // x / safe, correctly rounded: with a numerator of at most 11 bits one residual correction of x * RN(1 / safe) is
-    // enough (the quotient is at least 2^-13 ulp away from every rounding midpoint)
+    // enough (div_rn of quantize_fast.cu says why)
     const float y = __frcp_rn(safe);
     const f2 y2 = pack2(y, y), nb = pack2(-safe, -safe);
 #pragma unroll
@@ -524,8 +526,9 @@ paged_read_kernel(const ReadArgs a) {
 // 64).  The codes of such a pair are put side by side bit field by bit field, so that one table entry (a copy per half
 // warp lane: conflict free) is the packed pair of scaled centroids; the same butterfly, and ((x * s) * sign) * norm with
 // the sign applied to the rounded result (rounding is symmetric).  Rows leave through shared memory, so that every
-// store instruction covers two whole rows.  HBM-bound: 8 prefixes of up to 16384 tokens, 8 heads, 4-bit codes 65 us =
-// 4.75 TB/s (0.72 of the copy peak; a warp per row, 32-bit output: 282 us for 1.8 times the bytes).
+// store instruction covers two whole rows.  8 prefixes of up to 16384 tokens, 8 heads, 4-bit codes 67 us = 4.6 TB/s
+// (0.70 of the copy peak; a warp per row, 32-bit output: 282 us for 1.8 times the bytes): HBM, then the shared-memory pipe,
+// which the table, the butterfly's cross-thread stage and the output exchange have in common.
 constexpr int kReadRows = 16;
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kWarps * 32, 2)
@@ -732,7 +735,7 @@ extern "C" int tq_paged_append(const tq_paged_params* p) {
   a.counts = p->counts;
   cudaStream_t st = (cudaStream_t)p->stream;
   // From 16 tokens on a warp's worth of neighbouring rows exists: two threads per vector (six prompts of up to 5000
-  // tokens, 8 heads, 3-bit: 55 us against 184 with a warp per row).
+  // tokens, 8 heads, 3-bit: 59 us against 184 with a warp per row).
   const int64_t units = (int64_t)a.batch * a.heads * ((a.tokens + kSplitTokens - 1) / kSplitTokens);
   if (p->dim == 128 && a.tokens >= kSplitTokens && a.half[0].x_dtype == a.half[1].x_dtype && units < (1ll << 28)) {
     SplitArgs sp;

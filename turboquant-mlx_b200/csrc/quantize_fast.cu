@@ -43,11 +43,15 @@ struct FastQuantArgs {
 };
 
 // Correctly rounded a / b given y = RN(1 / b); a, b and the quotient in the normal
-// range.  One residual correction leaves an error below 2^-24 ulp.  When the
-// numerator has at most 11 significant bits (fp16 / bf16 inputs) the quotient is at
-// least 2^-13 ulp away from every rounding midpoint (|m 2^k - j b| >= 1 for the
-// integers involved), so the first correction already rounds correctly; a general
-// float32 numerator takes the second step.
+// range: Markstein's residual correction.  Scaled to a, b in [1, 2): |b y - 1| <= b 2^-25,
+// so q = RN(a y) is within 0.5 + a / 2 ulp of a / b and the corrected value, before it is
+// rounded, is off by |a / b - q| |b y - 1|.  Rounding it is wrong only if that passes a
+// midpoint m.  a - b m is a nonzero multiple of 2^-47 (2^-48 for a quotient below 1), so
+// a / b is d >= 2^-24 / b ulp away from m; while q is half an ulp from m, r is exact and the
+// error is (1/2 + d) b 2^-25 ulp, less than d since b < 2.  A numerator of at most 11
+// significant bits (fp16 / bf16 inputs) keeps q there (0.5 + a / 2 < 1.5 - 2^-11), so one
+// correction rounds correctly; a general float32 numerator may start 1.5 ulp away and takes a
+// second one.
 template <bool NARROW_NUMERATOR>
 __device__ __forceinline__ float div_rn(float a, float b, float y) {
   float q = __fmul_rn(a, y);
