@@ -28,11 +28,11 @@
 //     edge, the sinks' end or the diagonal crosses are masked per row; a row whose first tiles are masked whole keeps
 //     m = -inf and its P at zero until it sees a key.  The full form is compiled without any of it.
 // Measured: 32768 tokens causal, 28 / 4 heads, bf16: 1.33 PFLOP/s; 7000 tokens behind 1192 under a window of 2048 with 64
-// sinks: 208 to 217 us = 0.95 to 0.99 PFLOP/s in short runs of replays, 248 us = 0.83 under sustained load (one CTA per item, without the
-// overlap from item to item, the scores read twice and scalar arithmetic: 285 us against 208).  Of the products 15 % are
-// on pairs that the window, the sinks' end or the diagonal hides.  Without the softmax's arithmetic the latter takes 187 us, without most of the products
-// 113: what bounds it is the rate of 128 x 128 x 16 products, whose operands and the arriving tiles share the
-// bandwidth of shared memory.
+// sinks: 208 to 217 us = 0.95 to 0.99 PFLOP/s in short runs of replays, 248 us = 0.83 under sustained load (one CTA per
+// item, without the overlap from item to item, the scores read twice and scalar arithmetic: 285 us against 208).  Of its
+// products 15 % are on pairs that the window, the sinks' end or the diagonal hides.  Without the softmax's arithmetic it
+// takes 187 us, without most of the products 113: what bounds it is the rate of 128 x 128 x 16 products, whose operands
+// and the arriving tiles share the bandwidth of shared memory.
 //   * Every wait is bounded; a wait that gives up sets the status word, the CTA
 //     drains its copies, frees its tensor memory and returns.
 #include <cuda.h>
