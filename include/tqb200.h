@@ -54,6 +54,9 @@ typedef enum tq_kv_format {
 
 int tq_version(void);                      /* major * 10000 + minor * 100 + patch */
 const char* tq_last_error_string(void);    /* thread-local, never NULL */
+/* The capture `stream` is part of, a number that no other capture of the process has; 0: none.  Scratch
+ * whose zero fill is captured belongs to that capture's graph. */
+uint64_t tq_capture_id(void* stream);
 
 /* ---- fused quantize ------------------------------------------------------
  * Replaces fused_quantize (turboquant_mlx/metal.py:147-196) with the rounding

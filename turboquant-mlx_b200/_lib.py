@@ -12,7 +12,7 @@ import ctypes
 import os
 import warnings
 import weakref
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 import torch
 
@@ -122,6 +122,7 @@ _FP = POINTER(c_float)
 _SIGNATURES = {
     "tq_version": (c_int, []),
     "tq_last_error_string": (c_char_p, []),
+    "tq_capture_id": (c_uint64, [c_void_p]),
     "tq_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, _FP, _FP,
                             c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "tq_quantize_append": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, _FP, _FP,
@@ -320,20 +321,32 @@ def host_floats(x):
 # scratch memory: allocated by torch (the library never allocates), cached per
 # (device, stream) so stream-ordered reuse is safe
 # ---------------------------------------------------------------------------
-_workspaces: dict = {}
+_workspaces: dict = {}     # (tag, device, stream) -> tensor
+_captured: dict = {}       # (tag, device, stream) -> (capture, tensor) of the last capture on that stream
+
+
+def capture_id(stream: int) -> int:
+    """The capture a stream is part of, 0: none."""
+    return lib().tq_capture_id(stream)
 
 
 def workspace(nbytes: int, device, tag: str = "flash") -> torch.Tensor | None:
     """Zero-filled scratch tensor for one kind of call (`tag`): the flash-decode
     workspace starts with counters that must stay zero between calls, so other
-    kernels never share it."""
+    kernels never share it.  Calls in a capture share one per stream of that
+    capture: it comes from the graph's pool and every replay zeroes it."""
     if nbytes <= 0:
         return None
-    key = (tag, str(device), stream_handle(device))
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
+    stream = stream_handle(device)
+    key = (tag, str(device), stream)
+    capture = capture_id(stream)
+    made, ws = _captured.get(key, (0, None)) if capture else (0, _workspaces.get(key))
+    if ws is None or made != capture or ws.numel() < nbytes:
         ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-        _workspaces[key] = ws
+        if capture:
+            _captured[key] = capture, ws
+        else:
+            _workspaces[key] = ws
     return ws
 
 

@@ -88,3 +88,12 @@ int num_sms() {
 
 extern "C" int tq_version(void) { return 100; }  // 0.1.0
 extern "C" const char* tq_last_error_string(void) { return tq::g_err; }
+extern "C" uint64_t tq_capture_id(void* stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &st, &id) != cudaSuccess) {
+    cudaGetLastError();                        // another thread's capture forbids the question on the legacy stream
+    return 0;
+  }
+  return st == cudaStreamCaptureStatusNone ? 0 : id;
+}

@@ -307,8 +307,8 @@ def flash_decode(q: torch.Tensor, *, k=None, v=None, attn_scale: float, q_prerot
     workspace: a zero-initialised uint8 CUDA tensor owned by the caller and used by no other call
     that may be in flight together with this one (`decode_workspace` makes one; e.g. one per
     layer).  With kv_stable and q_stable such a call depends on nothing that is still running, so
-    consecutive decode launches overlap from start to end.  Without it the calls of a stream share
-    one workspace and each waits for its predecessor before writing it.  `workspace_owner`: any
+    consecutive decode launches overlap from start to end.  Without it the calls of a stream (the
+    calls of one capture on it) share one workspace and each waits for its predecessor before writing it.  `workspace_owner`: any
     object (a cache, say); its attribute `_decode_ws` holds such a workspace, made or grown here.
 
     gather (with partials=True and peers; see distributed.PeerExchange.gather_spec): after the
