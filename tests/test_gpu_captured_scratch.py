@@ -1,4 +1,6 @@
 """Decode and prompt calls captured in graphs: whose scratch they use."""
+import types
+
 import pytest
 import torch
 
@@ -43,3 +45,23 @@ def test_two_graphs_side_by_side(tq, dev):
         assert all(torch.equal(o, w) for o in outs[:5]) and torch.equal(outs[5], prompt)
     assert all(torch.equal(e, want[0]) for e in eager)
     assert tq.kernels.flash_status(dev, 2) == 0 and tq.kernels.prefill_status(dev) == 0
+
+
+def test_an_owner_first_seen_in_a_capture(tq, dev):
+    """The zero fill of a capture runs with the graph only, so what an eager call would use is not made there."""
+    call = _halves(tq, dev, 7)
+    want = call()
+    owner = types.SimpleNamespace(_decode_ws=None)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [call(workspace_owner=owner, kv_stable=True, q_stable=True) for _ in range(3)]
+    assert owner._decode_ws is None
+    assert torch.equal(call(workspace_owner=owner), want)
+    first = owner._decode_ws
+    assert first is not None
+    for _ in range(3):
+        g.replay()
+        assert torch.equal(call(workspace_owner=owner), want) and owner._decode_ws is first
+    assert all(torch.equal(o, want) for o in outs)
+    assert tq.kernels.workspace_status(first) == 0

@@ -505,8 +505,7 @@ def flash_decode(q: torch.Tensor, *, k=None, v=None, attn_scale: float, q_prerot
     if workspace is None and workspace_owner is not None:
         workspace = getattr(workspace_owner, "_decode_ws", None)
         if workspace is None or workspace.numel() < need or workspace.device != dev:
-            workspace = decode_workspace(dev, max(int(need), 1 << 20))
-            workspace_owner._decode_ws = workspace
+            workspace = _make_owned(workspace_owner, dev, max(int(need), 1 << 20), P.stream)
     if workspace is not None:
         _lib.require_cuda(workspace)
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
@@ -524,6 +523,20 @@ def flash_decode(q: torch.Tensor, *, k=None, v=None, attn_scale: float, q_prerot
     _lib.check(L.tq_flash_decode(ctypes.byref(P)))
     del keep
     return result
+
+
+def _make_owned(owner, dev, nbytes: int, stream: int) -> torch.Tensor:
+    """A decode workspace for `owner`, kept as its `_decode_ws`; in a capture one of that graph's, since the zero fill runs
+    with its replays only."""
+    capture = _lib.capture_id(stream)
+    if not capture:
+        owner._decode_ws = decode_workspace(dev, nbytes)
+        return owner._decode_ws
+    made, ws = getattr(owner, "_captured_ws", (0, None))
+    if made != capture or ws.numel() < nbytes or ws.device != dev:
+        ws = decode_workspace(dev, nbytes)
+        owner._captured_ws = capture, ws
+    return ws
 
 
 class FlashDecodePlan:
