@@ -49,19 +49,21 @@ def test_two_graphs_side_by_side(tq, dev):
 
 def test_an_owner_first_seen_in_a_capture(tq, dev):
     """The zero fill of a capture runs with the graph only, so what an eager call would use is not made there."""
+    # calls that overlap: each has an owner, and the geometry that overlapping calls take
     call = _halves(tq, dev, 7)
-    want = call()
-    owner = types.SimpleNamespace(_decode_ws=None)
+    stable = lambda owner: call(workspace_owner=owner, kv_stable=True, q_stable=True)
+    want = stable(types.SimpleNamespace(_decode_ws=None))
+    owners = [types.SimpleNamespace(_decode_ws=None) for _ in range(3)]
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
-        outs = [call(workspace_owner=owner, kv_stable=True, q_stable=True) for _ in range(3)]
-    assert owner._decode_ws is None
-    assert torch.equal(call(workspace_owner=owner), want)
-    first = owner._decode_ws
+        outs = [stable(o) for o in owners]
+    assert all(o._decode_ws is None for o in owners)
+    assert torch.equal(stable(owners[0]), want)
+    first = owners[0]._decode_ws
     assert first is not None
     for _ in range(3):
         g.replay()
-        assert torch.equal(call(workspace_owner=owner), want) and owner._decode_ws is first
+        assert torch.equal(stable(owners[0]), want) and owners[0]._decode_ws is first
     assert all(torch.equal(o, want) for o in outs)
     assert tq.kernels.workspace_status(first) == 0

@@ -308,8 +308,9 @@ def flash_decode(q: torch.Tensor, *, k=None, v=None, attn_scale: float, q_prerot
     that may be in flight together with this one (`decode_workspace` makes one; e.g. one per
     layer).  With kv_stable and q_stable such a call depends on nothing that is still running, so
     consecutive decode launches overlap from start to end.  Without it the calls of a stream (the
-    calls of one capture on it) share one workspace and each waits for its predecessor before writing it.  `workspace_owner`: any
-    object (a cache, say); its attribute `_decode_ws` holds such a workspace, made or grown here.
+    calls of one capture on it) share one workspace and each waits for its predecessor before
+    writing it.  `workspace_owner`: any object (a cache, say) whose calls do not overlap each other;
+    its attribute `_decode_ws` holds such a workspace, made or grown here.
 
     gather (with partials=True and peers; see distributed.PeerExchange.gather_spec): after the
     push the same launch waits (bounded) for every rank's rows in this GPU's own receive slot,
